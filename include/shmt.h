@@ -1,7 +1,8 @@
 /*
  * shmt.h — C ABI of libshmt.so: the GPU-cache hot path of ShmTensor
  * (static hashmap, cached feature fetch/set, cached neighbour sampling,
- * relabel, scan) as hand-written HIP for gfx950 (MI355X).
+ * relabel, scan) and a paged key/value cache held in 4 bits (plan, set, fetch,
+ * attention) as hand-written HIP for gfx950 (MI355X).
  *
  * Conventions
  *  - Every pointer is a raw address the GPU can dereference: device memory,
@@ -633,6 +634,121 @@ int shmt_subcsr_copy_rows(const void *indptr, const void *indices,
                           int seed_bytes, int64_t C, const void *cache_indptr,
                           const int64_t *row_begins, int64_t nnz,
                           void *cache_indices, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Paged key/value cache of a language model, held in 4 bits. No counterpart
+ * in the reference: its caches hold rows bit for bit (src/cache_feature_set.cu,
+ * src/cache_feature_fetch.cu), under slots that a map gives; here a row is
+ * rounded, and its slot comes from a block table.
+ *
+ * The cache is `pages` pages of `page` tokens. A slot s is place s % page of
+ * page s / page. For every token and head there are a key and a value of `dim`
+ * values each, as 4-bit floats (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6), the even dimension in the low half of a byte, and one
+ * power of two, 2^(byte - 127), for every 32 of them:
+ *   cache   uint8 [pages][kv_heads][2][page][dim / 2]   (keys 0, values 1)
+ *   scales  uint8 [pages][kv_heads][2][dim / 32][page]
+ * Pages may lie apart (page strides in bytes); everything within a page is
+ * contiguous. dim in {64, 128, 256}; page in {16, 32, 64, 128, 256}; addresses
+ * and page strides are multiples of 16. The struct is read by the call only.  */
+typedef struct shmt_paged_cache {
+  void *cache;
+  void *scales;
+  int64_t pages;
+  int64_t cache_page_stride;
+  int64_t scales_page_stride;
+  int kv_heads;
+  int dim;
+  int page;
+} shmt_paged_cache;
+
+/* Types of floating rows. */
+#define SHMT_F32 0
+#define SHMT_F16 1
+#define SHMT_BF16 2
+
+/* Block tables and slot maps of one step, from lengths that only the GPU need
+ * know. Request b holds cached_lens[b] tokens and gets new_lens[b] more
+ * (len_bytes in {4,8}; negative lengths count as 0). Its tokens fill its pages
+ * in order, so it needs ceil((cached + new) / page) - ceil(cached / page)
+ * further pages, which are taken from free_pages[0 .. n_free) in the order of
+ * the requests:
+ *   block_table[b, ceil(cached / page) + j] = the j-th of them   (in place)
+ *   query_starts[b] = new tokens of the requests before b        (requests + 1)
+ *   kv_lens[b] = cached + new
+ *   positions[t], slots[t] of new token t = query_starts[b] + i: its position
+ *     cached + i in the request, and its slot in the cache
+ *   counts[0], counts[1] = new tokens, pages needed
+ * Where the free pages run out or a request outgrows the table's `width`, the
+ * entry is -1 (within the width) and the slots of its tokens are -1: nothing
+ * is written there, and counts[1] > n_free tells. Tokens beyond max_tokens are
+ * not written (counts[0] > max_tokens tells); positions and slots behind the
+ * last token are -1, so the same buffers serve steps of any size. Rows of the
+ * table are table_stride entries apart. A request's length and the number of
+ * new tokens must be below 2^31. scratch: device memory of
+ * shmt_page_plan_scratch_bytes(requests) bytes, 8-byte aligned.             */
+int64_t shmt_page_plan_scratch_bytes(int64_t requests);
+int shmt_page_plan(const void *cached_lens, const void *new_lens,
+                   int len_bytes, int64_t requests, int32_t *block_table,
+                   int64_t width, int64_t table_stride,
+                   const int32_t *free_pages, int64_t n_free, int page,
+                   int64_t max_tokens, int32_t *query_starts, int32_t *kv_lens,
+                   int32_t *positions, int64_t *slots, int64_t *counts,
+                   void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Rounds n rows of keys and values [n, kv_heads, dim] (elem_type SHMT_F32,
+ * SHMT_F16 or SHMT_BF16; strides in elements, the values of a row contiguous,
+ * every row on 16 bytes) and writes them to their slots. Slots outside the
+ * cache (-1) are skipped; the same slot twice in one call leaves either row,
+ * or parts of both. The power of two of a block of 32 values is the smallest
+ * with max |x| < 7 * 2^e (e >= -127); values are rounded to the nearest code,
+ * ties to the even one, the sign of zero kept. A block that holds an infinity or NaN
+ * is marked (scale byte 255) and reads as NaN.                              */
+int shmt_page_set(const shmt_paged_cache *cache, const void *slots,
+                  int slot_bytes, int64_t n, const void *keys,
+                  int64_t key_token_stride, int64_t key_head_stride,
+                  const void *values, int64_t value_token_stride,
+                  int64_t value_head_stride, int elem_type, void *stream);
+/* The reverse: the values that the rows at `slots` stand for, rounded to
+ * elem_type, into contiguous keys and values [n, kv_heads, dim]. Rows of slots
+ * outside the cache are 0.                                                  */
+int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
+                    int slot_bytes, int64_t n, void *keys, void *values,
+                    int elem_type, void *stream);
+
+/* Attention over the cache. Request b's queries are rows query_starts[b] ..
+ * query_starts[b + 1) of `query` [tokens, heads, dim] (strides in elements, a
+ * row contiguous and on 16 bytes; SHMT_F16 or SHMT_BF16), and are the last of
+ * its kv_lens[b] tokens: row i has position p = kv_lens[b] - queries + i. With
+ * K, V the values that the cache holds for the request and head h / (heads /
+ * kv_heads),
+ *   out[row, h, :] = sum_j w_j V[j, :],  w = softmax_j(softmax_scale q . K[j])
+ * over the tokens j that the row sees:
+ *   j <= p,  and (window == 0 or j > p - window or j < sinks),
+ *   and block_table[b, j / page] is a page of the cache (not -1).
+ * A row that sees nothing, and a row of no request, is 0 with lse = -inf.
+ * What no row sees is not looked at for its value: it may be anything,
+ * infinities and NaN included. lse (may be NULL): float [tokens, heads],
+ * log(sum_j exp(softmax_scale q . K[j])), with which results over parts of the
+ * tokens can be joined. out: contiguous, of query's type. query_starts must
+ * not descend; starts and kv_lens are len_bytes in {4,8} wide. max_query_len:
+ * the most queries of a request, if known (0: not known): it only chooses the
+ * kernel. scratch: shmt_page_attention_scratch_bytes(...) bytes of device
+ * memory, 16-byte aligned, free again when the work queued has run. Sums and
+ * the softmax are held in 32 bits.                                          */
+int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads,
+                                          int kv_heads, int dim,
+                                          int64_t requests,
+                                          int64_t max_query_len);
+int shmt_page_attention(const shmt_paged_cache *cache, const void *query,
+                        int64_t query_token_stride, int64_t query_head_stride,
+                        int elem_type, int64_t tokens, int heads,
+                        const int32_t *block_table, int64_t width,
+                        int64_t table_stride, const void *query_starts,
+                        const void *kv_lens, int len_bytes, int64_t requests,
+                        float softmax_scale, int64_t window, int64_t sinks,
+                        int64_t max_query_len, void *out, float *lse,
+                        void *scratch, int64_t scratch_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -21,13 +21,14 @@ ORACLE_DIR = os.path.join(ROOT, "oracle")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "liboracle.so")
 
 HIP_SOURCES = ["hashmap.hip", "fetch.hip", "scan.hip", "relabel.hip", "sample.hip", "misc.hip",
-               "host_mem.hip", "errors.cc"]
+               "paged.hip", "paged_attention.hip", "host_mem.hip", "errors.cc"]
 
-MODULE_SOURCES = ["module.cc", "batch_driver.cc", "batch_sampler.cc", "host_tensors.cc"]
+MODULE_SOURCES = ["module.cc", "batch_driver.cc", "batch_sampler.cc", "host_tensors.cc", "paged_ops.cc"]
 
 # Packed-FP32 instruction selection is switched off for every HIP translation
-# unit (the kernels here do no floating-point arithmetic at all, rows are
-# moved as raw bytes).
+# unit: some of those instructions have given wrong results on this hardware.
+# (Only the paged key/value cache's kernels do floating-point arithmetic; all
+# others move rows as raw bytes.)
 HIPCC_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-Wno-unused-command-line-argument"]

@@ -83,12 +83,26 @@ SIGNATURES = {
     "shmt_subcsr_copy_rows": (_int, [_vp, _vp, _int, _int, _vp, _int, _i64, _vp, _vp, _i64, _vp, _vp]),
     "shmt_subcsr_plan": (_int, [_vp, _int, _vp, _int, _i64, _vp, _vp, _i64, _vp, _vp]),
     "shmt_subcsr_copy": (_int, [_vp, _vp, _int, _int, _vp, _int, _i64, _vp, _i64, _vp, _vp]),
+    "shmt_page_plan_scratch_bytes": (_i64, [_i64]),
+    "shmt_page_plan": (_int, [_vp, _vp, _int, _i64, _vp, _i64, _i64, _vp, _i64, _int, _i64, _vp, _vp, _vp, _vp, _vp,
+                              _vp, _i64, _vp]),
+    "shmt_page_set": (_int, [_vp, _vp, _int, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp]),
+    "shmt_page_fetch": (_int, [_vp, _vp, _int, _i64, _vp, _vp, _int, _vp]),
+    "shmt_page_attention_scratch_bytes": (_i64, [_i64, _int, _int, _int, _i64, _i64]),
+    "shmt_page_attention": (_int, [_vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _i64, _i64, _vp, _vp, _int, _i64,
+                                   _c.c_float, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
 }
 
 class HashmapLayout(_c.Structure):
     """shmt_hashmap_layout of include/shmt.h."""
     _fields_ = [("kind", _int), ("slot_bytes", _int), ("lo", _i64), ("span", _i64), ("delta", _i64),
                 ("table_bytes", _i64)]
+
+
+class PagedCache(_c.Structure):
+    """shmt_paged_cache of include/shmt.h: where a paged key/value cache lies and how it is laid out."""
+    _fields_ = [("cache", _vp), ("scales", _vp), ("pages", _i64), ("cache_page_stride", _i64),
+                ("scales_page_stride", _i64), ("kv_heads", _int), ("dim", _int), ("page", _int)]
 
 
 class HopJob(_c.Structure):

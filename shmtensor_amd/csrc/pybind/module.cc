@@ -6,7 +6,8 @@
 // torch's current HIP stream. Failures raise RuntimeError; nothing exits.
 // This file holds the reference's operators and the module definition; the
 // multi-batch driver is in batch_driver.cc, the graph-replaying sampler in
-// batch_sampler.cc, the host tensor providers in host_tensors.cc.
+// batch_sampler.cc, the host tensor providers in host_tensors.cc, the paged
+// key/value cache in paged_ops.cc.
 #include "shim.h"
 
 namespace shim {
@@ -486,6 +487,7 @@ PYBIND11_MODULE(ShmTensorLib, m) {
            py::arg("max_rows") = py::none(), py::arg("coo") = false);
 
   register_batch_sampler(m);
+  register_paged_ops(m);
 
   py::class_<StaticHashmap>(m, "CUCOStaticHashmap")
       .def(py::init<torch::Tensor, torch::Tensor, double, const std::string &>(), py::arg("keys"), py::arg("values"),

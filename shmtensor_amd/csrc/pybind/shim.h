@@ -352,6 +352,9 @@ std::vector<HopResult> sample_batch(const CsrArgs &g, torch::Tensor seeds, const
 // ---- graph-replaying sampler (batch_sampler.cc) ----
 void register_batch_sampler(py::module &m);
 
+// paged_ops.cc
+void register_paged_ops(py::module &m);
+
 }  // namespace shim
 
 // host tensor providers (host_tensors.cc)
