@@ -737,7 +737,7 @@ int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
  * memory, 16-byte aligned, free again when the work queued has run. Sums and
  * the softmax are held in 32 bits.                                          */
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads,
-                                          int kv_heads, int dim,
+                                          int kv_heads, int dim, int elem_type,
                                           int64_t requests,
                                           int64_t max_query_len);
 int shmt_page_attention(const shmt_paged_cache *cache, const void *query,

@@ -88,7 +88,7 @@ SIGNATURES = {
                               _vp, _i64, _vp]),
     "shmt_page_set": (_int, [_vp, _vp, _int, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp]),
     "shmt_page_fetch": (_int, [_vp, _vp, _int, _i64, _vp, _vp, _int, _vp]),
-    "shmt_page_attention_scratch_bytes": (_i64, [_i64, _int, _int, _int, _i64, _i64]),
+    "shmt_page_attention_scratch_bytes": (_i64, [_i64, _int, _int, _int, _int, _i64, _i64]),
     "shmt_page_attention": (_int, [_vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _i64, _i64, _vp, _vp, _int, _i64,
                                    _c.c_float, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
 }

@@ -178,7 +178,8 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
   if (tokens > 0) {
     query = rows_on_16(query);
     const int64_t scratch_bytes = shmt_page_attention_scratch_bytes(tokens, static_cast<int>(heads), c.kv_heads, c.dim,
-                                                                    n, max_query_len);
+                                                                    elem_type(query.scalar_type(), "query"), n,
+                                                                    max_query_len);
     TORCH_CHECK(scratch_bytes >= 0, shmt_last_error());
     torch::Tensor scratch = device_bytes(scratch_bytes);
     const float scale = softmax_scale ? static_cast<float>(*softmax_scale)
