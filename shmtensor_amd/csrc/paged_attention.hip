@@ -17,49 +17,68 @@ struct AttnArgs {
   int64_t tokens;
   int heads, group;
   const int32_t *table;
-  int64_t width, table_stride;
+  int64_t table_stride;
   const void *starts, *kv_lens;
   int len_bytes;
   int64_t requests;
   float scale;
-  int64_t window, sinks;
+  int32_t window, sinks;
+  int32_t limit;  // tokens that a row of the table has room for
   void *out;
   float *lse;
 };
 
-// What a workgroup left for the join: the item it finished that other workgroups had begun.
+// ---- items and units -------------------------------------------------------------
+// An item is up to kRows rows against one head of the cache: a row is a query token and a head of the group that shares the
+// cache's head, row r of a request being token r / group, head r % group. The tokens that an item's rows see are cut at
+// multiples of kUnit: the tiles that hold first tokens ("sinks"), then those from the window's begin to the last row's own
+// place. Units are numbered head by head, request by request, row tile by row tile; workgroup w of G takes units
+// floor(w U / G) up to floor((w + 1) U / G), so all end at about the same time whatever the lengths are. An item may be
+// shared by several workgroups; each leaves a part (maximum, sum, weighted values), which page_attention_join_kernel puts
+// together.
+constexpr int kUnit = 128;  // tokens: four waves of 32
+constexpr int kWaveTokens = 32;
+constexpr float kNothing = -__builtin_inff();
+constexpr float kLowest = -3.0e38f;  // subtracted instead of kNothing, so that nothing stays nothing
+
+struct AttnItem {
+  int64_t unit;  // units of one head in front of it
+  int32_t request, row0;
+};
+
+// What a workgroup left for the join: the item that it finished and others had begun.
 struct JoinRecord {
   int32_t first;  // the workgroup that began the item; -1: nothing to join
   int32_t head;   // of the cache
   int32_t rows;
-  int32_t row0;       // the item's first row, counted (token, head of the group) from the request's first query
+  int32_t row0;
   int64_t first_row;  // the request's first row of `query`
 };
-
-// ---- items and units -------------------------------------------------------------
-// An item is kRows rows (queries of one request, all heads of one group: row r is token r / group, head r % group) against one head of
-// the cache. Its tokens are cut at multiples of kUnit: the tiles that hold first tokens ("sinks") that are seen,
-// then those from the window's begin to the last row's own place. Units are numbered request by request, head by
-// head, row tile by row tile; workgroup w of G takes units floor(w U / G) up to floor((w + 1) U / G), so all end at
-// the same time whatever the lengths are, and an item may be shared by several workgroups, each of which leaves a
-// part (maximum, sum, weighted values) that page_attention_join_kernel puts together.
-constexpr int kUnit = 128;      // tokens: four waves of 32
-constexpr int kWaveTokens = 32;
 
 struct Request {
   int64_t first_row;  // of `query`
   int32_t queries;
-  int32_t before;     // tokens in front of the first query (may be negative: then the first rows see nothing)
-  int32_t limit;      // tokens that the table has room for
+  int32_t before;  // tokens in front of the first query; negative: the first rows see nothing
 };
 
 struct Span {
   int32_t sink_tiles;  // tiles 0 .. sink_tiles
   int32_t tile0;       // then tiles from here
   int32_t units;
-  int32_t sink_end;    // tokens below this are seen as sinks by every row that has them outside of its window
-  int32_t begin, end;  // tokens [begin, end) and [0, sink_end) are all that any row of the item sees
+  int32_t sink_end;    // tokens [0, sink_end) and [begin, end) are all that any row of the item sees
+  int32_t begin, end;
 };
+
+// A value that is the same for the whole wave, as the compiler cannot tell of what came from memory: held once, not per lane.
+__device__ __forceinline__ int same(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t same(int64_t v) {
+  const uint32_t lo = same(static_cast<int>(v)), hi = same(static_cast<int>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ Request same(Request r) { return {same(r.first_row), same(r.queries), same(r.before)}; }
+__device__ __forceinline__ Span same(Span s) {
+  return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.sink_end), same(s.begin), same(s.end)};
+}
 
 __device__ __forceinline__ Request attn_request(const AttnArgs &a, int64_t b) {
   int64_t lo, hi;
@@ -71,34 +90,79 @@ __device__ __forceinline__ Request attn_request(const AttnArgs &a, int64_t b) {
   r.first_row = lo;
   r.queries = static_cast<int32_t>(hi - lo);
   r.before = static_cast<int32_t>(min(max(len, int64_t{0}), int64_t{0x7fffffff}) - (hi - lo));
-  r.limit = a.v.pages > 0 ? static_cast<int32_t>(a.width << a.v.log2_page) : 0;
   return r;
 }
 
 template <int ROWS>
-__device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, int64_t row0) {
-  const int64_t all = static_cast<int64_t>(r.queries) * a.group;
-  const int32_t t_first = static_cast<int32_t>(row0 / a.group);
-  const int32_t t_last = static_cast<int32_t>((min(row0 + ROWS, all) - 1) / a.group);
+__device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, int row0) {
+  const int all = r.queries * a.group;
+  const int t_first = static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group));
+  const int t_last =
+      static_cast<int>(static_cast<uint32_t>(min(row0 + ROWS, all) - 1) / static_cast<uint32_t>(a.group));
   Span s;
-  s.end = max(min(r.before + t_last + 1, r.limit), 0);
-  s.begin = 0;
-  if (a.window > 0) s.begin = static_cast<int32_t>(max(min(int64_t{r.before} + t_first + 1 - a.window, int64_t{s.end}), int64_t{0}));
+  s.end = max(min(r.before + t_last + 1, a.limit), 0);
+  s.begin = a.window > 0 ? max(min(max(r.before + t_first, -1) - a.window + 1, s.end), 0) : 0;
   s.tile0 = s.begin / kUnit;
-  s.sink_end = static_cast<int32_t>(min(a.sinks, int64_t{s.begin}));
+  s.sink_end = min(a.sinks, s.begin);
   s.sink_tiles = min((s.sink_end + kUnit - 1) / kUnit, s.tile0);
   s.units = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1);
   return s;
 }
 
-// Units of request b for one head.
+// Units of a request for one head.
 template <int ROWS>
 __device__ __forceinline__ int64_t attn_units(const AttnArgs &a, const Request &r) {
   int64_t n = 0;
-  const int64_t all = static_cast<int64_t>(r.queries) * a.group;
-  for (int64_t row0 = 0; row0 < all; row0 += ROWS) n += attn_span<ROWS>(a, r, row0).units;
+  const int all = r.queries * a.group;
+  for (int row0 = 0; row0 < all; row0 += ROWS) n += attn_span<ROWS>(a, r, row0).units;
   return n;
 }
+
+// Items of all requests with the units in front of each, for calls in which a request has many row tiles: one workgroup.
+// items[0 .. n) and, behind the last, the number of units; *count = n. (Only starts that descend could make more items than
+// there is room for.)
+template <int ROWS>
+__global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, int32_t *first_item, AttnItem *items,
+                                                                    int64_t room, int32_t *count) {
+  __shared__ uint64_t lds[16];
+  int64_t n = 0;
+  for (int64_t base = 0; base < a.requests; base += 1024) {
+    const int64_t b = base + threadIdx.x;
+    int64_t mine = 0;
+    if (b < a.requests) mine = (attn_request(a, b).queries * a.group + ROWS - 1) / ROWS;
+    uint64_t sum;
+    const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
+    if (b < a.requests) first_item[b] = static_cast<int32_t>(n + at);
+    n += sum;
+  }
+  n = min(n, room);
+  __syncthreads();
+  int64_t units = 0;
+  for (int64_t base = 0; base < n; base += 1024) {
+    const int64_t i = base + threadIdx.x;
+    int64_t mine = 0, lo = 0;
+    int row0 = 0;
+    if (i < n) {
+      int64_t hi = a.requests - 1;  // the last request whose first item is i or before it
+      while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) >> 1;
+        if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      row0 = static_cast<int>(i - first_item[lo]) * ROWS;
+      mine = attn_span<ROWS>(a, attn_request(a, lo), row0).units;
+    }
+    uint64_t sum;
+    const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
+    if (i < n) items[i] = AttnItem{units + at, static_cast<int32_t>(lo), row0};
+    units += sum;
+  }
+  if (threadIdx.x == 0) {
+    items[n] = AttnItem{units, 0, 0};
+    *count = static_cast<int32_t>(n);
+  }
+}
+
+// ---- arithmetic of a tile ------------------------------------------------------------
 
 // x of this lane and of the lane 32 (16) further on: the swap instructions exchange halves (odd and even quarters) of two
 // registers.
@@ -152,31 +216,43 @@ struct KvTile {
   uint32_t value_scale[2];  // a byte for each of the four tokens
 };
 
-// Loads the 16 tokens at place `off` of page `at`.
+// Where a lane's pieces lie behind the first of 16 tokens of a page; the rest of an address is the same for the wave.
+struct LaneOffsets {
+  uint32_t key, key_scale, value, value_scale;
+};
 template <int DIM>
-__device__ __forceinline__ void load_half(const PagedView &v, int head, int64_t at, int off, int lane, int half,
-                                          KvTile<DIM> &t) {
+__device__ __forceinline__ LaneOffsets lane_offsets(int lane, int page) {
   const int m = lane & 15, g = lane >> 4;
-  const int page = 1 << v.log2_page;
-  const uint8_t *tile = v.cache + at * v.cache_stride + (static_cast<int64_t>(head) * 2 << v.log2_page) * (DIM / 2);
-  const uint8_t *sc = v.scales + at * v.scales_stride + (static_cast<int64_t>(head) * 2 << v.log2_page) * (DIM / 32);
-  const uint8_t *k = tile + (off + m) * (DIM / 2) + g * (DIM / 8);
+  LaneOffsets o;
+  o.key = m * (DIM / 2) + g * (DIM / 8);
+  o.key_scale = (DIM == 64 ? g >> 1 : g * (DIM / 128)) * page + m;
+  o.value = (page + 4 * g) * (DIM / 2) + m * (DIM / 32);
+  o.value_scale = (DIM / 32 + m * (DIM / 16) / 32) * page + 4 * g;
+  return o;
+}
+
+// Loads the 16 tokens at place `off` of page `at` (both the same for the wave).
+template <int DIM>
+__device__ __forceinline__ void load_half(const PagedView &v, int head, int at, int off, const LaneOffsets &o, int half,
+                                          KvTile<DIM> &t) {
+  const int64_t tile = int64_t{2} * head << v.log2_page;
+  const uint8_t *rows = v.cache + at * v.cache_stride + (tile + off) * (DIM / 2);
+  const uint8_t *sc = v.scales + at * v.scales_stride + tile * (DIM / 32) + off;
   if constexpr (DIM == 64) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(k);
+    const uint2 x = *reinterpret_cast<const uint2 *>(rows + o.key);
     t.key[half][0] = x.x, t.key[half][1] = x.y;
-    t.key_scale[half][0] = sc[(g >> 1) * page + off + m];
+    t.key_scale[half][0] = sc[o.key_scale];
   } else {
 #pragma unroll
     for (int i = 0; i < DIM / 128; ++i) {
-      const uint4 x = reinterpret_cast<const uint4 *>(k)[i];
+      const uint4 x = reinterpret_cast<const uint4 *>(rows + o.key)[i];
       t.key[half][4 * i] = x.x, t.key[half][4 * i + 1] = x.y, t.key[half][4 * i + 2] = x.z, t.key[half][4 * i + 3] = x.w;
-      t.key_scale[half][i] = sc[(g * (DIM / 128) + i) * page + off + m];
+      t.key_scale[half][i] = sc[o.key_scale + (i << v.log2_page)];
     }
   }
-  const uint8_t *val = tile + (page + off + 4 * g) * (DIM / 2) + m * (DIM / 32);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const uint8_t *p = val + r * (DIM / 2);
+    const uint8_t *p = rows + o.value + r * (DIM / 2);
     if constexpr (DIM == 64) t.value[half][r][0] = *reinterpret_cast<const uint16_t *>(p);
     else if constexpr (DIM == 128) t.value[half][r][0] = *reinterpret_cast<const uint32_t *>(p);
     else {
@@ -184,8 +260,7 @@ __device__ __forceinline__ void load_half(const PagedView &v, int head, int64_t 
       t.value[half][r][0] = x.x, t.value[half][r][1] = x.y;
     }
   }
-  t.value_scale[half] =
-      *reinterpret_cast<const uint32_t *>(sc + (DIM / 32 + m * (DIM / 16) / 32) * page + off + 4 * g);
+  t.value_scale[half] = *reinterpret_cast<const uint32_t *>(sc + o.value_scale);
 }
 
 // Softmax state and weighted values of NT x 16 rows: lane (n, g) has row n of each 16, and the dimensions
@@ -196,7 +271,32 @@ struct RowState {
   f32x4 acc[NT][DIM / 16];
 };
 
-constexpr float kNothing = -__builtin_inff();
+// Queries of an item, as the right operand of K Q^T: fragment i of 16 rows holds, for lane (n, g), eight dimensions of
+// row n from g * DIM / 4 + 8 i on. They stay in registers where they are few, else in LDS, where the four waves share them.
+template <int DIM, int NT, int PARTS>
+struct Queries {
+  static constexpr int kFrags = PARTS * NT * (DIM / 32);
+  static constexpr bool kShared = kFrags > 8;
+  u32x4 own[kShared ? 1 : kFrags];
+  const u32x4 *shared;
+  __device__ __forceinline__ u32x4 at(int part, int n, int i, int lane) const {
+    const int f = (part * NT + n) * (DIM / 32) + i;
+    if constexpr (kShared) return shared[f * kWave + lane];
+    else return own[f];
+  }
+};
+
+// Which tokens of a tile the rows of a lane see.
+template <int NT>
+struct Sight {
+  int last[NT];   // tokens up to here ...
+  int after[NT];  // ... from behind here, or
+  int sinks;      // before here
+  int begin, end, sink_end;  // no row of the item sees any outside of [begin, end) and [0, sink_end)
+};
+
+// Scale bytes from here on make values that are infinite in bfloat16, or not a number.
+constexpr uint32_t kWild = 253;
 
 // One wave's step over 32 tokens.
 //   S^T = K Q^T, 16 tokens x 16 rows at a time: lane (n, g) gets the scores of row n with tokens 4g .. 4g + 3, which is
@@ -205,50 +305,60 @@ constexpr float kNothing = -__builtin_inff();
 // Keys and values become bfloat16 exactly. The weights of float16 queries are held as the sum of two bfloat16 (16 bits), as
 // are the queries themselves; with bfloat16 queries the weights are rounded to bfloat16, an error of the size of the
 // result's own rounding.
-template <int DIM, int NT, int PARTS, bool MASKED>
-__device__ __forceinline__ void attend_tile(const AttnArgs &a, const KvTile<DIM> &t, const u32x4 (&q)[PARTS][NT][DIM / 32],
-                                            RowState<DIM, NT> &st, float scale2, int lane, int token0, const bool (&there)[2],
-                                            const int (&pos)[NT], int limit) {
+// `whole`: all rows see all tokens. Otherwise scores are masked; and values that are not finite in bfloat16 must not meet the
+// weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
+template <int DIM, int NT, int PARTS>
+__device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
+                                            float scale2, int lane, bool whole, int token0, bool there0, bool there1,
+                                            const Sight<NT> &sight, bool &wild) {
   const int g = lane >> 4;
   f32x4 s[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int i = 0; i < DIM / 32; ++i) {
+    u32x4 k[2];
 #pragma unroll
-    for (int i = 0; i < DIM / 32; ++i) {
+    for (int half = 0; half < 2; ++half) {
       const float f = scale_operand(t.key_scale[half][i / 4]);
       const uint32_t c = t.key[half][i];
-      const u32x4 k = {decode2_bf16<0>(c, f), decode2_bf16<1>(c, f), decode2_bf16<2>(c, f), decode2_bf16<3>(c, f)};
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) s[n][half] = mfma(k, q[p][n][i], s[n][half]);
+      k[half] = u32x4{decode2_bf16<0>(c, f), decode2_bf16<1>(c, f), decode2_bf16<2>(c, f), decode2_bf16<3>(c, f)};
     }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const u32x4 x = q.at(p, n, i, lane);
+        s[n][0] = mfma(k[0], x, s[n][0]);
+        s[n][1] = mfma(k[1], x, s[n][1]);
+      }
   }
-  u32x4 w[PARTS][NT];
-  float seen[NT][8];  // MASKED: the weights, -1 where the row does not see the token
-  bool grows = false;
+  if (!whole) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
+        const bool sees = (j < 4 ? there0 : there1) && token <= sight.last[n] &&
+                          (token > sight.after[n] || token < sight.sinks);
+        s[n][j / 4][j % 4] = sees ? s[n][j / 4][j % 4] : kNothing;
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if ((t.value_scale[j / 4] >> (8 * (j % 4)) & 255u) >= kWild) {
+        const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
+        t.value_scale[j / 4] &= ~(255u << (8 * (j % 4)));
+        wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
+      }
+  }
   float most[NT];
+  bool grows = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float x = kNothing;
+    float x = s[n][0][0];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = s[n][half][r] * scale2;
-        if constexpr (MASKED) {
-          const int j = token0 + 16 * half + 4 * g + r;
-          const bool sees = there[half] && j <= pos[n] && j < limit &&
-                            (a.window == 0 || int64_t{j} > int64_t{pos[n]} - a.window || j < a.sinks);
-          v = sees ? v : kNothing;
-          seen[n][4 * half + r] = sees ? 0.0f : -1.0f;
-        }
-        s[n][half][r] = v;
-        x = fmaxf(x, v);
-      }
-    most[n] = across_max(x);
+    for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n][j / 4][j % 4]);
+    most[n] = across_max(x) * scale2;
     grows |= most[n] > st.top[n] + 8.0f;
   }
   // The running maximum moves only where a weight would pass 2^8 (the first one always does).
@@ -256,74 +366,37 @@ __device__ __forceinline__ void attend_tile(const AttnArgs &a, const KvTile<DIM>
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float next = fmaxf(st.top[n], most[n]);
-      const float f = __builtin_amdgcn_exp2f(st.top[n] - fmaxf(next, -3.0e38f));
+      const float f = __builtin_amdgcn_exp2f(st.top[n] - fmaxf(next, kLowest));
       st.top[n] = next;
       st.sum[n] *= f;
 #pragma unroll
       for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] *= f;
     }
   }
+  u32x4 w[PARTS][NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float base = fmaxf(st.top[n], -3.0e38f);
-    float e[8];
+    const float base = fmaxf(st.top[n], kLowest);
+    float e[8], sum = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = __builtin_amdgcn_exp2f(s[n][j / 4][j % 4] - base);
-      st.sum[n] += e[j];
-      if constexpr (MASKED) seen[n][j] = seen[n][j] < 0 ? -1.0f : e[j];
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j / 4][j % 4], scale2, -base));
+      sum += e[j];
     }
+    st.sum[n] += sum;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t hi = pack_bf16(e[2 * j], e[2 * j + 1]);
       w[0][n][j] = hi;
       if constexpr (PARTS == 2)
-        w[1][n][j] = pack_bf16(e[2 * j] - __builtin_bit_cast(float, hi << 16),
-                               e[2 * j + 1] - __builtin_bit_cast(float, hi & 0xffff0000u));
+        w[1][n][j] = pack_bf16(e[2 * j] - __uint_as_float(hi << 16), e[2 * j + 1] - __uint_as_float(hi & 0xffff0000u));
     }
   }
-  uint32_t vs[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) vs[j] = (t.value_scale[j / 4] >> (8 * (j % 4))) & 255u;
-  if constexpr (MASKED) {
-    // Values that are not finite in bfloat16 must not meet the weight 0 of a row that does not see them: they are taken
-    // out of the product (their scale becomes the smallest) and added for the rows that do see them, one token at a time.
-    bool wild = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) wild |= vs[j] >= 253u;
-    if (__ballot(wild)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        for (int gt = 0; gt < 4; ++gt) {
-          if (!(__ballot(vs[j] >= 253u) >> (16 * gt) & 0xffffull)) continue;
-          float p[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) p[n] = __shfl(seen[n][j], (lane & 15) + 16 * gt);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int from = 4 * g + r + 16 * gt;
-            const uint32_t byte = static_cast<uint32_t>(__shfl(static_cast<int>(vs[j]), from));
-#pragma unroll
-            for (int word = 0; word < KvTile<DIM>::kValueWords; ++word) {
-              const uint32_t c = static_cast<uint32_t>(__shfl(static_cast<int>(t.value[j / 4][j % 4][word]), from));
-              const float f = scale_operand(byte);
-              const f32x2 x[4] = {decode2_f32<0>(c, f), decode2_f32<1>(c, f), decode2_f32<2>(c, f), decode2_f32<3>(c, f)};
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < (DIM == 64 ? 4 : 8); ++i)
-                  if (byte >= 253u && p[n] >= 0) st.acc[n][8 * word + i][r] += p[n] * x[i / 2][i % 2];
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) vs[j] = vs[j] >= 253u ? 0u : vs[j];
-    }
-  }
+  // The conversion reads nothing of a scale but its exponent field, so the byte need not be cut out.
   float f[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = scale_operand(vs[j]);
+  for (int j = 0; j < 8; ++j)
+    f[j] = __uint_as_float(j % 4 == 3 ? t.value_scale[j / 4] >> 1 : t.value_scale[j / 4] << (23 - 8 * (j % 4)));
 #pragma unroll
   for (int word = 0; word < KvTile<DIM>::kValueWords; ++word) {
     auto two = [&](auto byte) {  // dimensions 2 B and 2 B + 1 of this lane's
@@ -354,6 +427,23 @@ __device__ __forceinline__ void attend_tile(const AttnArgs &a, const KvTile<DIM>
   }
 }
 
+// q . K[j] of one row and token, element by element.
+template <typename T, int DIM>
+__device__ float score_of(const T *q, const uint8_t *codes, const uint8_t *scales, int page) {
+  float s = 0;
+#pragma unroll 1
+  for (int p = 0; p < DIM / 8; ++p) {
+    const uint32_t c = reinterpret_cast<const uint32_t *>(codes)[p];
+    const float f = scale_operand(scales[p / 4 * page]);
+    const f32x2 x[4] = {decode2_f32<0>(c, f), decode2_f32<1>(c, f), decode2_f32<2>(c, f), decode2_f32<3>(c, f)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += static_cast<float>(q[8 * p + i]) * x[i / 2][i % 2];
+  }
+  return s;
+}
+
+// ---- the kernel ------------------------------------------------------------------------
+
 // What the waves of a workgroup exchange at the end of an item.
 template <int DIM>
 struct JoinShared {
@@ -362,15 +452,23 @@ struct JoinShared {
   float top[4][16], sum[4][16];
 };
 
+// Waves per SIMD that the registers are meant for.
+constexpr int attn_waves(int dim, int tiles) { return tiles * dim <= 128 ? 3 : tiles * dim <= 512 ? 2 : 1; }
+
 template <typename T, int DIM, int NT>
-__global__ __launch_bounds__(256, NT * DIM <= 128 ? 4 : NT * DIM <= 256 ? 2 : 1) void page_attention_kernel(
-    AttnArgs a, float *parts, float *part_stats, JoinRecord *records) {
+__global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kernel(
+    AttnArgs a, const AttnItem *items, const int32_t *item_count, float *parts, float *part_stats, JoinRecord *records) {
   constexpr int kRows = 16 * NT;
-  constexpr int kParts = sizeof(T) == 2 && std::is_same<T, _Float16>::value ? 2 : 1;
-  __shared__ JoinShared<DIM> shared;
-  __shared__ int64_t scan[4];
+  constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
+  using Q = Queries<DIM, NT, kParts>;
+  union Shared {
+    JoinShared<DIM> join;
+    u32x4 queries[Q::kShared ? Q::kFrags * kWave : 1];
+    uint64_t scan[4];
+  };
+  __shared__ Shared shared;
   __shared__ int64_t found[2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
   const int kv_heads = a.v.kv_heads;
 
@@ -381,91 +479,138 @@ __global__ __launch_bounds__(256, NT * DIM <= 128 ? 4 : NT * DIM <= 256 ? 2 : 1)
       row_lo = min(max(load_int(a.starts, 0, a.len_bytes), int64_t{0}), a.tokens);
       row_hi = min(max(load_int(a.starts, a.requests, a.len_bytes), row_lo), a.tokens);
     }
-    const int64_t row16 = static_cast<int64_t>(a.heads) * DIM / 8;  // pieces of 16 bytes
     const int64_t none = row_lo + a.tokens - row_hi;
-    for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * row16; i += int64_t{gridDim.x} * 256) {
-      const int64_t row = i / row16;
-      reinterpret_cast<uint4 *>(a.out)[(row < row_lo ? row : row - row_lo + row_hi) * row16 + i % row16] = uint4{0, 0, 0, 0};
-    }
-    if (a.lse)
-      for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * a.heads; i += int64_t{gridDim.x} * 256) {
-        const int64_t row = i / a.heads;
-        a.lse[(row < row_lo ? row : row - row_lo + row_hi) * a.heads + i % a.heads] = kNothing;
+    if (none > 0) {
+      const int64_t row16 = static_cast<int64_t>(a.heads) * DIM / 8;  // pieces of 16 bytes
+      for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * row16; i += int64_t{gridDim.x} * 256) {
+        const int64_t row = i / row16;
+        reinterpret_cast<uint4 *>(a.out)[(row < row_lo ? row : row - row_lo + row_hi) * row16 + i % row16] =
+            uint4{0, 0, 0, 0};
       }
+      if (a.lse)
+        for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * a.heads; i += int64_t{gridDim.x} * 256) {
+          const int64_t row = i / a.heads;
+          a.lse[(row < row_lo ? row : row - row_lo + row_hi) * a.heads + i % a.heads] = kNothing;
+        }
+    }
   }
 
-  // This workgroup's units: each thread counts a run of requests.
-  const int64_t each = (a.requests + 255) / 256;
-  const int64_t b_lo = min(threadIdx.x * each, a.requests), b_hi = min(b_lo + each, a.requests);
-  int64_t mine = 0;
-  for (int64_t b = b_lo; b < b_hi; ++b) mine += attn_units<kRows>(a, attn_request(a, b)) * kv_heads;
-  uint64_t total;
-  const int64_t at = static_cast<int64_t>(
-      block_exclusive_scan<uint64_t, 256>(static_cast<uint64_t>(mine), reinterpret_cast<uint64_t *>(scan), &total));
-  const int64_t U = static_cast<int64_t>(total);
+  // Where this workgroup's units begin: in the list of items, or, without one, by counting: each thread a run of requests.
+  int64_t per_head, mine = 0, at = 0, each = 0, b_lo = 0;
+  if (items) {
+    per_head = same(items[same(*item_count)].unit);
+  } else {
+    each = (a.requests + 255) / 256;
+    b_lo = min(threadIdx.x * each, a.requests);
+    const int64_t b_hi = min(b_lo + each, a.requests);
+    for (int64_t b = b_lo; b < b_hi; ++b) mine += attn_units<kRows>(a, attn_request(a, b));
+    uint64_t total;
+    at = static_cast<int64_t>(block_exclusive_scan<uint64_t, 256>(static_cast<uint64_t>(mine), shared.scan, &total));
+    per_head = same(static_cast<int64_t>(total));
+  }
+  const int64_t U = per_head * kv_heads;
   // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same pages. With fewer
   // units than workgroups each has one, on all XCDs.
   const int64_t G = min(int64_t{gridDim.x}, U);
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
   if (threadIdx.x == 0) records[wg].first = -1;
   if (wg >= G) return;
-  const int64_t u_begin = wg * U / G, u_end = (wg + 1) * U / G;
-  if (at <= u_begin && u_begin < at + mine) {
-    int64_t b = b_lo, before = at;
-    for (;; ++b) {
-      const int64_t n = attn_units<kRows>(a, attn_request(a, b)) * kv_heads;
-      if (u_begin < before + n) break;
-      before += n;
+  const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
+  int head = same(static_cast<int>(u_begin / per_head));
+  const int64_t x = u_begin - head * per_head;  // within one head's units
+  int64_t b, item = 0;
+  int row0 = 0;
+  Request req;
+  Span span;
+  int64_t u_item;  // the item's first unit
+  if (items) {
+    const int64_t count = same(*item_count);
+    int64_t lo = 0, width = count;  // the item is among [lo, lo + width)
+    while (width > 1) {
+      const int64_t step = (width + 255) / 256;
+      const int64_t i = lo + threadIdx.x * step, end = min(i + step, lo + width);
+      if (i < lo + width && items[i].unit <= x && x < items[end].unit) found[0] = i, found[1] = end - i;
+      __syncthreads();
+      lo = found[0], width = found[1];
+      __syncthreads();
     }
-    found[0] = b, found[1] = before;
-  }
-  __syncthreads();
-  int64_t b = found[0], u_request = found[1];  // units in front of request b
-  Request req = attn_request(a, b);
-  int64_t per_head = attn_units<kRows>(a, req);
-  int head = static_cast<int>((u_begin - u_request) / per_head);
-  int64_t u_item = u_request + head * per_head, row0 = 0;
-  Span span = attn_span<kRows>(a, req, 0);
-  while (u_item + span.units <= u_begin) {
-    u_item += span.units;
-    row0 += kRows;
-    span = attn_span<kRows>(a, req, row0);
+    item = same(lo);
+    const AttnItem it = items[item];
+    b = same(it.request), row0 = same(it.row0);
+    req = same(attn_request(a, b));
+    span = same(attn_span<kRows>(a, req, row0));
+    u_item = head * per_head + same(it.unit);
+  } else {
+    if (at <= x && x < at + mine) {
+      int64_t i = b_lo, before = at;
+      for (;; ++i) {
+        const int64_t n = attn_units<kRows>(a, attn_request(a, i));
+        if (x < before + n) break;
+        before += n;
+      }
+      found[0] = i, found[1] = before;
+    }
+    __syncthreads();
+    b = same(found[0]), u_item = head * per_head + same(found[1]);
+    req = same(attn_request(a, b));
+    span = same(attn_span<kRows>(a, req, 0));
+    while (u_item + span.units <= u_begin) {
+      u_item += span.units;
+      row0 += kRows;
+      span = same(attn_span<kRows>(a, req, row0));
+    }
   }
 
-  const float scale2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
+  // scores in powers of two; a negative scale goes to the queries' signs
+  // (a scale of 0 becomes the smallest number, with which a masked score stays where it is)
+  const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, __uint_as_float(1u));
+  const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
+  const LaneOffsets offsets = lane_offsets<DIM>(lane, 1 << a.v.log2_page);
   for (int64_t u = u_begin; u < u_end;) {
-    const int64_t stop = min(u_item + span.units, u_end);
-    const int rows = static_cast<int>(min(int64_t{kRows}, static_cast<int64_t>(req.queries) * a.group - row0));
-    // queries: row n of each 16, quarter g of the dimensions, as the right operand
-    u32x4 q[kParts][NT][DIM / 32];
-    int pos[NT];
+    const int rows = min(kRows, req.queries * a.group - row0);
+    Q q;
+    q.shared = shared.queries;
+    Sight<NT> sight;
+    sight.sinks = a.window > 0 ? a.sinks : 0;
+    sight.begin = span.begin, sight.end = span.end, sight.sink_end = span.sink_end;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = 16 * n + n_lane;
-      const int64_t row = row0 + min(r, rows - 1);
-      const int64_t token = row / a.group;
-      const int64_t h = head * a.group + row % a.group;
-      pos[n] = r < rows ? req.before + static_cast<int>(token) : -1;
-      const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head + g * (DIM / 4);
+      const uint32_t row = row0 + min(r, rows - 1);
+      const uint32_t token = row / static_cast<uint32_t>(a.group);
+      const int h = head * a.group + static_cast<int>(row - token * a.group);
+      const int pos = r < rows ? req.before + static_cast<int>(token) : -1;
+      sight.last[n] = min(pos, a.limit - 1);
+      sight.after[n] = a.window > 0 && pos >= 0 ? pos - a.window : -1;
+      const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
+                     g * (DIM / 4);
+      constexpr int kSteps = DIM / 32;
 #pragma unroll
-      for (int i = 0; i < DIM / 32; ++i) {
-        const u32x4 x = reinterpret_cast<const u32x4 *>(src)[i];
-        if constexpr (kParts == 1) {
-          q[0][n][i] = x;
-        } else {
+      for (int i = 0; i < kSteps; ++i) {
+        if (Q::kShared && ((n * kSteps + i) & 3) != wave) continue;  // the waves fill LDS together
+        u32x4 y = reinterpret_cast<const u32x4 *>(src)[i] ^ flip, z;
+        if constexpr (kParts == 2) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-            const f16x2 y = __builtin_bit_cast(f16x2, static_cast<uint32_t>(x[j]));
-            const float y0 = static_cast<float>(y[0]), y1 = static_cast<float>(y[1]);
-            const uint32_t hi = pack_bf16(y0, y1);
-            q[0][n][i][j] = hi;
-            q[kParts - 1][n][i][j] = pack_bf16(y0 - __builtin_bit_cast(float, hi << 16),
-                                               y1 - __builtin_bit_cast(float, hi & 0xffff0000u));
+            const uint32_t both = y[j];
+            const f16x2 v = __builtin_bit_cast(f16x2, both);
+            const float v0 = static_cast<float>(v[0]), v1 = static_cast<float>(v[1]);
+            const uint32_t hi = pack_bf16(v0, v1);
+            y[j] = hi;
+            z[j] = pack_bf16(v0 - __uint_as_float(hi << 16), v1 - __uint_as_float(hi & 0xffff0000u));
           }
+        }
+        if constexpr (Q::kShared) {
+          shared.queries[(n * kSteps + i) * kWave + lane] = y;
+          if constexpr (kParts == 2) shared.queries[((NT + n) * kSteps + i) * kWave + lane] = z;
+        } else {
+          q.own[n * kSteps + i] = y;
+          if constexpr (kParts == 2) q.own[(NT + n) * kSteps + i] = z;
         }
       }
     }
+    if constexpr (Q::kShared) __syncthreads();
     RowState<DIM, NT> st;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -474,92 +619,165 @@ __global__ __launch_bounds__(256, NT * DIM <= 128 ? 4 : NT * DIM <= 256 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
     }
-    const int pos_first = req.before + static_cast<int>(row0 / a.group);
-    const int pos_last = req.before + static_cast<int>((row0 + rows - 1) / a.group);
+    // All rows see a whole tile that ends at or before the first row's place and begins in the last row's window.
+    const int pos_first = same(min(
+        req.before + static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group)), a.limit - 1));
+    const int after_last = same(
+        a.window > 0
+            ? max(req.before + static_cast<int>(static_cast<uint32_t>(row0 + rows - 1) / static_cast<uint32_t>(a.group)), -1) -
+                  a.window
+            : -1);
     const int32_t *table = a.table + b * a.table_stride;
-    for (; u < stop; ++u) {
-      const int k = static_cast<int>(u - u_item);
-      const int tile = k < span.sink_tiles ? k : span.tile0 + k - span.sink_tiles;
-      const int token0 = __builtin_amdgcn_readfirstlane(tile * kUnit + wave * kWaveTokens);
-      bool there[2];
-      int64_t page_at[2];
-      int off[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = token0 + 16 * half;
-        there[half] = j < span.end && (j + 15 >= span.begin || j < span.sink_end);
-        const int p = there[half] ? table[j >> a.v.log2_page] : 0;
-        there[half] = there[half] && p >= 0 && p < a.v.pages;
-        page_at[half] = there[half] ? p : 0;
-        off[half] = j & ((1 << a.v.log2_page) - 1);
+    const int first = same(static_cast<int>(u - u_item));
+    const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item));
+    auto token_of = [&](int k) {  // unit k's first token of this wave
+      return (k < span.sink_tiles ? k : span.tile0 + k - span.sink_tiles) * kUnit + wave * kWaveTokens;
+    };
+    // The page of the 16 tokens from j on; -1 where no row sees any of them.
+    auto page_at = [&](const int32_t *entries, const Span &sp, int j) {
+      int p = -1;
+      if (j < sp.end && (j + 15 >= sp.begin || j < sp.sink_end)) p = entries[j >> a.v.log2_page];
+      return p >= 0 && p < a.v.pages ? p : -1;
+    };
+    // Whether all rows see all of a wave's 32 tokens from token0 on, on pages p0 and p1.
+    auto tile_whole = [&](int token0, int p0, int p1) {
+      return p0 >= 0 && p1 >= 0 && token0 + kWaveTokens - 1 <= pos_first &&
+             (token0 > after_last || token0 + kWaveTokens <= sight.sinks);
+    };
+    // The pages of the next 32 units' tokens, one 16 of them a lane: -1 where no row sees any.
+    int page_of = -1, page_base = 0;
+    auto look_up = [&](int k0) {
+      page_base = k0;
+      const int k = k0 + (lane >> 1);
+      page_of = k < last ? page_at(table, span, token_of(k) + 16 * (lane & 1)) : -1;
+    };
+    struct Step {
+      int token0, page0, page1;
+    };
+    KvTile<DIM> ahead;
+    auto fetch = [&](int k) {
+      Step s;
+      s.token0 = token_of(k);
+      s.page0 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base));
+      s.page1 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base) + 1);
+      if (s.page0 >= 0 || s.page1 >= 0) {  // a half that is not there is loaded as page 0 and not looked at
+        const int mask = (1 << a.v.log2_page) - 1;
+        load_half<DIM>(a.v, head, max(s.page0, 0), s.token0 & mask, offsets, 0, ahead);
+        load_half<DIM>(a.v, head, max(s.page1, 0), (s.token0 + 16) & mask, offsets, 1, ahead);
       }
-      if (!there[0] && !there[1]) continue;
-      KvTile<DIM> t;
-      load_half<DIM>(a.v, head, page_at[0], off[0], lane, 0, t);
-      load_half<DIM>(a.v, head, page_at[1], off[1], lane, 1, t);
-      const bool whole = there[0] && there[1] && token0 + kWaveTokens - 1 <= pos_first && token0 + kWaveTokens <= span.end &&
-                         (a.window == 0 || int64_t{token0} > int64_t{pos_last} - a.window || token0 + kWaveTokens <= a.sinks);
-      if (whole) attend_tile<DIM, NT, kParts, false>(a, t, q, st, scale2, lane, token0, there, pos, span.end);
-      else attend_tile<DIM, NT, kParts, true>(a, t, q, st, scale2, lane, token0, there, pos, span.end);
+      return s;
+    };
+    bool wild = false;
+    look_up(first);
+    Step next = fetch(first);
+    for (int k = first; k < last; ++k) {
+      const Step now = next;
+      KvTile<DIM> t = ahead;
+      if (k + 1 < last) {
+        if (k + 1 - page_base == 32) look_up(k + 1);
+        next = fetch(k + 1);
+      }
+      if (now.page0 < 0 && now.page1 < 0) continue;
+      const bool whole = tile_whole(now.token0, now.page0, now.page1);
+      attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.page0 >= 0, now.page1 >= 0, sight, wild);
     }
+    u = u_item + last;
 
     // The four waves' states, 16 rows at a time, into the result or into a part.
-    const bool begins = u_item >= u_begin, ends = stop == u_item + span.units;
+    const bool begins = u_item >= u_begin, ends = last == span.units;
     const int64_t slot = 2 * wg + (begins ? 1 : 0);
+    const bool any_wild = __syncthreads_or(wild);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (16 * n < rows) {
         const float sum = across_sum(st.sum[n]);
         if (g == 0) {
-          shared.top[wave][n_lane] = st.top[n];
-          shared.sum[wave][n_lane] = sum;
+          shared.join.top[wave][n_lane] = st.top[n];
+          shared.join.sum[wave][n_lane] = sum;
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int i = 0; i < DIM / 16; i += 4)
-            *reinterpret_cast<f32x4 *>(&shared.acc[wave][n_lane * JoinShared<DIM>::kStride + (4 * g + r) * (DIM / 16) + i]) =
+            *reinterpret_cast<f32x4 *>(
+                &shared.join.acc[wave][n_lane * JoinShared<DIM>::kStride + (4 * g + r) * (DIM / 16) + i]) =
                 f32x4{st.acc[n][i][r], st.acc[n][i + 1][r], st.acc[n][i + 2][r], st.acc[n][i + 3][r]};
         __syncthreads();
         const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (DIM / 16);
         if (16 * n + r < rows) {
           float top = kNothing;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) top = fmaxf(top, shared.top[v][r]);
-          const float base = fmaxf(top, -3.0e38f);
-          float f[4], total_sum = 0;
+          for (int v = 0; v < 4; ++v) top = fmaxf(top, shared.join.top[v][r]);
+          const float base = fmaxf(top, kLowest);
+          float f[4], total = 0;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            f[v] = __builtin_amdgcn_exp2f(shared.top[v][r] - base);
-            total_sum += f[v] * shared.sum[v][r];
+            f[v] = __builtin_amdgcn_exp2f(shared.join.top[v][r] - base);
+            total += f[v] * shared.join.sum[v][r];
           }
-          float o[DIM / 16];
+          const uint32_t row = row0 + 16 * n + r;
+          const uint32_t token = row / static_cast<uint32_t>(a.group);
+          const int h = head * a.group + static_cast<int>(row - token * a.group);
+          const int64_t line = (req.first_row + token) * a.heads + h;
+          f32x4 o[DIM / 64];
 #pragma unroll
-          for (int i = 0; i < DIM / 16; ++i) {
-            o[i] = 0;
+          for (int i = 0; i < DIM / 64; ++i) {
+            o[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int v = 0; v < 4; ++v) o[i] += f[v] * shared.acc[v][r * JoinShared<DIM>::kStride + d0 + i];
+            for (int v = 0; v < 4; ++v)
+              o[i] += f[v] * *reinterpret_cast<const f32x4 *>(&shared.join.acc[v][r * JoinShared<DIM>::kStride + d0 + 4 * i]);
           }
-          if (begins && ends) {
-            const int64_t row = row0 + 16 * n + r;
-            const int64_t line = (req.first_row + row / a.group) * a.heads + head * a.group + row % a.group;
-            const float inv = total_sum == 0 ? 0 : 1 / total_sum;
-            T *out = static_cast<T *>(a.out) + line * DIM + d0;
-            typedef T out_vec __attribute__((ext_vector_type(4)));
+          if (any_wild) {
+            const int pos = req.before + static_cast<int>(token);
+            const int see_last = min(pos, a.limit - 1), see_after = a.window > 0 && pos >= 0 ? pos - a.window : -1;
+            const T *q_row = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head;
+            const int page = 1 << a.v.log2_page;
+#pragma unroll 1
+            for (int j16 = 0; j16 < (last - first) * (kUnit / 16); ++j16) {
+              const int k = first + j16 / (kUnit / 16);
+              const int j0 = (k < span.sink_tiles ? k : span.tile0 + k - span.sink_tiles) * kUnit + j16 % (kUnit / 16) * 16;
+              const int t0 = j0 & ~(kWaveTokens - 1);
+              const int p0 = page_at(table, span, t0), p1 = page_at(table, span, t0 + 16), at = j0 == t0 ? p0 : p1;
+              if (at < 0 || tile_whole(t0, p0, p1)) continue;
+              const int64_t tile = int64_t{2} * head << a.v.log2_page;
+              const int off = j0 & (page - 1);
+              const uint8_t *codes = a.v.cache + at * a.v.cache_stride + (tile + off) * (DIM / 2);
+              const uint8_t *sc = a.v.scales + at * a.v.scales_stride + tile * (DIM / 32) + off;
+#pragma unroll 1
+              for (int i = 0; i < 16; ++i) {
+                const int j = j0 + i;
+                const uint32_t byte = sc[(DIM / 32 + d0 / 32) * page + i];
+                if (byte < kWild || j > see_last || (j <= see_after && j >= sight.sinks)) continue;
+                const float x = score_of<T, DIM>(q_row, codes + i * (DIM / 2), sc + i, page);
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(a.scale < 0 ? -x : x, scale2, -base));
+                const uint8_t *v = codes + (page + i) * (DIM / 2) + d0 / 2;
 #pragma unroll
-            for (int i = 0; i < DIM / 16; i += 4)
-              *reinterpret_cast<out_vec *>(out + i) =
-                  out_vec{static_cast<T>(o[i] * inv), static_cast<T>(o[i + 1] * inv), static_cast<T>(o[i + 2] * inv),
-                          static_cast<T>(o[i + 3] * inv)};
-            if (a.lse && (threadIdx.x & 15) == 0)
-              a.lse[line] = total_sum == 0 ? kNothing : (top + __builtin_log2f(total_sum)) * 0.69314718055994530942f;
-          } else {
-            float *out = parts + (slot * kRows + 16 * n + r) * DIM + d0;
+                for (int d = 0; d < DIM / 16; d += 2) {
+                  const f32x2 y = decode2_f32<0>(v[d / 2], scale_operand(byte));
+                  o[d / 4][d % 4] += e * y[0];
+                  o[d / 4][d % 4 + 1] += e * y[1];
+                }
+              }
+            }
+          }
+          const float inv = total == 0 ? 0 : 1 / total;
 #pragma unroll
-            for (int i = 0; i < DIM / 16; i += 4) *reinterpret_cast<f32x4 *>(out + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
-            if ((threadIdx.x & 15) == 0) {
+          for (int i = 0; i < DIM / 64; ++i) {
+            if (begins && ends) {
+              typedef T out_vec __attribute__((ext_vector_type(4)));
+              *reinterpret_cast<out_vec *>(static_cast<T *>(a.out) + line * DIM + d0 + 4 * i) =
+                  out_vec{static_cast<T>(o[i][0] * inv), static_cast<T>(o[i][1] * inv), static_cast<T>(o[i][2] * inv),
+                          static_cast<T>(o[i][3] * inv)};
+            } else {
+              *reinterpret_cast<f32x4 *>(parts + (slot * kRows + 16 * n + r) * DIM + d0 + 4 * i) = o[i];
+            }
+          }
+          if ((threadIdx.x & 15) == 0) {
+            if (begins && ends) {
+              if (a.lse) a.lse[line] = total == 0 ? kNothing : (top + __builtin_log2f(total)) * 0.69314718055994530942f;
+            } else {
               part_stats[(slot * kRows + 16 * n + r) * 2] = top;
-              part_stats[(slot * kRows + 16 * n + r) * 2 + 1] = total_sum;
+              part_stats[(slot * kRows + 16 * n + r) * 2 + 1] = total;
             }
           }
         }
@@ -567,53 +785,74 @@ __global__ __launch_bounds__(256, NT * DIM <= 128 ? 4 : NT * DIM <= 256 ? 2 : 1)
       }
     }
     if (!begins && ends && threadIdx.x == 0) {
-      // the last workgroup whose units begin at the item's first unit or before it
-      records[wg] = JoinRecord{static_cast<int32_t>(((u_item + 1) * G - 1) / U), head, rows, static_cast<int32_t>(row0),
-                               req.first_row};
+      // begun by the last workgroup whose units begin at the item's first unit or before it
+      records[wg] = JoinRecord{static_cast<int32_t>(((u_item + 1) * G - 1) / U), head, rows, row0, req.first_row};
     }
     if (u >= u_end) break;
     // the next item
-    u_item += span.units;
-    row0 += kRows;
-    if (row0 >= static_cast<int64_t>(req.queries) * a.group) {
-      row0 = 0;
-      if (++head == kv_heads) {
-        head = 0;
+    u_item = u;
+    if (items) {
+      if (++item == same(*item_count)) item = 0, ++head;
+      const AttnItem it = items[item];
+      if (same(it.request) != b) req = same(attn_request(a, same(it.request)));
+      b = same(it.request), row0 = same(it.row0);
+    } else {
+      row0 += kRows;
+      if (row0 >= req.queries * a.group) {
+        row0 = 0;
         do {
-          req = attn_request(a, ++b);
+          if (++b == a.requests) b = 0, ++head;
+          req = same(attn_request(a, b));
         } while (req.queries == 0);
       }
     }
-    span = attn_span<kRows>(a, req, row0);
+    span = same(attn_span<kRows>(a, req, row0));
   }
 }
 
-// Puts the parts of an item together; a workgroup for each 4 rows of each record.
+// Puts the parts of an item together: a workgroup for a row of a record, a part for each DIM / 4 threads at a time.
 template <typename T, int DIM, int ROWS>
 __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, const float *parts, const float *part_stats,
                                                                   const JoinRecord *records) {
+  constexpr int kLanes = DIM / 4, kTeams = 256 / kLanes;
+  __shared__ f32x4 acc_shared[kTeams][kLanes];
+  __shared__ float top_shared[kTeams], sum_shared[kTeams];
   const int64_t wg = blockIdx.x;
   const JoinRecord rec = records[wg];
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int r = blockIdx.y;
   if (rec.first < 0 || r >= rec.rows) return;
-  const int lane = threadIdx.x & 63;
-  constexpr int kOwn = DIM / 64;
-  float top = kNothing, sum = 0, acc[kOwn] = {};
-  for (int64_t w = rec.first; w <= wg; ++w) {
+  const int team = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  float top = kNothing, sum = 0;
+  f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int64_t w = rec.first + team; w <= wg; w += kTeams) {
     const int64_t line = (2 * w + (w == rec.first ? 1 : 0)) * ROWS + r;
     const float m = part_stats[line * 2], l = part_stats[line * 2 + 1];
-    const float next = fmaxf(top, m), base = fmaxf(next, -3.0e38f);
+    const f32x4 o = *reinterpret_cast<const f32x4 *>(parts + line * DIM + lane * 4);
+    const float next = fmaxf(top, m), base = fmaxf(next, kLowest);
     const float f = __builtin_amdgcn_exp2f(top - base), e = __builtin_amdgcn_exp2f(m - base);
     sum = sum * f + l * e;
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) acc[o] = acc[o] * f + parts[line * DIM + lane * kOwn + o] * e;
+    acc = acc * f + o * e;
     top = next;
   }
-  const int64_t row = rec.row0 + r;
-  const int64_t line = (rec.first_row + row / a.group) * a.heads + rec.head * a.group + row % a.group;
-  T *out = static_cast<T *>(a.out) + line * DIM + lane * kOwn;
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) out[o] = static_cast<T>(sum == 0 ? 0 : acc[o] / sum);
+  acc_shared[team][lane] = acc;
+  if (lane == 0) top_shared[team] = top, sum_shared[team] = sum;
+  __syncthreads();
+  if (team != 0) return;
+  for (int i = 1; i < kTeams; ++i) top = fmaxf(top, top_shared[i]);
+  const float base = fmaxf(top, kLowest);
+  sum = 0, acc = f32x4{0, 0, 0, 0};
+  for (int i = 0; i < kTeams; ++i) {
+    const float f = __builtin_amdgcn_exp2f(top_shared[i] - base);
+    sum += f * sum_shared[i];
+    acc += f * acc_shared[i][lane];
+  }
+  const uint32_t row = rec.row0 + r, token = row / static_cast<uint32_t>(a.group);
+  const int64_t line = (rec.first_row + token) * a.heads + rec.head * a.group + (row - token * a.group);
+  const float inv = sum == 0 ? 0 : 1 / sum;
+  typedef T out_vec __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<out_vec *>(static_cast<T *>(a.out) + line * DIM + lane * 4) = out_vec{
+      static_cast<T>(acc[0] * inv), static_cast<T>(acc[1] * inv), static_cast<T>(acc[2] * inv), static_cast<T>(acc[3] * inv)};
   if (a.lse && lane == 0) a.lse[line] = sum == 0 ? kNothing : (top + __builtin_log2f(sum)) * 0.69314718055994530942f;
 }
 
@@ -621,47 +860,58 @@ __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, co
 
 struct AttnShape {
   int tiles;       // of 16 rows an item
+  int rows;        // the most that an item has
   int64_t groups;  // workgroups
-  int64_t parts_bytes, stats_bytes, record_bytes;
-  int64_t bytes() const { return parts_bytes + stats_bytes + record_bytes; }
+  int64_t items;   // room in the list of items; 0: none, every request is one item of a head
+  int64_t parts_bytes, stats_bytes, record_bytes, item_bytes, first_bytes;
+  int64_t bytes() const { return parts_bytes + stats_bytes + record_bytes + item_bytes + first_bytes; }
 };
 
-// How many rows an item has, and how many workgroups share the units: what the card holds at once, or the most units that
-// there can be.
-inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, int elem_type, int64_t requests,
-                            int64_t max_query_len) {
+// How many rows an item has, and how many workgroups share the units: as many as the card holds at once.
+inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, int64_t requests, int64_t max_query_len) {
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
-  const int64_t rows = longest * (heads / kv_heads);
-  const int most = (elem_type == SHMT_F16 ? 2 : 4) / (dim == 256 ? 2 : 1);
+  const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
-  s.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  s.tiles = std::min(s.tiles, most);
-  s.groups = s.tiles * dim <= 128 ? 1024 : s.tiles * dim <= 256 ? 512 : 256;
+  s.tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
+  s.rows = static_cast<int>(std::min<int64_t>(rows, 16 * s.tiles));
+  s.groups = 256 * attn_waves(dim, s.tiles);
+  s.items = rows > 16 * s.tiles ? tokens * group / (16 * s.tiles) + requests : 0;
   const int64_t lines = 2 * s.groups * 16 * s.tiles;
   s.parts_bytes = lines * dim * 4;
   s.stats_bytes = lines * 8;
   s.record_bytes = s.groups * static_cast<int64_t>(sizeof(JoinRecord));
+  s.item_bytes = s.items ? (s.items + 2) * static_cast<int64_t>(sizeof(AttnItem)) : 0;  // the count behind the last one
+  s.first_bytes = s.items ? (requests + 4) / 4 * 16 : 0;
   return s;
 }
 
 template <typename T, int DIM, int NT>
 void launch_tiles(const AttnArgs &a, const AttnShape &s, void *scratch, hipStream_t stream) {
-  float *parts = static_cast<float *>(scratch);
-  float *stats = reinterpret_cast<float *>(static_cast<char *>(scratch) + s.parts_bytes);
-  JoinRecord *records = reinterpret_cast<JoinRecord *>(static_cast<char *>(scratch) + s.parts_bytes + s.stats_bytes);
+  char *at = static_cast<char *>(scratch);
+  float *parts = reinterpret_cast<float *>(at);
+  float *stats = reinterpret_cast<float *>(at += s.parts_bytes);
+  JoinRecord *records = reinterpret_cast<JoinRecord *>(at += s.stats_bytes);
+  AttnItem *items = nullptr;
+  int32_t *count = nullptr;
+  if (s.items) {
+    items = reinterpret_cast<AttnItem *>(at += s.record_bytes);
+    count = reinterpret_cast<int32_t *>(items + s.items + 1);
+    int32_t *first_item = reinterpret_cast<int32_t *>(at += s.item_bytes);
+    hipLaunchKernelGGL((page_attention_items_kernel<16 * NT>), dim3(1), dim3(1024), 0, stream, a, first_item, items,
+                       s.items, count);
+  }
   const unsigned groups = static_cast<unsigned>(s.groups);
-  hipLaunchKernelGGL((page_attention_kernel<T, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, parts, stats, records);
-  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(groups, 4 * NT), dim3(256), 0, stream, a, parts,
+  hipLaunchKernelGGL((page_attention_kernel<T, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, items, count, parts, stats,
+                     records);
+  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(groups, 16 * NT), dim3(256), 0, stream, a, parts,
                      stats, records);
 }
 
 template <typename T, int DIM>
 void launch_dim(const AttnArgs &a, const AttnShape &s, void *scratch, hipStream_t stream) {
-  constexpr int kMost = (std::is_same<T, _Float16>::value ? 2 : 4) / (DIM == 256 ? 2 : 1);
   if (s.tiles == 1) return launch_tiles<T, DIM, 1>(a, s, scratch, stream);
-  if constexpr (kMost >= 2)
-    if (s.tiles == 2) return launch_tiles<T, DIM, 2>(a, s, scratch, stream);
-  if constexpr (kMost >= 4) launch_tiles<T, DIM, 4>(a, s, scratch, stream);
+  if (s.tiles == 2) return launch_tiles<T, DIM, 2>(a, s, scratch, stream);
+  if constexpr (DIM < 256) launch_tiles<T, DIM, 4>(a, s, scratch, stream);
 }
 
 template <typename T>
@@ -684,7 +934,7 @@ int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads, int kv_head
     set_error("bad arguments for the attention's scratch size");
     return -1;
   }
-  return attn_shape(tokens, heads, kv_heads, dim, elem_type, requests, max_query_len).bytes();
+  return attn_shape(tokens, heads, kv_heads, dim, requests, max_query_len).bytes();
 }
 
 int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_t query_token_stride,
@@ -700,6 +950,7 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_
   SHMT_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31), "the number of query rows must be in [0, 2^31)");
   SHMT_REQUIRE(heads >= 1 && heads <= 65535 && heads % cache->kv_heads == 0,
                "%d query heads do not share %d heads of the cache evenly", heads, cache->kv_heads);
+  SHMT_REQUIRE(tokens * heads < (int64_t{1} << 30), "query rows x heads must be below 2^30");
   SHMT_REQUIRE(requests >= 0 && requests < (int64_t{1} << 31), "the number of requests must be in [0, 2^31)");
   SHMT_REQUIRE(width >= 0 && width < (int64_t{1} << 31) / cache->page, "the block table holds too many tokens");
   SHMT_REQUIRE(width_ok(len_bytes), "query_starts and kv_lens can only be int32 or int64");
@@ -712,16 +963,18 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_
   SHMT_REQUIRE(((reinterpret_cast<int64_t>(query) | query_token_stride * 2 | query_head_stride * 2) & 15) == 0,
                "every row of query has to begin on 16 bytes");
   SHMT_REQUIRE((reinterpret_cast<int64_t>(out) & 15) == 0, "out has to begin on 16 bytes");
-  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, cache->dim, elem_type, requests, max_query_len);
+  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, cache->dim, requests, max_query_len);
   if (scratch_bytes < shape.bytes() || !scratch) {
     set_error("scratch too small: %lld bytes, needed %lld", static_cast<long long>(scratch_bytes),
               static_cast<long long>(shape.bytes()));
     return SHMT_ENOMEM;
   }
   SHMT_REQUIRE((reinterpret_cast<int64_t>(scratch) & 15) == 0, "scratch has to begin on 16 bytes");
-  const AttnArgs a{v, query, query_token_stride, query_head_stride, tokens, heads, heads / cache->kv_heads,
-                   block_table, width, table_stride, query_starts, kv_lens, len_bytes, requests, softmax_scale,
-                   window, sinks, out, lse};
+  constexpr int64_t kMost = 0x7fffffff;  // a longer window, or more sinks, than any request has tokens
+  const AttnArgs a{v, query, query_token_stride, query_head_stride, tokens, heads, heads / cache->kv_heads, block_table,
+                   table_stride, query_starts, kv_lens, len_bytes, requests, softmax_scale,
+                   static_cast<int32_t>(std::min(window, kMost)), static_cast<int32_t>(std::min(sinks, kMost)),
+                   v.pages > 0 ? static_cast<int32_t>(width * cache->page) : 0, out, lse};
   if (elem_type == SHMT_F16) launch_attention<_Float16>(a, cache->dim, shape, scratch, as_stream(stream));
   else launch_attention<__bf16>(a, cache->dim, shape, scratch, as_stream(stream));
   SHMT_LAUNCH_CHECK();
