@@ -267,7 +267,7 @@ __device__ __forceinline__ void load_half(const PagedView &v, int head, int at, 
 // (4 g + r) * DIM / 16 + i in acc[.][i][r].
 template <int DIM, int NT>
 struct RowState {
-  float top[NT], sum[NT];  // of scores in powers of two; the sum over this lane's tokens only
+  float top[NT], sum[NT];  // the reference of the weights, in powers of two; their sum over this lane's tokens only
   f32x4 acc[NT][DIM / 16];
 };
 
@@ -307,8 +307,9 @@ constexpr uint32_t kWild = 253;
 // result's own rounding.
 // `whole`: all rows see all tokens. Otherwise scores are masked; and values that are not finite in bfloat16 must not meet the
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
+// Returns whether the item has to be begun again (see below).
 template <int DIM, int NT, int PARTS>
-__device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
+__device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int lane, bool whole, int token0, bool there0, bool there1,
                                             const Sight<NT> &sight, bool &wild) {
   const int g = lane >> 4;
@@ -324,6 +325,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
       const uint32_t c = t.key[half][i];
       k[half] = u32x4{decode2_bf16<0>(c, f), decode2_bf16<1>(c, f), decode2_bf16<2>(c, f), decode2_bf16<3>(c, f)};
     }
+    if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int p = 0; p < PARTS; ++p)
 #pragma unroll
@@ -333,6 +335,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
         s[n][1] = mfma(k[1], x, s[n][1]);
       }
   }
+  if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
   if (!whole) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -351,27 +354,18 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
         wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
       }
   }
-  float most[NT];
-  bool grows = false;
+  // Weights are taken relative to the maximum of the first tile in which a row saw anything. With floats' exponents any
+  // reference near the true maximum does as well, so nothing is rescaled; where a score passes it by 2^40, which ordinary
+  // scores do not, the wave begins its tokens again with the greater one.
+  bool passed = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float x = s[n][0][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n][j / 4][j % 4]);
-    most[n] = across_max(x) * scale2;
-    grows |= most[n] > st.top[n] + 8.0f;
-  }
-  // The running maximum moves only where a weight would pass 2^8 (the first one always does).
-  if (__ballot(grows)) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float next = fmaxf(st.top[n], most[n]);
-      const float f = __builtin_amdgcn_exp2f(st.top[n] - fmaxf(next, kLowest));
-      st.top[n] = next;
-      st.sum[n] *= f;
-#pragma unroll
-      for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] *= f;
-    }
+    const float most = across_max(x) * scale2;
+    st.top[n] = st.top[n] == kNothing ? most : st.top[n];
+    if (most > st.top[n] + 40.0f) passed = true, st.top[n] = most;
   }
   u32x4 w[PARTS][NT];
 #pragma unroll
@@ -400,6 +394,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
 #pragma unroll
   for (int word = 0; word < KvTile<DIM>::kValueWords; ++word) {
     auto two = [&](auto byte) {  // dimensions 2 B and 2 B + 1 of this lane's
+      if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
       constexpr int B = decltype(byte)::value;
       uint32_t x[8];
 #pragma unroll
@@ -425,6 +420,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
       two(std::integral_constant<int, 3>{});
     }
   }
+  return __ballot(passed) != 0;
 }
 
 // q . K[j] of one row and token, element by element.
@@ -611,14 +607,6 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       }
     }
     if constexpr (Q::kShared) __syncthreads();
-    RowState<DIM, NT> st;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      st.top[n] = kNothing;
-      st.sum[n] = 0;
-#pragma unroll
-      for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
-    }
     // All rows see a whole tile that ends at or before the first row's place and begins in the last row's window.
     const int pos_first = same(min(
         req.before + static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group)), a.limit - 1));
@@ -654,33 +642,56 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
     struct Step {
       int token0, page0, page1;
     };
+    // The next unit from k on that has anything for this wave; `last` if there is none.
+    auto find = [&](int k) {
+      for (; k < last; ++k) {
+        if (k - page_base >= 32) look_up(k);
+        const int at = 2 * (k - page_base);
+        if (__builtin_amdgcn_readlane(page_of, at) >= 0 || __builtin_amdgcn_readlane(page_of, at + 1) >= 0) break;
+      }
+      return k;
+    };
     KvTile<DIM> ahead;
     auto fetch = [&](int k) {
       Step s;
       s.token0 = token_of(k);
       s.page0 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base));
       s.page1 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base) + 1);
-      if (s.page0 >= 0 || s.page1 >= 0) {  // a half that is not there is loaded as page 0 and not looked at
-        const int mask = (1 << a.v.log2_page) - 1;
-        load_half<DIM>(a.v, head, max(s.page0, 0), s.token0 & mask, offsets, 0, ahead);
-        load_half<DIM>(a.v, head, max(s.page1, 0), (s.token0 + 16) & mask, offsets, 1, ahead);
-      }
+      const int mask = (1 << a.v.log2_page) - 1;  // a half that is not there is loaded as page 0 and not looked at
+      load_half<DIM>(a.v, head, max(s.page0, 0), s.token0 & mask, offsets, 0, ahead);
+      load_half<DIM>(a.v, head, max(s.page1, 0), (s.token0 + 16) & mask, offsets, 1, ahead);
       return s;
     };
-    bool wild = false;
-    look_up(first);
-    Step next = fetch(first);
-    for (int k = first; k < last; ++k) {
-      const Step now = next;
-      KvTile<DIM> t = ahead;
-      if (k + 1 < last) {
-        if (k + 1 - page_base == 32) look_up(k + 1);
-        next = fetch(k + 1);
+    bool wild = false, again;
+    RowState<DIM, NT> st;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) st.top[n] = kNothing;
+    // Nothing in this loop changes the accumulators but the products, on every way through it: only so do they stay in one
+    // place.
+    do {
+      again = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        st.sum[n] = 0;
+#pragma unroll
+        for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
       }
-      if (now.page0 < 0 && now.page1 < 0) continue;
-      const bool whole = tile_whole(now.token0, now.page0, now.page1);
-      attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.page0 >= 0, now.page1 >= 0, sight, wild);
-    }
+      look_up(first);
+      int k = find(first);
+      if (k >= last) break;
+      Step next = fetch(k);
+      bool more;
+      do {
+        const Step now = next;
+        KvTile<DIM> t = ahead;
+        k = find(k + 1);
+        more = k < last;
+        if (more) next = fetch(k);
+        const bool whole = tile_whole(now.token0, now.page0, now.page1);
+        again = attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.page0 >= 0, now.page1 >= 0, sight,
+                                             wild);
+      } while (more && !again);
+    } while (again);
     u = u_item + last;
 
     // The four waves' states, 16 rows at a time, into the result or into a part.
