@@ -7,6 +7,8 @@
 #include "paged_host.h"
 #include "wave.h"
 
+#include <algorithm>
+
 namespace shmt {
 
 // ---- plan ---------------------------------------------------------------------
@@ -23,36 +25,137 @@ struct PlanArgs {
   int64_t max_tokens;
   int32_t *starts, *kv_lens, *positions;
   int64_t *slots, *counts;
-  int64_t *first_free;  // scratch: [requests]
 };
 
-__device__ __forceinline__ int64_t plan_len(const void *p, int64_t i, int bytes) {
-  const int64_t v = load_int(p, i, bytes);
-  return v < 0 ? 0 : v;
+// A request: its tokens, and what lies in front of it in the step.
+struct PlanRequest {
+  int64_t cached, fresh;
+  int64_t start, first_free;  // new tokens and pages needed by the requests before it
+};
+
+__device__ __forceinline__ int64_t plan_pages(const PlanArgs &a, int64_t tokens) {
+  return (tokens + (int64_t{1} << a.log2_page) - 1) >> a.log2_page;
 }
 
-// Token counts and page needs of all requests, summed in front of each: one workgroup, 1024 requests a step.
-__global__ __launch_bounds__(1024) void page_plan_scan_kernel(PlanArgs a) {
-  __shared__ uint64_t lds[32];
-  const int64_t page = int64_t{1} << a.log2_page;
+__device__ __forceinline__ void plan_lens(const PlanArgs &a, int64_t i, int64_t *cached, int64_t *fresh) {
+  const int64_t at[1] = {i};
+  const bool ok[1] = {true};
+  int64_t c[1], n[1];
+  load_ints(a.cached, at, ok, a.len_bytes, c);
+  load_ints(a.fresh, at, ok, a.len_bytes, n);
+  *cached = max(c[0], int64_t{0});
+  *fresh = max(n[0], int64_t{0});
+}
+
+// Page p of a request after the step; -1 where there is none.
+__device__ __forceinline__ int64_t planned_page(const PlanArgs &a, int64_t b, int64_t p, int64_t have,
+                                                int64_t first_free) {
+  if (p >= a.width) return -1;
+  if (p < have) return a.table[b * a.table_stride + p];
+  const int64_t f = first_free + p - have;
+  return f < a.n_free ? a.free_pages[f] : -1;
+}
+
+// Position and slot of new token t, which is request b's.
+__device__ __forceinline__ void plan_token(const PlanArgs &a, int64_t t, int64_t b, const PlanRequest &r) {
+  const int64_t page = int64_t{1} << a.log2_page, pos = r.cached + t - r.start;
+  const int64_t at = planned_page(a, b, pos >> a.log2_page, plan_pages(a, r.cached), r.first_free);
+  a.positions[t] = static_cast<int32_t>(pos);
+  a.slots[t] = at < 0 ? -1 : (at << a.log2_page) + (pos & (page - 1));
+}
+
+// The new table entries of request b, by `lanes` lanes.
+__device__ __forceinline__ void plan_entries(const PlanArgs &a, int64_t b, const PlanRequest &r, int lane, int lanes) {
+  const int64_t have = plan_pages(a, r.cached), end = min(plan_pages(a, r.cached + r.fresh), a.width);
+  for (int64_t p = have + lane; p < end; p += lanes)
+    a.table[b * a.table_stride + p] = static_cast<int32_t>(planned_page(a, b, p, have, r.first_free));
+}
+
+// Up to kPlanOne requests, in one launch: every workgroup adds up all lengths for itself (they are few, and it costs less than
+// a second launch), keeps the sums in LDS and takes its share of the tokens and of the requests' table rows. No workgroup
+// reads a table entry that another writes: tokens on new pages take them from the list of free pages.
+constexpr int kPlanOne = 2048;
+
+__global__ __launch_bounds__(256) void page_plan_one_kernel(PlanArgs a) {
+  __shared__ int64_t cached[kPlanOne], start[kPlanOne + 1], first_free[kPlanOne];
+  __shared__ uint64_t scan[4];
+  const int n = static_cast<int>(a.requests);
+  // lengths, all in flight at once; counts to where the sums will be
+  constexpr int kEach = kPlanOne / 256;
+  int64_t at[kEach], c[kEach] = {}, f[kEach] = {};
+  bool ok[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) at[k] = threadIdx.x + 256 * k, ok[k] = at[k] < n;
+  load_ints(a.cached, at, ok, a.len_bytes, c);
+  load_ints(a.fresh, at, ok, a.len_bytes, f);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (ok[k]) {
+      c[k] = max(c[k], int64_t{0}), f[k] = max(f[k], int64_t{0});
+      cached[at[k]] = c[k];
+      start[at[k]] = f[k];
+      first_free[at[k]] = plan_pages(a, c[k] + f[k]) - plan_pages(a, c[k]);
+      if (blockIdx.x == 0) a.kv_lens[at[k]] = static_cast<int32_t>(c[k] + f[k]);
+    }
+  __syncthreads();
+  const int each = (n + 255) / 256, lo = min(static_cast<int>(threadIdx.x) * each, n), hi = min(lo + each, n);
+  uint64_t tokens = 0, pages = 0;
+  for (int b = lo; b < hi; ++b) tokens += start[b], pages += first_free[b];
+  uint64_t all_tokens, all_pages;
+  uint64_t at_token = block_exclusive_scan<uint64_t, 256>(tokens, scan, &all_tokens);
+  uint64_t at_page = block_exclusive_scan<uint64_t, 256>(pages, scan, &all_pages);
+  for (int b = lo; b < hi; ++b) {
+    const uint64_t t = start[b], p = first_free[b];
+    start[b] = at_token;
+    first_free[b] = at_page;
+    if (blockIdx.x == 0) a.starts[b] = static_cast<int32_t>(at_token);
+    at_token += t;
+    at_page += p;
+  }
+  if (threadIdx.x == 0) {
+    start[n] = all_tokens;
+    if (blockIdx.x == 0) {
+      a.starts[n] = static_cast<int32_t>(all_tokens);
+      a.counts[0] = static_cast<int64_t>(all_tokens);
+      a.counts[1] = static_cast<int64_t>(all_pages);
+    }
+  }
+  __syncthreads();
+  const int64_t total = static_cast<int64_t>(all_tokens);
+  for (int64_t t = int64_t{blockIdx.x} * 256 + threadIdx.x; t < a.max_tokens; t += int64_t{gridDim.x} * 256) {
+    if (t >= total) {
+      a.positions[t] = -1;
+      a.slots[t] = -1;
+      continue;
+    }
+    int b = 0, last = n - 1;  // the last request that starts at t or before
+    while (b < last) {
+      const int mid = (b + last + 1) >> 1;
+      if (start[mid] <= t) b = mid; else last = mid - 1;
+    }
+    plan_token(a, t, b, PlanRequest{cached[b], 0, start[b], first_free[b]});
+  }
+  // 16 lanes a request
+  for (int64_t b = int64_t{blockIdx.x} * 16 + threadIdx.x / 16; b < n; b += int64_t{gridDim.x} * 16)
+    plan_entries(a, b, PlanRequest{cached[b], start[b + 1] - start[b], start[b], first_free[b]}, threadIdx.x % 16, 16);
+}
+
+// More requests: the sums by one workgroup, 1024 requests a step ...
+__global__ __launch_bounds__(1024) void page_plan_scan_kernel(PlanArgs a, int64_t *first_free) {
+  __shared__ uint64_t lds[16];
   uint64_t tokens = 0, taken = 0;
   for (int64_t base = 0; base < a.requests; base += 1024) {
     const int64_t i = base + threadIdx.x;
     int64_t c = 0, n = 0;
-    if (i < a.requests) {
-      c = plan_len(a.cached, i, a.len_bytes);
-      n = plan_len(a.fresh, i, a.len_bytes);
-    }
-    const int64_t need = ((c + n + page - 1) >> a.log2_page) - ((c + page - 1) >> a.log2_page);
+    if (i < a.requests) plan_lens(a, i, &c, &n);
     uint64_t sum_n, sum_need;
     const uint64_t at_n = block_exclusive_scan<uint64_t, 1024>(n, lds, &sum_n);
-    __syncthreads();
-    const uint64_t at_need = block_exclusive_scan<uint64_t, 1024>(need, lds, &sum_need);
-    __syncthreads();
+    const uint64_t at_need =
+        block_exclusive_scan<uint64_t, 1024>(plan_pages(a, c + n) - plan_pages(a, c), lds, &sum_need);
     if (i < a.requests) {
       a.starts[i] = static_cast<int32_t>(tokens + at_n);
       a.kv_lens[i] = static_cast<int32_t>(c + n);
-      a.first_free[i] = static_cast<int64_t>(taken + at_need);
+      first_free[i] = static_cast<int64_t>(taken + at_need);
     }
     tokens += sum_n;
     taken += sum_need;
@@ -64,47 +167,31 @@ __global__ __launch_bounds__(1024) void page_plan_scan_kernel(PlanArgs a) {
   }
 }
 
-// Page p of request b after the step; -1 where there is none.
-__device__ __forceinline__ int64_t planned_page(const PlanArgs &a, int64_t b, int64_t p, int64_t have) {
-  if (p >= a.width) return -1;
-  if (p < have) return a.table[b * a.table_stride + p];
-  const int64_t f = a.first_free[b] + p - have;
-  return f < a.n_free ? a.free_pages[f] : -1;
-}
-
-__global__ __launch_bounds__(256) void page_plan_tokens_kernel(PlanArgs a) {
-  const int64_t page = int64_t{1} << a.log2_page;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+// ... then tokens and table rows by all.
+__global__ __launch_bounds__(256) void page_plan_rest_kernel(PlanArgs a, const int64_t *first_free) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256, me = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t total = a.counts[0];
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < a.max_tokens; t += stride) {
-    int64_t pos = -1, slot = -1;
-    if (t < total) {
-      int64_t lo = 0, hi = a.requests - 1;  // the last request that starts at t or before
-      while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) >> 1;
-        if (a.starts[mid] <= t) lo = mid; else hi = mid - 1;
-      }
-      const int64_t c = plan_len(a.cached, lo, a.len_bytes);
-      pos = c + t - a.starts[lo];
-      const int64_t at = planned_page(a, lo, pos >> a.log2_page, (c + page - 1) >> a.log2_page);
-      slot = at < 0 ? -1 : (at << a.log2_page) + (pos & (page - 1));
+  for (int64_t t = me; t < a.max_tokens; t += stride) {
+    if (t >= total) {
+      a.positions[t] = -1;
+      a.slots[t] = -1;
+      continue;
     }
-    a.positions[t] = static_cast<int32_t>(pos);
-    a.slots[t] = slot;
+    int64_t b = 0, last = a.requests - 1;  // the last request that starts at t or before
+    while (b < last) {
+      const int64_t mid = (b + last + 1) >> 1;
+      if (a.starts[mid] <= t) b = mid; else last = mid - 1;
+    }
+    PlanRequest r;
+    plan_lens(a, b, &r.cached, &r.fresh);
+    r.start = a.starts[b], r.first_free = first_free[b];
+    plan_token(a, t, b, r);
   }
-}
-
-// The new entries of the block table, a wave per request.
-__global__ __launch_bounds__(256) void page_plan_table_kernel(PlanArgs a) {
-  const int64_t page = int64_t{1} << a.log2_page;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave; b < a.requests; b += stride) {
-    const int64_t c = plan_len(a.cached, b, a.len_bytes), n = plan_len(a.fresh, b, a.len_bytes);
-    const int64_t have = (c + page - 1) >> a.log2_page;
-    int64_t end = (c + n + page - 1) >> a.log2_page;
-    if (end > a.width) end = a.width;
-    for (int64_t p = have + lane_id(); p < end; p += kWave)
-      a.table[b * a.table_stride + p] = static_cast<int32_t>(planned_page(a, b, p, have));
+  for (int64_t b = me / 16; b < a.requests; b += stride / 16) {
+    PlanRequest r;
+    plan_lens(a, b, &r.cached, &r.fresh);
+    r.first_free = first_free[b];
+    plan_entries(a, b, r, threadIdx.x % 16, 16);
   }
 }
 
@@ -122,7 +209,8 @@ struct RowsArgs {
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+    const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p)),
+                b = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p) + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[i] = a[i];
@@ -130,7 +218,7 @@ __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
     }
   } else {
     typedef T vec __attribute__((ext_vector_type(8)));
-    const vec a = *reinterpret_cast<const vec *>(p);
+    const vec a = __builtin_nontemporal_load(reinterpret_cast<const vec *>(p));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
   }
@@ -139,40 +227,80 @@ __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
 template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<f32x4 *>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4 *>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(p));
+    __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(p) + 1);
   } else {
     typedef T vec __attribute__((ext_vector_type(8)));
     vec a;
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = static_cast<T>(x[i]);
-    *reinterpret_cast<vec *>(p) = a;
+    __builtin_nontemporal_store(a, reinterpret_cast<vec *>(p));
   }
 }
 
-// Eight values a lane, DIM / 8 lanes a row, four lanes a block of 32 that shares a scale.
-template <typename T, int DIM>
+// A workgroup takes PASSES * 2048 / DIM tokens in a row of one head's keys or values: DIM / 8 lanes a token, eight values a
+// lane, four lanes a block of 32 that shares a scale. Tokens in a row mostly lie in a row in their page too, so the codes
+// leave (or come) as one piece, and the scale bytes, which lie token by token, meet in one L2. All of a lane's rows are in
+// flight together. Bound by HBM.
+template <int DIM, int PASSES>
+struct RowPlace {
+  static constexpr int kLanes = DIM / 8;
+  static constexpr int kPasses = PASSES;
+  int head, which, piece;
+  int64_t token0;  // of pass 0; 256 / kLanes tokens a pass
+  int64_t slot[kPasses];  // -1: nowhere
+
+  __device__ __forceinline__ explicit RowPlace(const RowsArgs &a) {
+    const uint32_t tiles = 2 * a.v.kv_heads;
+    const uint32_t tile = blockIdx.x % tiles;
+    which = tile / a.v.kv_heads;
+    head = tile % a.v.kv_heads;
+    piece = threadIdx.x % kLanes;
+    token0 = int64_t{blockIdx.x / tiles} * (PASSES * 256 / kLanes) + threadIdx.x / kLanes;
+    int64_t at[kPasses];
+    bool ok[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      at[p] = token0 + p * (256 / kLanes);
+      ok[p] = at[p] < a.tokens;
+      slot[p] = -1;
+    }
+    load_ints(a.slots, at, ok, a.slot_bytes, slot);
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+      if (slot[p] < 0 || slot[p] >> a.v.log2_page >= a.v.pages) slot[p] = -1;
+  }
+  __device__ __forceinline__ int64_t token(int p) const { return token0 + p * (256 / kLanes); }
+  __device__ __forceinline__ uint32_t *codes(const RowsArgs &a, int p) const {
+    const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
+    return reinterpret_cast<uint32_t *>(a.v.cache + at * a.v.cache_stride +
+                                        ((int64_t{2} * head + which << a.v.log2_page) + off) * (DIM / 2) + piece * 4);
+  }
+  __device__ __forceinline__ uint8_t *scale(const RowsArgs &a, int p) const {
+    const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
+    return a.v.scales + at * a.v.scales_stride +
+           (((int64_t{2} * head + which) * (DIM / 32) + piece / 4) << a.v.log2_page) + off;
+  }
+};
+
+template <typename T, int DIM, int PASSES>
 __global__ __launch_bounds__(256) void page_set_kernel(RowsArgs a) {
-  constexpr int kLanes = DIM / 8;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  const int64_t all = a.tokens * a.v.kv_heads * 2 * kLanes;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += stride) {
-    const int piece = static_cast<int>(i % kLanes);
-    const int64_t row = i / kLanes;
-    const int head = static_cast<int>(row % a.v.kv_heads);
-    const int64_t th = row / a.v.kv_heads;
-    const int which = static_cast<int>(th & 1);
-    const int64_t token = th >> 1;
-    const int64_t slot = load_int(a.slots, token, a.slot_bytes);
-    if (slot < 0 || slot >> a.v.log2_page >= a.v.pages) continue;  // the same for all lanes of a row
-    const T *src = which ? static_cast<const T *>(a.values) + token * a.value_token + head * a.value_head
-                         : static_cast<const T *>(a.keys) + token * a.key_token + head * a.key_head;
-    float x[8];
-    load8(src + piece * 8, x);
+  const RowPlace<DIM, PASSES> r(a);
+  constexpr int kPasses = PASSES;
+  const T *src = r.which ? static_cast<const T *>(a.values) + r.head * a.value_head
+                         : static_cast<const T *>(a.keys) + r.head * a.key_head;
+  const int64_t token_stride = r.which ? a.value_token : a.key_token;
+  float x[kPasses][8];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p)
+    if (r.slot[p] >= 0) load8(src + r.token(p) * token_stride + r.piece * 8, x[p]);
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    if (r.slot[p] < 0) continue;  // the same for all lanes of a row
     // the largest magnitude, compared as bits, so that "not a number" comes out on top
     uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[p][j]) & 0x7fffffffu);
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 1)));
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 2)));
     // The smallest power of two with most < 7 * 2^e: nothing is cut by more than half the step at its place (6 is
@@ -181,70 +309,61 @@ __global__ __launch_bounds__(256) void page_set_kernel(RowsArgs a) {
     const int e = max(static_cast<int>((most + 0x200000u) >> 23) - 2, 0);
     const float s = scale_operand(static_cast<uint32_t>(e));
     uint32_t codes = 0;
-    if (!broken) {
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], s, 0);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], s, 1);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], s, 2);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], s, 3);
-    }
-    const int64_t at = slot >> a.v.log2_page, page = int64_t{1} << a.v.log2_page, off = slot & (page - 1);
-    const int64_t tile = head * 2 + which;
-    *reinterpret_cast<uint32_t *>(a.v.cache + at * a.v.cache_stride + (tile * page + off) * (DIM / 2) + piece * 4) =
-        codes;
-    if ((piece & 3) == 0)
-      a.v.scales[at * a.v.scales_stride + (tile * (DIM / 32) + piece / 4) * page + off] =
-          static_cast<uint8_t>(broken ? 255 : e);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][0], x[p][1], s, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][2], x[p][3], s, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][4], x[p][5], s, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][6], x[p][7], s, 3);
+    *r.codes(a, p) = broken ? 0u : codes;
+    if ((r.piece & 3) == 0) *r.scale(a, p) = static_cast<uint8_t>(broken ? 255 : e);
   }
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int PASSES>
 __global__ __launch_bounds__(256) void page_fetch_kernel(RowsArgs a) {
-  constexpr int kLanes = DIM / 8;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  const int64_t all = a.tokens * a.v.kv_heads * 2 * kLanes;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += stride) {
-    const int piece = static_cast<int>(i % kLanes);
-    const int64_t row = i / kLanes;
-    const int head = static_cast<int>(row % a.v.kv_heads);
-    const int64_t th = row / a.v.kv_heads;
-    const int which = static_cast<int>(th & 1);
-    const int64_t token = th >> 1;
-    const int64_t slot = load_int(a.slots, token, a.slot_bytes);
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (slot >= 0 && slot >> a.v.log2_page < a.v.pages) {
-      const int64_t at = slot >> a.v.log2_page, page = int64_t{1} << a.v.log2_page, off = slot & (page - 1);
-      const int64_t tile = head * 2 + which;
-      const uint32_t codes = *reinterpret_cast<const uint32_t *>(
-          a.v.cache + at * a.v.cache_stride + (tile * page + off) * (DIM / 2) + piece * 4);
-      const float s =
-          scale_operand(a.v.scales[at * a.v.scales_stride + (tile * (DIM / 32) + piece / 4) * page + off]);
-      const f32x2 p0 = decode2_f32<0>(codes, s), p1 = decode2_f32<1>(codes, s), p2 = decode2_f32<2>(codes, s),
-                  p3 = decode2_f32<3>(codes, s);
-      x[0] = p0[0], x[1] = p0[1], x[2] = p1[0], x[3] = p1[1], x[4] = p2[0], x[5] = p2[1], x[6] = p3[0], x[7] = p3[1];
-    }
-    T *dst = which ? static_cast<T *>(const_cast<void *>(a.values)) + token * a.value_token + head * a.value_head
-                   : static_cast<T *>(const_cast<void *>(a.keys)) + token * a.key_token + head * a.key_head;
-    store8(dst + piece * 8, x);
+  const RowPlace<DIM, PASSES> r(a);
+  constexpr int kPasses = PASSES;
+  uint32_t codes[kPasses], scale[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    codes[p] = scale[p] = 0;
+    if (r.slot[p] >= 0) codes[p] = *r.codes(a, p), scale[p] = *r.scale(a, p);
+  }
+  T *dst = static_cast<T *>(const_cast<void *>(r.which ? a.values : a.keys)) + r.head * a.key_head + r.piece * 8;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    if (r.token(p) >= a.tokens) continue;
+    const float s = scale_operand(scale[p]);
+    const f32x2 y[4] = {decode2_f32<0>(codes[p], s), decode2_f32<1>(codes[p], s), decode2_f32<2>(codes[p], s),
+                        decode2_f32<3>(codes[p], s)};
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = y[j / 2][j % 2];
+    store8(dst + r.token(p) * a.key_token, x);
+  }
+}
+
+// 64 tokens a workgroup where that makes enough of them to fill the card, else as few as its lanes can hold.
+template <typename T, int DIM>
+void launch_rows(const RowsArgs &a, bool set, hipStream_t s) {
+  constexpr int kMany = DIM / 32, kOne = 2048 / DIM;  // passes for 64 tokens; tokens of one pass
+  const int64_t tiles = 2 * a.v.kv_heads, many = (a.tokens + 63) / 64 * tiles, few = (a.tokens + kOne - 1) / kOne * tiles;
+  const dim3 block(256);
+  if (many >= 1024) {
+    const dim3 grid(static_cast<unsigned>(many));
+    if (set) hipLaunchKernelGGL((page_set_kernel<T, DIM, kMany>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((page_fetch_kernel<T, DIM, kMany>), grid, block, 0, s, a);
+  } else {
+    const dim3 grid(static_cast<unsigned>(few));
+    if (set) hipLaunchKernelGGL((page_set_kernel<T, DIM, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((page_fetch_kernel<T, DIM, 1>), grid, block, 0, s, a);
   }
 }
 
 template <typename T>
 int launch_rows(const RowsArgs &a, int dim, bool set, hipStream_t s) {
-  const int64_t lanes = a.tokens * a.v.kv_heads * 2 * (dim / 8);
-  const dim3 grid(grid_for(lanes, 256, 256 * 32)), block(256);
-  switch (dim) {
-    case 64:
-      if (set) hipLaunchKernelGGL((page_set_kernel<T, 64>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((page_fetch_kernel<T, 64>), grid, block, 0, s, a);
-      break;
-    case 128:
-      if (set) hipLaunchKernelGGL((page_set_kernel<T, 128>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((page_fetch_kernel<T, 128>), grid, block, 0, s, a);
-      break;
-    default:
-      if (set) hipLaunchKernelGGL((page_set_kernel<T, 256>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((page_fetch_kernel<T, 256>), grid, block, 0, s, a);
-  }
+  if (dim == 64) launch_rows<T, 64>(a, set, s);
+  else if (dim == 128) launch_rows<T, 128>(a, set, s);
+  else launch_rows<T, 256>(a, set, s);
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;
 }
@@ -261,7 +380,7 @@ int rows_entry(const shmt_paged_cache *c, const void *slots, int slot_bytes, int
                elem_type);
   if (n == 0) return SHMT_OK;
   SHMT_REQUIRE(slots && keys && values, "slots, keys or values is null");
-  SHMT_REQUIRE(n <= (int64_t{1} << 40) / (int64_t{c->kv_heads} * c->dim), "too many rows in one call");
+  SHMT_REQUIRE(n / 64 < (int64_t{1} << 30) / c->kv_heads, "too many rows in one call");
   const int64_t esize = elem_type == SHMT_F32 ? 4 : 2;
   const int64_t bits = reinterpret_cast<int64_t>(keys) | reinterpret_cast<int64_t>(values) |
                        (key_token | key_head | value_token | value_head) * esize;
@@ -278,7 +397,7 @@ using namespace shmt;
 
 extern "C" {
 
-int64_t shmt_page_plan_scratch_bytes(int64_t requests) { return requests > 0 ? requests * 8 : 0; }
+int64_t shmt_page_plan_scratch_bytes(int64_t requests) { return requests > kPlanOne ? requests * 8 : 0; }
 
 int shmt_page_plan(const void *cached_lens, const void *new_lens, int len_bytes, int64_t requests,
                    int32_t *block_table, int64_t width, int64_t table_stride, const int32_t *free_pages,
@@ -296,19 +415,22 @@ int shmt_page_plan(const void *cached_lens, const void *new_lens, int len_bytes,
   SHMT_REQUIRE(requests == 0 || width == 0 || (block_table && table_stride >= width), "block_table is null or narrow");
   SHMT_REQUIRE(n_free == 0 || free_pages, "free_pages is null");
   SHMT_REQUIRE(max_tokens == 0 || (positions && slots), "positions or slots is null");
-  if (scratch_bytes < shmt_page_plan_scratch_bytes(requests) || (requests > 0 && !scratch)) {
+  if (scratch_bytes < shmt_page_plan_scratch_bytes(requests) || (requests > kPlanOne && !scratch)) {
     set_error("scratch too small: %lld bytes", static_cast<long long>(scratch_bytes));
     return SHMT_ENOMEM;
   }
   const PlanArgs a{cached_lens, new_lens, len_bytes, requests, block_table, width, table_stride,
                    free_pages, n_free, log2_page, max_tokens, query_starts, kv_lens, positions,
-                   slots, counts, static_cast<int64_t *>(scratch)};
+                   slots, counts};
   hipStream_t s = as_stream(stream);
-  hipLaunchKernelGGL(page_plan_scan_kernel, dim3(1), dim3(1024), 0, s, a);
-  if (requests > 0 && width > 0)
-    hipLaunchKernelGGL(page_plan_table_kernel, dim3(grid_for(requests, 4)), dim3(256), 0, s, a);
-  if (max_tokens > 0)
-    hipLaunchKernelGGL(page_plan_tokens_kernel, dim3(grid_for(max_tokens, 256)), dim3(256), 0, s, a);
+  if (requests <= kPlanOne) {
+    hipLaunchKernelGGL(page_plan_one_kernel, dim3(grid_for(std::max(max_tokens, requests * 16), 256, 512)), dim3(256), 0, s, a);
+  } else {
+    int64_t *first_free = static_cast<int64_t *>(scratch);
+    hipLaunchKernelGGL(page_plan_scan_kernel, dim3(1), dim3(1024), 0, s, a, first_free);
+    hipLaunchKernelGGL(page_plan_rest_kernel, dim3(grid_for(std::max(max_tokens, requests * 16), 256)), dim3(256), 0, s, a,
+                       first_free);
+  }
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;
 }

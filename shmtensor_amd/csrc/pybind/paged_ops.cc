@@ -23,6 +23,15 @@ void check_device(const torch::Tensor &t, const torch::Tensor &like, const char 
   TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", the cache on ", like.device());
 }
 
+bool page_contiguous(const torch::Tensor &t) {
+  int64_t want = 1;
+  for (int64_t d = 4; d >= 1; --d) {
+    if (t.size(d) > 1 && t.stride(d) != want) return false;
+    want *= t.size(d);
+  }
+  return true;
+}
+
 shmt_paged_cache describe(const torch::Tensor &cache, const torch::Tensor &scales) {
   TORCH_CHECK(cache.is_cuda(), "cache must be a CUDA tensor");
   TORCH_CHECK(cache.device().index() == c10::hip::current_device(), "cache is on ", cache.device(),
@@ -40,7 +49,7 @@ shmt_paged_cache describe(const torch::Tensor &cache, const torch::Tensor &scale
               cache.sizes());
   TORCH_CHECK(page <= 256 && heads >= 1 && heads <= 65535, "a page must hold 16, 32, 64, 128 or 256 tokens of 1 to 65535 heads");
   // within a page everything is contiguous; pages may lie apart
-  TORCH_CHECK(pages == 0 || (cache.select(0, 0).is_contiguous() && scales.select(0, 0).is_contiguous()),
+  TORCH_CHECK(pages == 0 || (page_contiguous(cache) && page_contiguous(scales)),
               "the pages of cache and scales must be contiguous");
   shmt_paged_cache c;
   c.cache = cache.data_ptr();
@@ -102,12 +111,13 @@ std::vector<torch::Tensor> page_plan(torch::Tensor cached_lens, torch::Tensor ne
   torch::Tensor positions = torch::empty({max_tokens}, i32), slots = torch::empty({max_tokens}, i64);
   torch::Tensor counts = torch::empty({2}, i64);
   const int64_t scratch_bytes = shmt_page_plan_scratch_bytes(n);
-  torch::Tensor scratch = device_bytes(scratch_bytes);
+  torch::Tensor scratch = scratch_bytes > 0 ? device_bytes(scratch_bytes) : torch::Tensor();
   check(shmt_page_plan(cached_lens.data_ptr(), new_lens.data_ptr(), static_cast<int>(cached_lens.element_size()), n,
                        block_table.data_ptr<int32_t>(), block_table.size(1), stride, free_pages.data_ptr<int32_t>(),
                        free_pages.numel(), static_cast<int>(page), max_tokens, starts.data_ptr<int32_t>(),
                        kv_lens.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
-                       counts.data_ptr<int64_t>(), scratch.data_ptr(), scratch_bytes, current_stream()));
+                       counts.data_ptr<int64_t>(), scratch_bytes > 0 ? scratch.data_ptr() : nullptr, scratch_bytes,
+                       current_stream()));
   return {starts, kv_lens, positions, slots, counts};
 }
 
