@@ -449,7 +449,7 @@ struct JoinShared {
 };
 
 // Waves per SIMD that the registers are meant for.
-constexpr int attn_waves(int dim, int tiles) { return tiles * dim <= 128 ? 3 : tiles * dim <= 512 ? 2 : 1; }
+constexpr int attn_waves(int dim, int tiles) { return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2; }
 
 template <typename T, int DIM, int NT>
 __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kernel(
@@ -821,57 +821,106 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   }
 }
 
-// Puts the parts of an item together: a workgroup for a row of a record, a part for each DIM / 4 threads at a time.
+// Puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
+// rows to join (a grid that has a workgroup for each row that there could be takes longer to start than to run). Where they
+// are few, a workgroup takes one at a time, its teams of DIM / 4 threads a part each; else every team takes a row.
+constexpr int kMostGroups = 256 * 4;
+
 template <typename T, int DIM, int ROWS>
 __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, const float *parts, const float *part_stats,
-                                                                  const JoinRecord *records) {
-  constexpr int kLanes = DIM / 4, kTeams = 256 / kLanes;
+                                                                  const JoinRecord *records, int groups) {
+  constexpr int kLanes = DIM / 4, kTeams = 256 / kLanes, kEach = kMostGroups / 256;
+  __shared__ uint32_t before[kMostGroups + 1];  // rows to join in front of each workgroup's record
+  __shared__ uint32_t scan[4];
   __shared__ f32x4 acc_shared[kTeams][kLanes];
   __shared__ float top_shared[kTeams], sum_shared[kTeams];
-  const int64_t wg = blockIdx.x;
-  const JoinRecord rec = records[wg];
-  const int r = blockIdx.y;
-  if (rec.first < 0 || r >= rec.rows) return;
-  const int team = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  float top = kNothing, sum = 0;
-  f32x4 acc = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int64_t w = rec.first + team; w <= wg; w += kTeams) {
-    const int64_t line = (2 * w + (w == rec.first ? 1 : 0)) * ROWS + r;
-    const float m = part_stats[line * 2], l = part_stats[line * 2 + 1];
-    const f32x4 o = *reinterpret_cast<const f32x4 *>(parts + line * DIM + lane * 4);
-    const float next = fmaxf(top, m), base = fmaxf(next, kLowest);
-    const float f = __builtin_amdgcn_exp2f(top - base), e = __builtin_amdgcn_exp2f(m - base);
-    sum = sum * f + l * e;
-    acc = acc * f + o * e;
-    top = next;
+  uint32_t rows[kEach], mine = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int w = threadIdx.x * kEach + i;
+    rows[i] = w < groups && records[w].first >= 0 ? records[w].rows : 0;
   }
-  acc_shared[team][lane] = acc;
-  if (lane == 0) top_shared[team] = top, sum_shared[team] = sum;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) mine += rows[i];
+  uint32_t total;
+  uint32_t at = block_exclusive_scan<uint32_t, 256>(mine, scan, &total);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) before[threadIdx.x * kEach + i] = at, at += rows[i];
+  if (threadIdx.x == 0) before[kMostGroups] = total;
   __syncthreads();
-  if (team != 0) return;
-  for (int i = 1; i < kTeams; ++i) top = fmaxf(top, top_shared[i]);
-  const float base = fmaxf(top, kLowest);
-  sum = 0, acc = f32x4{0, 0, 0, 0};
-  for (int i = 0; i < kTeams; ++i) {
-    const float f = __builtin_amdgcn_exp2f(top_shared[i] - base);
-    sum += f * sum_shared[i];
-    acc += f * acc_shared[i][lane];
+  const int team = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const bool few = total <= 2 * gridDim.x;
+  const uint32_t step = few ? 1 : kTeams;
+  for (uint32_t base_row = blockIdx.x * step; base_row < total; base_row += gridDim.x * step) {
+    const uint32_t row_at = few ? base_row : base_row + team;
+    float top = kNothing, sum = 0;
+    f32x4 acc = {0, 0, 0, 0};
+    int64_t line_out = 0;
+    if (row_at < total) {
+      int w_end = 0, last = groups - 1;  // the last record with no more rows in front of it
+      while (w_end < last) {
+        const int mid = (w_end + last + 1) >> 1;
+        if (before[mid] <= row_at) w_end = mid; else last = mid - 1;
+      }
+      const JoinRecord rec = records[w_end];
+      const int r = row_at - before[w_end];
+      const uint32_t row = rec.row0 + r, token = row / static_cast<uint32_t>(a.group);
+      line_out = (rec.first_row + token) * a.heads + rec.head * a.group + (row - token * a.group);
+      constexpr int kBatch = 4;  // parts in flight
+      const int stride = few ? kTeams : 1;
+      for (int w0 = rec.first + (few ? team : 0); w0 <= w_end; w0 += stride * kBatch) {
+        f32x2 stats[kBatch];
+        f32x4 o[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int64_t w = min(w0 + i * stride, w_end);
+          const int64_t line = (2 * w + (w == rec.first ? 1 : 0)) * ROWS + r;
+          stats[i] = *reinterpret_cast<const f32x2 *>(part_stats + line * 2);
+          o[i] = *reinterpret_cast<const f32x4 *>(parts + line * DIM + lane * 4);
+        }
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) next = fmaxf(next, stats[i][0]);
+        const float base = fmaxf(next, kLowest), f = __builtin_amdgcn_exp2f(top - base);
+        sum *= f, acc *= f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (w0 + i * stride > w_end) continue;
+          const float e = __builtin_amdgcn_exp2f(stats[i][0] - base);
+          sum += stats[i][1] * e;
+          acc += o[i] * e;
+        }
+        top = next;
+      }
+    }
+    if (few) {
+      acc_shared[team][lane] = acc;
+      if (lane == 0) top_shared[team] = top, sum_shared[team] = sum;
+      __syncthreads();
+      for (int i = 0; i < kTeams; ++i) top = fmaxf(top, top_shared[i]);
+      const float base = fmaxf(top, kLowest);
+      sum = 0, acc = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < kTeams; ++i) {
+        const float f = __builtin_amdgcn_exp2f(top_shared[i] - base);
+        sum += f * sum_shared[i];
+        acc += f * acc_shared[i][lane];
+      }
+      __syncthreads();
+    }
+    if (row_at < total && (!few || team == 0)) {
+      const float inv = sum == 0 ? 0 : 1 / sum;
+      typedef T out_vec __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<out_vec *>(static_cast<T *>(a.out) + line_out * DIM + lane * 4) = out_vec{
+          static_cast<T>(acc[0] * inv), static_cast<T>(acc[1] * inv), static_cast<T>(acc[2] * inv), static_cast<T>(acc[3] * inv)};
+      if (a.lse && lane == 0) a.lse[line_out] = sum == 0 ? kNothing : (top + __builtin_log2f(sum)) * 0.69314718055994530942f;
+    }
   }
-  const uint32_t row = rec.row0 + r, token = row / static_cast<uint32_t>(a.group);
-  const int64_t line = (rec.first_row + token) * a.heads + rec.head * a.group + (row - token * a.group);
-  const float inv = sum == 0 ? 0 : 1 / sum;
-  typedef T out_vec __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<out_vec *>(static_cast<T *>(a.out) + line * DIM + lane * 4) = out_vec{
-      static_cast<T>(acc[0] * inv), static_cast<T>(acc[1] * inv), static_cast<T>(acc[2] * inv), static_cast<T>(acc[3] * inv)};
-  if (a.lse && lane == 0) a.lse[line] = sum == 0 ? kNothing : (top + __builtin_log2f(sum)) * 0.69314718055994530942f;
 }
 
 // ---- launch ------------------------------------------------------------------------
 
 struct AttnShape {
   int tiles;       // of 16 rows an item
-  int rows;        // the most that an item has
   int64_t groups;  // workgroups
   int64_t items;   // room in the list of items; 0: none, every request is one item of a head
   int64_t parts_bytes, stats_bytes, record_bytes, item_bytes, first_bytes;
@@ -884,7 +933,6 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, in
   const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
   s.tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-  s.rows = static_cast<int>(std::min<int64_t>(rows, 16 * s.tiles));
   s.groups = 256 * attn_waves(dim, s.tiles);
   s.items = rows > 16 * s.tiles ? tokens * group / (16 * s.tiles) + requests : 0;
   const int64_t lines = 2 * s.groups * 16 * s.tiles;
@@ -911,11 +959,13 @@ void launch_tiles(const AttnArgs &a, const AttnShape &s, void *scratch, hipStrea
     hipLaunchKernelGGL((page_attention_items_kernel<16 * NT>), dim3(1), dim3(1024), 0, stream, a, first_item, items,
                        s.items, count);
   }
-  const unsigned groups = static_cast<unsigned>(s.groups);
+  // no more workgroups than there can be units
+  const int64_t units = (a.tokens * a.group / (16 * NT) + a.requests) * a.v.kv_heads * (a.limit / kUnit + 1);
+  const unsigned groups = static_cast<unsigned>(std::min(s.groups, std::max<int64_t>(units, 1)));
   hipLaunchKernelGGL((page_attention_kernel<T, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, items, count, parts, stats,
                      records);
-  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(groups, 16 * NT), dim3(256), 0, stream, a, parts,
-                     stats, records);
+  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(std::min(groups, 512u)), dim3(256), 0, stream, a,
+                     parts, stats, records, static_cast<int>(groups));
 }
 
 template <typename T, int DIM>
