@@ -233,13 +233,37 @@ __device__ __forceinline__ LaneOffsets lane_offsets(int lane, int page) {
   return o;
 }
 
-// Loads the 16 tokens at place `off` of page `at` (both the same for the wave).
+// Where 16 tokens of one head lie: the first one's key and its scale. Lanes hold those of the tokens to come; a wave takes one
+// lane's for a load, so that nothing of it is computed per lane or per step.
+struct Place16 {
+  uint32_t row_lo, row_hi, scale_lo, scale_hi;
+  __device__ __forceinline__ Place16 of_lane(int l) const {
+    return {static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, l)), static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, l)),
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(scale_lo, l)),
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(scale_hi, l))};
+  }
+  __device__ __forceinline__ const uint8_t *row() const {
+    return reinterpret_cast<const uint8_t *>(static_cast<uint64_t>(row_hi) << 32 | row_lo);
+  }
+  __device__ __forceinline__ const uint8_t *scale() const {
+    return reinterpret_cast<const uint8_t *>(static_cast<uint64_t>(scale_hi) << 32 | scale_lo);
+  }
+};
+// Those of page `at` from the place of token j on.
 template <int DIM>
-__device__ __forceinline__ void load_half(const PagedView &v, int head, int at, int off, const LaneOffsets &o, int half,
-                                          KvTile<DIM> &t) {
+__device__ __forceinline__ Place16 place16(const PagedView &v, int head, int at, int j) {
+  const int off = j & ((1 << v.log2_page) - 1);
   const int64_t tile = int64_t{2} * head << v.log2_page;
-  const uint8_t *rows = v.cache + at * v.cache_stride + (tile + off) * (DIM / 2);
-  const uint8_t *sc = v.scales + at * v.scales_stride + tile * (DIM / 32) + off;
+  const uint64_t row = reinterpret_cast<uint64_t>(v.cache + at * v.cache_stride + (tile + off) * (DIM / 2));
+  const uint64_t scale = reinterpret_cast<uint64_t>(v.scales + at * v.scales_stride + tile * (DIM / 32) + off);
+  return {static_cast<uint32_t>(row), static_cast<uint32_t>(row >> 32), static_cast<uint32_t>(scale),
+          static_cast<uint32_t>(scale >> 32)};
+}
+
+// Loads 16 tokens.
+template <int DIM>
+__device__ __forceinline__ void load_half(const Place16 &at, int page, const LaneOffsets &o, int half, KvTile<DIM> &t) {
+  const uint8_t *rows = at.row(), *sc = at.scale();
   if constexpr (DIM == 64) {
     const uint2 x = *reinterpret_cast<const uint2 *>(rows + o.key);
     t.key[half][0] = x.x, t.key[half][1] = x.y;
@@ -247,9 +271,9 @@ __device__ __forceinline__ void load_half(const PagedView &v, int head, int at, 
   } else {
 #pragma unroll
     for (int i = 0; i < DIM / 128; ++i) {
-      const uint4 x = reinterpret_cast<const uint4 *>(rows + o.key)[i];
+      const uint4 x = *reinterpret_cast<const uint4 *>(rows + o.key + 16 * i);
       t.key[half][4 * i] = x.x, t.key[half][4 * i + 1] = x.y, t.key[half][4 * i + 2] = x.z, t.key[half][4 * i + 3] = x.w;
-      t.key_scale[half][i] = sc[o.key_scale + (i << v.log2_page)];
+      t.key_scale[half][i] = sc[o.key_scale + i * page];
     }
   }
 #pragma unroll

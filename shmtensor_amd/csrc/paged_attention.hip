@@ -119,40 +119,41 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
     const int first = same(static_cast<int>(u - u_item));
     const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item));
     auto token_of = [&](int k) { return unit_token(span, k) + wave * kWaveTokens; };  // unit k's first token of this wave
-    // Whether all rows see all of a wave's 32 tokens from token0 on, on pages p0 and p1.
-    auto tile_whole = [&](int token0, int p0, int p1) {
-      return p0 >= 0 && p1 >= 0 && token0 + kWaveTokens - 1 <= pos_first &&
+    // Whether all rows see all of a wave's 32 tokens from token0 on, of which `there` are present.
+    auto tile_whole = [&](int token0, uint32_t there) {
+      return there == 3 && token0 + kWaveTokens - 1 <= pos_first &&
              (token0 > after_last || token0 + kWaveTokens <= sight.sinks);
     };
-    // The pages of the next 32 units' tokens, one 16 of them a lane: -1 where no row sees any.
-    int page_of = -1, page_base = 0;
+    // Where the next 32 units' tokens lie, 16 a lane, and of which of them any row sees any.
+    Place16 places;
+    uint64_t present = 0;
+    int page_base = 0;
     auto look_up = [&](int k0) {
       page_base = k0;
-      const int k = k0 + (lane >> 1);
-      page_of = k < last ? page_at(a, table, span, token_of(k) + 16 * (lane & 1)) : -1;
+      const int k = k0 + (lane >> 1), j = token_of(k) + 16 * (lane & 1);
+      const int p = k < last ? page_at(a, table, span, j) : -1;
+      places = place16<DIM>(a.v, head, max(p, 0), j);  // what is not there is loaded from page 0 and not looked at
+      present = __ballot(p >= 0);
     };
     struct Step {
-      int token0, page0, page1;
+      int token0;
+      uint32_t there;  // a bit for each 16 tokens
     };
+    auto present_of = [&](int k) { return static_cast<uint32_t>(present >> (2 * (k - page_base))) & 3u; };
     // The next unit from k on that has anything for this wave; `last` if there is none.
     auto find = [&](int k) {
       for (; k < last; ++k) {
         if (k - page_base >= 32) look_up(k);
-        const int at = 2 * (k - page_base);
-        if (__builtin_amdgcn_readlane(page_of, at) >= 0 || __builtin_amdgcn_readlane(page_of, at + 1) >= 0) break;
+        if (present_of(k)) break;
       }
       return k;
     };
     KvTile<DIM> ahead;
     auto fetch = [&](int k) {
-      Step s;
-      s.token0 = token_of(k);
-      s.page0 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base));
-      s.page1 = __builtin_amdgcn_readlane(page_of, 2 * (k - page_base) + 1);
-      const int mask = (1 << a.v.log2_page) - 1;  // a half that is not there is loaded as page 0 and not looked at
-      load_half<DIM>(a.v, head, max(s.page0, 0), s.token0 & mask, offsets, 0, ahead);
-      load_half<DIM>(a.v, head, max(s.page1, 0), (s.token0 + 16) & mask, offsets, 1, ahead);
-      return s;
+      const int at = 2 * (k - page_base);
+      load_half<DIM>(places.of_lane(at), 1 << a.v.log2_page, offsets, 0, ahead);
+      load_half<DIM>(places.of_lane(at + 1), 1 << a.v.log2_page, offsets, 1, ahead);
+      return Step{token_of(k), present_of(k)};
     };
     bool wild = false, again;
     RowState<DIM, NT> st;
@@ -179,8 +180,8 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
         k = find(k + 1);
         more = k < last;
         if (more) next = fetch(k);
-        const bool whole = tile_whole(now.token0, now.page0, now.page1);
-        again = attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.page0 >= 0, now.page1 >= 0, sight,
+        const bool whole = tile_whole(now.token0, now.there);
+        again = attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.there & 1, now.there & 2, sight,
                                              wild);
       } while (more && !again);
     } while (again);
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
               for (int w = 0; w < kUnit / kWaveTokens; ++w) {
                 const int t0 = unit_token(span, k) + w * kWaveTokens;
                 const int p0 = page_at(a, table, span, t0), p1 = page_at(a, table, span, t0 + 16);
-                if (tile_whole(t0, p0, p1)) continue;
+                if (tile_whole(t0, (p0 >= 0 ? 1u : 0u) | (p1 >= 0 ? 2u : 0u))) continue;
                 add_left_out<T, DIM>(a, head, p0, t0, q_row, sees, scale2, base, d0, o);
                 add_left_out<T, DIM>(a, head, p1, t0 + 16, q_row, sees, scale2, base, d0, o);
               }

@@ -4,6 +4,10 @@
 
 namespace shmt {
 
+// Beginning and ending an item costs about as much as this many units do: so many are added to each, with no tokens in
+// them, for the sake of even shares.
+constexpr int kItemCost = 2;
+
 // Items of all requests with the units in front of each, for calls in which a request has many row tiles: one workgroup.
 // items[0 .. n) and, behind the last, the number of units; *count = n. (Only starts that descend could make more items than
 // there is room for.)
@@ -35,7 +39,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
         if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
       }
       row0 = static_cast<int>(i - first_item[lo]) * ROWS;
-      mine = attn_span<ROWS>(a, attn_request(a, lo), row0).units;
+      mine = attn_span<ROWS>(a, attn_request(a, lo), row0).units + kItemCost;
     }
     uint64_t sum;
     const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
@@ -135,7 +139,8 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     const int64_t b = same(it.request);
     const int row0 = same(it.row0);
     const Request req = same(attn_request(a, b));
-    const Span span = same(attn_span<kRows>(a, req, row0));
+    Span span = same(attn_span<kRows>(a, req, row0));
+    span.units += kItemCost;
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
     int see_last[NT], see_after[NT];
@@ -163,19 +168,26 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item)) * kSub;
 
     auto token_of = [&](int t) { return unit_token(span, t / kSub) + t % kSub * kTile; };  // of the item's tile t
-    // The pages of the next tiles, 16 tokens a lane: -1 where no row sees any of them.
+    // Where the next tiles' tokens lie, 16 tokens a lane, and of which of them any row sees any.
     constexpr int kAhead = kWave / kHalves;
-    int page_of = -1, page_base = 0;
+    Place16 places;
+    uint64_t present = 0;
+    int page_base = 0;
     auto look_up = [&](int t0) {
       page_base = t0;
-      const int t = t0 + lane / kHalves;
-      page_of = t < last ? page_at(a, table, span, token_of(t) + lane % kHalves * 16) : -1;
+      const int t = t0 + lane / kHalves, j = token_of(t) + lane % kHalves * 16;
+      const int p = t < last ? page_at(a, table, span, j) : -1;
+      places = place16<DIM>(a.v, head, max(p, 0), j);  // what is not there is loaded from page 0 and not looked at
+      present = __ballot(p >= 0);
+    };
+    auto present_of = [&](int t) {
+      return static_cast<uint32_t>(present >> ((t - page_base) * kHalves)) & ((1u << kHalves) - 1);
     };
     // The next tile from t on of which any row sees something; `last` if there is none.
     auto find = [&](int t) {
       for (; t < last; ++t) {
         if (t - page_base >= kAhead) look_up(t);
-        if (__ballot(page_of >= 0) >> ((t - page_base) * kHalves) & ((1u << kHalves) - 1)) break;
+        if (present_of(t)) break;
       }
       return t;
     };
@@ -189,36 +201,33 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
       return there == (1u << kHalves) - 1 && token0 + kTile - 1 <= pos_first &&
              (token0 > after_last || token0 + kTile <= sinks);
     };
-    auto fetch = [&](int t) {  // what is not there is loaded as page 0 and not looked at
+    auto fetch = [&](int t) {
       Step s;
       s.token0 = token_of(t);
-      s.there = static_cast<uint32_t>(__ballot(page_of >= 0) >> ((t - page_base) * kHalves)) & ((1u << kHalves) - 1);
+      s.there = present_of(t);
       s.whole = sees_all(s.token0, s.there, item_first, item_after);
-      const int64_t tile = int64_t{2} * head << a.v.log2_page;
-      auto at = [&](int half) { return max(__builtin_amdgcn_readlane(page_of, (t - page_base) * kHalves + half), 0); };
+      const int at = (t - page_base) * kHalves;
       {
-        const int p = at(key_half), off = (s.token0 + 16 * key_half) & (page - 1);
-        const uint8_t *x = a.v.cache + p * a.v.cache_stride + (tile + off) * (DIM / 2) + key_at;
+        const Place16 x = places.of_lane(at + key_half);
         if constexpr (DIM == 64) {
-          const uint2 y = *reinterpret_cast<const uint2 *>(x);
+          const uint2 y = *reinterpret_cast<const uint2 *>(x.row() + key_at);
           raw.key[0] = y.x, raw.key[1] = y.y;
         } else {
-          const uint4 y = *reinterpret_cast<const uint4 *>(x);
+          const uint4 y = *reinterpret_cast<const uint4 *>(x.row() + key_at);
           raw.key[0] = y.x, raw.key[1] = y.y, raw.key[2] = y.z, raw.key[3] = y.w;
         }
-        raw.key_scale = (a.v.scales + p * a.v.scales_stride + tile * (DIM / 32) + off)[key_scale_at];
+        raw.key_scale = x.scale()[key_scale_at];
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int p = at(2 * value_group + half), off = (s.token0 + 32 * value_group + 16 * half) & (page - 1);
-        const uint8_t *x = a.v.cache + p * a.v.cache_stride + (tile + off) * (DIM / 2) + value_at;
+        const Place16 x = places.of_lane(at + 2 * value_group + half);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if constexpr (DIM == 64) raw.value[4 * half + r] = *reinterpret_cast<const uint16_t *>(x + r * (DIM / 2));
-          else raw.value[4 * half + r] = *reinterpret_cast<const uint32_t *>(x + r * (DIM / 2));
+          const uint8_t *y = x.row() + value_at + r * (DIM / 2);
+          if constexpr (DIM == 64) raw.value[4 * half + r] = *reinterpret_cast<const uint16_t *>(y);
+          else raw.value[4 * half + r] = *reinterpret_cast<const uint32_t *>(y);
         }
-        raw.value_scale[half] = *reinterpret_cast<const uint32_t *>(a.v.scales + p * a.v.scales_stride + tile * (DIM / 32) +
-                                                                    off + value_scale_at);
+        raw.value_scale[half] = *reinterpret_cast<const uint32_t *>(x.scale() + value_scale_at);
       }
       return s;
     };
@@ -284,6 +293,18 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     auto multiply = [&](const Step &s, const ManyStage<DIM> &from) {
       const bool whole = sees_all(s.token0, s.there, wave_first, wave_after);
       bool passed = false;
+      // All fragments of a product are on their way from LDS before it begins: those of the values under the softmax, those
+      // of the next keys under the values' product. Reads of LDS keep their place at the fences, all else may move.
+      auto fence = [] { __builtin_amdgcn_sched_barrier(0x67f); };
+      u32x4 keys[kSteps][2], values[Shape::kValueFrags];
+      auto read_keys = [&](int group) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) keys[i][half] = from.key[2 * group + half][i][lane];
+        fence();
+      };
+      read_keys(0);
 #pragma unroll
       for (int group = 0; group < Shape::kGroups; ++group) {
         f32x4 x[NT][2];
@@ -292,13 +313,14 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const u32x4 k = from.key[2 * group + half][i][lane];
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int p = 0; p < kParts; ++p) x[n][half] = mfma(k, q[p][n][i], x[n][half]);
-          }
+              for (int p = 0; p < kParts; ++p) x[n][half] = mfma(keys[i][half], q[p][n][i], x[n][half]);
+#pragma unroll
+        for (int i = 0; i < Shape::kValueFrags; ++i) values[i] = from.value[group][i][lane];
+        fence();
         if (!whole) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -320,14 +342,13 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
           if (most > st.top[n] + 40.0f) passed = true, st.top[n] = most;
           weights<kParts>(x[n], scale2, st.top[n], st.sum[n], w, n);
         }
+        if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
-        for (int i = 0; i < Shape::kValueFrags; ++i) {
-          const u32x4 v = from.value[group][i][lane];
+        for (int i = 0; i < Shape::kValueFrags; ++i)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) st.acc[n][i] = mfma(v, w[p][n], st.acc[n][i]);
-        }
+            for (int p = 0; p < kParts; ++p) st.acc[n][i] = mfma(values[i], w[p][n], st.acc[n][i]);
       }
       return __ballot(passed) != 0;
     };
