@@ -341,6 +341,48 @@ __device__ __forceinline__ void weights(const f32x4 (&s)[2], float scale2, float
   }
 }
 
+// References. Weights are taken relative to the maximum of the first tile in which a row sees anything: with floats' exponents
+// any reference near the true maximum does as well as that, so there is no maximum to follow from tile to tile and nothing to
+// rescale. Only a sum of weights above 2^40, which takes scores that ordinary ones do not come near, makes a wave begin its
+// tokens again, with a greater reference.
+constexpr float kPassed = 1099511627776.0f;  // 2^40
+
+template <int NT>
+__device__ __forceinline__ float most_of(const f32x4 (&s)[NT][2], int n, float scale2) {
+  float x = s[n][0][0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n][j / 4][j % 4]);
+  return across_max(x) * scale2;
+}
+
+// Rows without a reference take this tile's maximum. Returns whether any is still without.
+template <int NT, typename State>
+__device__ __forceinline__ bool first_reference(const f32x4 (&s)[NT][2], float scale2, State &st) {
+  bool none = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float most = most_of<NT>(s, n, scale2);
+    st.top[n] = st.top[n] == kNothing ? most : st.top[n];
+    none |= st.top[n] == kNothing;
+  }
+  return __ballot(none) != 0;
+}
+
+// Where a row's sum has passed 2^40: a reference that is greater by 2^20 at least. Returns whether there is such a row.
+template <int NT, typename State>
+__device__ __forceinline__ bool raise_reference(const f32x4 (&s)[NT][2], float scale2, State &st) {
+  bool passed = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) passed |= st.sum[n] > kPassed;
+  if (!__ballot(passed)) return false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float most = most_of<NT>(s, n, scale2);
+    if (across_max(st.sum[n]) > kPassed) st.top[n] = fmaxf(st.top[n] + 20.0f, most);
+  }
+  return true;
+}
+
 // Scale bytes from here on make values that are infinite in bfloat16, or not a number.
 constexpr uint32_t kWild = 253;
 
@@ -357,7 +399,7 @@ constexpr uint32_t kWild = 253;
 template <int DIM, int NT, int PARTS>
 __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int lane, bool whole, int token0, bool there0, bool there1,
-                                            const Sight<NT> &sight, bool &wild) {
+                                            const Sight<NT> &sight, bool &wild, bool &waiting) {
   const int g = lane >> 4;
   f32x4 s[NT][2];
 #pragma unroll
@@ -400,24 +442,11 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
         wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
       }
   }
-  // Weights are taken relative to the maximum of the first tile in which a row saw anything. With floats' exponents any
-  // reference near the true maximum does as well, so nothing is rescaled; where a score passes it by 2^40, which ordinary
-  // scores do not, the wave begins its tokens again with the greater one.
-  bool passed = false;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float x = s[n][0][0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n][j / 4][j % 4]);
-    const float most = across_max(x) * scale2;
-    st.top[n] = st.top[n] == kNothing ? most : st.top[n];
-    if (most > st.top[n] + 40.0f) passed = true, st.top[n] = most;
-  }
+  if (waiting) waiting = first_reference<NT>(s, scale2, st);
   u32x4 w[PARTS][NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    weights<PARTS>(s[n], scale2, st.top[n], st.sum[n], w, n);
-  }
+  for (int n = 0; n < NT; ++n) weights<PARTS>(s[n], scale2, st.top[n], st.sum[n], w, n);
+  const bool again = raise_reference<NT>(s, scale2, st);
   // The conversion reads nothing of a scale but its exponent field, so the byte need not be cut out.
   float f[8];
 #pragma unroll
@@ -452,7 +481,7 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
       two(std::integral_constant<int, 3>{});
     }
   }
-  return __ballot(passed) != 0;
+  return again;
 }
 
 // Eight values of a query row as a fragment: bfloat16 as they are, float16 as the sum of two.
@@ -544,7 +573,7 @@ __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, co
   if (threadIdx.x == 0) before[kMostGroups] = total;
   __syncthreads();
   const int team = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  const bool few = total <= 2 * gridDim.x;
+  const bool few = total <= 1024;
   const uint32_t step = few ? 1 : kTeams;
   for (uint32_t base_row = blockIdx.x * step; base_row < total; base_row += gridDim.x * step) {
     const uint32_t row_at = few ? base_row : base_row + team;

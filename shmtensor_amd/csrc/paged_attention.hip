@@ -155,10 +155,10 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       load_half<DIM>(places.of_lane(at + 1), 1 << a.v.log2_page, offsets, 1, ahead);
       return Step{token_of(k), present_of(k)};
     };
-    bool wild = false, again;
+    bool wild = false, again, waiting = true;
     RowState<DIM, NT> st;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) st.top[n] = kNothing;
+    for (int n = 0; n < NT; ++n) st.top[n] = 16 * n + n_lane < rows ? kNothing : 0;  // what is not a row waits for nothing
     // Nothing in this loop changes the accumulators but the products, on every way through it: only so do they stay in one
     // place.
     do {
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
         if (more) next = fetch(k);
         const bool whole = tile_whole(now.token0, now.there);
         again = attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.there & 1, now.there & 2, sight,
-                                             wild);
+                                             wild, waiting);
       } while (more && !again);
     } while (again);
     u = u_item + last;

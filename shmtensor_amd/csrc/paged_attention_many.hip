@@ -288,8 +288,9 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
 
     RowState<DIM, NT> st;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) st.top[n] = kNothing;
-    // A wave's rows and the tile in `from`. Returns whether a row's score passed its reference by 2^40 (see attend_tile).
+    for (int n = 0; n < NT; ++n) st.top[n] = wave * 32 + 16 * n + n_lane < rows ? kNothing : 0;  // no row waits for nothing
+    bool waiting = true;
+    // A wave's rows and the tile in `from`. Returns whether the item has to be begun again (see raise_reference).
     auto multiply = [&](const Step &s, const ManyStage<DIM> &from) {
       const bool whole = sees_all(s.token0, s.there, wave_first, wave_after);
       bool passed = false;
@@ -331,17 +332,11 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
               x[n][j / 4][j % 4] = sees ? x[n][j / 4][j % 4] : kNothing;
             }
         }
+        if (waiting) waiting = first_reference<NT>(x, scale2, st);
         u32x4 w[kParts][NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float top = x[n][0][0];
-#pragma unroll
-          for (int j = 1; j < 8; ++j) top = fmaxf(top, x[n][j / 4][j % 4]);
-          const float most = across_max(top) * scale2;
-          st.top[n] = st.top[n] == kNothing ? most : st.top[n];
-          if (most > st.top[n] + 40.0f) passed = true, st.top[n] = most;
-          weights<kParts>(x[n], scale2, st.top[n], st.sum[n], w, n);
-        }
+        for (int n = 0; n < NT; ++n) weights<kParts>(x[n], scale2, st.top[n], st.sum[n], w, n);
+        passed |= raise_reference<NT>(x, scale2, st);
         if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
         for (int i = 0; i < Shape::kValueFrags; ++i)
@@ -350,7 +345,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
 #pragma unroll
             for (int p = 0; p < kParts; ++p) st.acc[n][i] = mfma(values[i], w[p][n], st.acc[n][i]);
       }
-      return __ballot(passed) != 0;
+      return passed;
     };
 
     bool again;
@@ -466,7 +461,7 @@ static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s
                      s.count);
   hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(256), 0, stream, a, s.items, s.count, s.parts,
                      s.stats, s.records);
-  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, kManyRows>), dim3(std::min(groups, 512u)), dim3(256), 0, stream, a,
+  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, kManyRows>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }
 
