@@ -32,7 +32,8 @@ struct AttnArgs {
 // An item is up to kRows rows against one head of the cache: a row is a query token and a head of the group that shares the
 // cache's head, row r of a request being token r / group, head r % group. The tokens that an item's rows see are cut at
 // multiples of kUnit: the tiles that hold first tokens ("sinks"), then those from the window's begin to the last row's own
-// place. Units are numbered head by head, request by request, row tile by row tile; workgroup w of G takes units
+// place. Units are numbered (few rows: request by request, head by head, row tile by row tile; many: head by head, request by
+// request, row tile by row tile), and workgroup w of G takes units
 // floor(w U / G) up to floor((w + 1) U / G), so all end at about the same time whatever the lengths are. An item may be
 // shared by several workgroups; each leaves a part (maximum, sum, weighted values), which page_attention_join_kernel puts
 // together.
@@ -40,6 +41,10 @@ constexpr int kUnit = 128;  // tokens: four waves of 32
 constexpr int kWaveTokens = 32;
 constexpr float kNothing = -__builtin_inff();
 constexpr float kLowest = -3.0e38f;  // subtracted instead of kNothing, so that nothing stays nothing
+
+// Beginning and ending an item costs about as much as this many units: so many are added to each, without tokens in them, for
+// the sake of even shares.
+constexpr int item_cost(int rows) { return rows > 32 ? 2 : 1; }
 
 struct AttnItem {
   int64_t unit;  // units of one head in front of it
@@ -105,7 +110,7 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
   s.tile0 = s.begin / kUnit;
   s.sink_end = min(a.sinks, s.begin);
   s.sink_tiles = min((s.sink_end + kUnit - 1) / kUnit, s.tile0);
-  s.units = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1);
+  s.units = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1) + item_cost(ROWS);
   return s;
 }
 

@@ -38,34 +38,34 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   // Where this workgroup's units begin: each thread counts a run of requests.
   const int64_t each = (a.requests + 255) / 256, b_lo = min(threadIdx.x * each, a.requests), b_hi = min(b_lo + each, a.requests);
   int64_t mine = 0;
-  for (int64_t i = b_lo; i < b_hi; ++i) mine += attn_units<kRows>(a, attn_request(a, i));
+  for (int64_t i = b_lo; i < b_hi; ++i) mine += attn_units<kRows>(a, attn_request(a, i)) * kv_heads;
   uint64_t total;
   const int64_t at =
       static_cast<int64_t>(block_exclusive_scan<uint64_t, 256>(static_cast<uint64_t>(mine), shared.scan, &total));
-  const int64_t per_head = same(static_cast<int64_t>(total));
-  const int64_t U = per_head * kv_heads;
-  // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same pages. With fewer
-  // units than workgroups each has one, on all XCDs.
+  const int64_t U = same(static_cast<int64_t>(total));
+  // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same lines of scales and
+  // of the table. With fewer units than workgroups each has one, on all XCDs.
   const int64_t G = min(int64_t{gridDim.x}, U);
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
   if (threadIdx.x == 0) records[wg].first = -1;
   if (wg >= G) return;
   const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
-  int head = same(static_cast<int>(u_begin / per_head));
-  const int64_t x = u_begin - head * per_head;  // within one head's units
-  if (at <= x && x < at + mine) {
+  if (at <= u_begin && u_begin < at + mine) {
     int64_t i = b_lo, before = at;
     for (;; ++i) {
-      const int64_t n = attn_units<kRows>(a, attn_request(a, i));
-      if (x < before + n) break;
+      const int64_t n = attn_units<kRows>(a, attn_request(a, i)) * kv_heads;
+      if (u_begin < before + n) break;
       before += n;
     }
     found[0] = i, found[1] = before;
   }
   __syncthreads();
-  int64_t b = same(found[0]), u_item = head * per_head + same(found[1]);  // the item's first unit
+  int64_t b = same(found[0]), u_item = same(found[1]);  // the item's first unit
   int row0 = 0;
   Request req = same(attn_request(a, b));
+  const int64_t per_head = same(attn_units<kRows>(a, req));
+  int head = same(static_cast<int>((u_begin - u_item) / per_head));
+  u_item += head * per_head;
   Span span = same(attn_span<kRows>(a, req, 0));
   while (u_item + span.units <= u_begin) {
     u_item += span.units;
@@ -278,10 +278,10 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
     row0 += kRows;
     if (row0 >= req.queries * a.group) {
       row0 = 0;
-      do {
-        if (++b == a.requests) b = 0, ++head;
-        req = same(attn_request(a, b));
-      } while (req.queries == 0);
+      if (++head == kv_heads) {
+        head = 0;
+        do req = same(attn_request(a, ++b)); while (req.queries == 0);
+      }
     }
     span = same(attn_span<kRows>(a, req, row0));
   }

@@ -4,10 +4,6 @@
 
 namespace shmt {
 
-// Beginning and ending an item costs about as much as this many units do: so many are added to each, with no tokens in
-// them, for the sake of even shares.
-constexpr int kItemCost = 2;
-
 // Items of all requests with the units in front of each, for calls in which a request has many row tiles: one workgroup.
 // items[0 .. n) and, behind the last, the number of units; *count = n. (Only starts that descend could make more items than
 // there is room for.)
@@ -39,7 +35,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
         if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
       }
       row0 = static_cast<int>(i - first_item[lo]) * ROWS;
-      mine = attn_span<ROWS>(a, attn_request(a, lo), row0).units + kItemCost;
+      mine = attn_span<ROWS>(a, attn_request(a, lo), row0).units;
     }
     uint64_t sum;
     const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
@@ -139,8 +135,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     const int64_t b = same(it.request);
     const int row0 = same(it.row0);
     const Request req = same(attn_request(a, b));
-    Span span = same(attn_span<kRows>(a, req, row0));
-    span.units += kItemCost;
+    const Span span = same(attn_span<kRows>(a, req, row0));
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
     int see_last[NT], see_after[NT];
