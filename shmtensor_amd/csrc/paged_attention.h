@@ -123,6 +123,12 @@ __device__ __forceinline__ int64_t attn_units(const AttnArgs &a, const Request &
   return n;
 }
 
+// Where a workgroup begins, as the thread that found it tells the others.
+struct Found {
+  Request req;
+  int64_t request, before, units;  // units in front of the request (many: of the item), of the request for one head
+};
+
 // Rows that belong to no request are 0.
 template <typename T, int DIM>
 __device__ __forceinline__ void attn_clear_rows(const AttnArgs &a) {
@@ -550,7 +556,7 @@ __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at
   }
 }
 
-// Puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
+// Clears what belongs to no request, and puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
 // rows to join (a grid that has a workgroup for each row that there could be takes longer to start than to run). Where they
 // are few, a workgroup takes one at a time, its teams of DIM / 4 threads a part each; else every team takes a row.
 constexpr int kMostGroups = 256 * 4;
@@ -563,6 +569,7 @@ __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, co
   __shared__ uint32_t scan[4];
   __shared__ f32x4 acc_shared[kTeams][kLanes];
   __shared__ float top_shared[kTeams], sum_shared[kTeams];
+  attn_clear_rows<T, DIM>(a);
   uint32_t rows[kEach], mine = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {

@@ -28,12 +28,10 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
     uint64_t scan[4];
   };
   __shared__ Shared shared;
-  __shared__ int64_t found[2];
+  __shared__ Found found;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
   const int kv_heads = a.v.kv_heads;
-
-  attn_clear_rows<T, DIM>(a);
 
   // Where this workgroup's units begin: each thread counts a run of requests.
   const int64_t each = (a.requests + 255) / 256, b_lo = min(threadIdx.x * each, a.requests), b_hi = min(b_lo + each, a.requests);
@@ -51,19 +49,22 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   if (wg >= G) return;
   const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
   if (at <= u_begin && u_begin < at + mine) {
-    int64_t i = b_lo, before = at;
-    for (;; ++i) {
-      const int64_t n = attn_units<kRows>(a, attn_request(a, i)) * kv_heads;
-      if (u_begin < before + n) break;
-      before += n;
+    int64_t before = at;
+    for (int64_t i = b_lo;; ++i) {
+      const Request r = attn_request(a, i);
+      const int64_t n = attn_units<kRows>(a, r);
+      if (u_begin < before + n * kv_heads) {
+        found = Found{r, i, before, n};
+        break;
+      }
+      before += n * kv_heads;
     }
-    found[0] = i, found[1] = before;
   }
   __syncthreads();
-  int64_t b = same(found[0]), u_item = same(found[1]);  // the item's first unit
+  int64_t b = same(found.request), u_item = same(found.before);  // the item's first unit
   int row0 = 0;
-  Request req = same(attn_request(a, b));
-  const int64_t per_head = same(attn_units<kRows>(a, req));
+  Request req = same(found.req);
+  const int64_t per_head = same(found.units);
   int head = same(static_cast<int>((u_begin - u_item) / per_head));
   u_item += head * per_head;
   Span span = same(attn_span<kRows>(a, req, 0));

@@ -88,13 +88,52 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
   constexpr int kSub = kUnit / kTile;  // tiles of a unit
   __shared__ ManyStage<DIM> stage[2];
-  __shared__ int64_t found[2];
+  __shared__ Found found;
+  __shared__ uint64_t scan[4];
+  __shared__ int32_t first_item[256];
   __shared__ int again_at[2], wild_any;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
-  attn_clear_rows<T, DIM>(a);
-
-  const int64_t count = same(*item_count), per_head = same(items[count].unit), U = per_head * a.v.kv_heads;
+  // The units of one head, and, later, the item that holds a given one of them: from the list of items, or, without one (not
+  // more than 256 requests, few items), by counting.
+  int64_t per_head, count;
+  if (items) {
+    count = same(*item_count), per_head = same(items[count].unit);
+  } else {
+    Request r{};
+    if (threadIdx.x < a.requests) r = attn_request(a, threadIdx.x);
+    const uint64_t mine = (r.queries * a.group + kRows - 1) / kRows;
+    uint64_t all;
+    const uint64_t at = block_exclusive_scan<uint64_t, 256>(mine, scan, &all);
+    first_item[threadIdx.x] = static_cast<int32_t>(at);
+    count = same(static_cast<int64_t>(all));
+    __syncthreads();
+    per_head = 0;
+  }
+  // Item i of a head, without the list.
+  auto item_of = [&](int64_t i, Request *r, int *row0) {
+    int lo = 0, hi = static_cast<int>(a.requests) - 1;  // the last request whose first item is i or before it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
+    }
+    *r = attn_request(a, lo);
+    *row0 = static_cast<int>(i - first_item[lo]) * kRows;
+    return lo;
+  };
+  if (!items)
+    for (int64_t base = 0; base < count; base += 256) {
+      uint64_t mine = 0, all;
+      if (base + threadIdx.x < count) {
+        Request r;
+        int row0;
+        item_of(base + threadIdx.x, &r, &row0);
+        mine = attn_span<kRows>(a, r, row0).units;
+      }
+      block_exclusive_scan<uint64_t, 256>(mine, scan, &all);
+      per_head += same(static_cast<int64_t>(all));
+    }
+  const int64_t U = per_head * a.v.kv_heads;
   // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same pages.
   const int64_t G = min(int64_t{gridDim.x}, U);
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
@@ -102,20 +141,42 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   if (wg >= G) return;
   const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
   int head = same(static_cast<int>(u_begin / per_head));
-  int64_t item = 0;
-  {
-    const int64_t x = u_begin - head * per_head;  // within one head's units
-    int64_t width = count;                        // the item is among [item, item + width)
+  const int64_t x = u_begin - head * per_head;  // within one head's units
+  int64_t b, u_item;                            // the item's request and first unit
+  int row0;
+  Request req;
+  if (items) {
+    int64_t item = 0, width = count;  // the item is among [item, item + width)
     while (width > 1) {
       const int64_t step = (width + 255) / 256;
       const int64_t i = item + threadIdx.x * step, end = min(i + step, item + width);
-      if (i < item + width && items[i].unit <= x && x < items[end].unit) found[0] = i, found[1] = end - i;
+      if (i < item + width && items[i].unit <= x && x < items[end].unit) found.before = i, found.units = end - i;
       __syncthreads();
-      item = same(found[0]), width = same(found[1]);
+      item = same(found.before), width = same(found.units);
       __syncthreads();
     }
+    const AttnItem it = items[item];
+    b = same(it.request), row0 = same(it.row0), u_item = head * per_head + same(it.unit);
+    req = same(attn_request(a, b));
+  } else {
+    int64_t before = 0;
+    for (int64_t base = 0; base < count; base += 256) {
+      uint64_t mine = 0, all;
+      Request r{};
+      int r0 = 0, lo = 0;
+      if (base + threadIdx.x < count) {
+        lo = item_of(base + threadIdx.x, &r, &r0);
+        mine = attn_span<kRows>(a, r, r0).units;
+      }
+      const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, 256>(mine, scan, &all));
+      if (at <= x && x < at + static_cast<int64_t>(mine)) found = Found{r, lo, at, r0};
+      before += same(static_cast<int64_t>(all));
+      if (x < before) break;
+    }
+    __syncthreads();
+    b = same(found.request), row0 = same(static_cast<int>(found.units)), u_item = head * per_head + same(found.before);
+    req = same(found.req);
   }
-  int64_t u_item = head * per_head + same(items[item].unit);  // the item's first unit
 
   // scores in powers of two; a negative scale goes to the queries' signs
   // (a scale of 0 becomes the smallest number, with which a masked score stays where it is)
@@ -131,10 +192,6 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   const uint32_t value_scale_at = (DIM / 32 + n_lane * (DIM / 16) / 32) * page + 4 * g;
 
   for (int64_t u = u_begin; u < u_end;) {
-    const AttnItem it = items[item];
-    const int64_t b = same(it.request);
-    const int row0 = same(it.row0);
-    const Request req = same(attn_request(a, b));
     const Span span = same(attn_span<kRows>(a, req, row0));
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
@@ -443,8 +500,17 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
       // begun by the last workgroup whose units begin at the item's first unit or before it
       records[wg] = JoinRecord{static_cast<int32_t>(((u_item + 1) * G - 1) / U), head, rows, row0, req.first_row};
     }
+    if (u >= u_end) break;
+    // the next item
     u_item = u;
-    if (++item == count) item = 0, ++head;
+    row0 += kRows;
+    if (row0 >= req.queries * a.group) {
+      row0 = 0;
+      do {
+        if (++b == a.requests) b = 0, ++head;
+        req = same(attn_request(a, b));
+      } while (req.queries == 0);
+    }
   }
 }
 
@@ -452,9 +518,14 @@ int attn_many_groups(int dim) { return 256 * many_waves(dim); }
 
 template <typename T, int DIM>
 static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  hipLaunchKernelGGL(page_attention_items_kernel<kManyRows>, dim3(1), dim3(1024), 0, stream, a, s.first_item, s.items, s.room,
-                     s.count);
-  hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(256), 0, stream, a, s.items, s.count, s.parts,
+  // A list of items costs a launch; every workgroup counts for itself where that takes no longer.
+  const AttnItem *items = nullptr;
+  if (a.requests > 256 || s.room > 1024) {
+    hipLaunchKernelGGL(page_attention_items_kernel<kManyRows>, dim3(1), dim3(1024), 0, stream, a, s.first_item, s.items, s.room,
+                       s.count);
+    items = s.items;
+  }
+  hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(256), 0, stream, a, items, s.count, s.parts,
                      s.stats, s.records);
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, kManyRows>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
