@@ -33,10 +33,9 @@ struct AttnArgs {
 // cache's head, row r of a request being token r / group, head r % group. The tokens that an item's rows see are cut at
 // multiples of kUnit: the tiles that hold first tokens ("sinks"), then those from the window's begin to the last row's own
 // place. Units are numbered (few rows: request by request, head by head, row tile by row tile; many: head by head, request by
-// request, row tile by row tile), and workgroup w of G takes units
-// floor(w U / G) up to floor((w + 1) U / G), so all end at about the same time whatever the lengths are. An item may be
-// shared by several workgroups; each leaves a part (maximum, sum, weighted values), which page_attention_join_kernel puts
-// together.
+// request, row tile by row tile), and workgroups take equal runs of them, so all end at about the same time whatever the
+// lengths are. An item may be shared by several workgroups; each leaves a part (reference, sum, weighted values), which
+// page_attention_join_kernel puts together.
 constexpr int kUnit = 128;  // tokens: four waves of 32
 constexpr int kWaveTokens = 32;
 constexpr float kNothing = -__builtin_inff();
@@ -123,20 +122,32 @@ __device__ __forceinline__ int64_t attn_units(const AttnArgs &a, const Request &
   return n;
 }
 
+// Division of numbers that mostly fit 32 bits.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
+
+// U units for G workgroups: workgroup w takes units floor(w U / G) up to floor((w + 1) U / G), so that longer shares are spread
+// evenly over the workgroups, and with them over the XCDs.
+struct Shares {
+  int64_t U, G, each, more;
+  __device__ __forceinline__ Shares(int64_t units, int64_t groups) : U(units), G(groups), each(divide(units, groups)) {
+    more = U - each * G;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t w) const { return w * each + divide(w * more, G); }
+  __device__ __forceinline__ int64_t owner(int64_t u) const { return divide((u + 1) * G - 1, U); }  // of unit u
+};
+
 // Where a workgroup begins, as the thread that found it tells the others.
 struct Found {
   Request req;
   int64_t request, before, units;  // units in front of the request (many: of the item), of the request for one head
 };
 
-// Rows that belong to no request are 0.
+// Rows in front of row_lo and from row_hi on, which belong to no request, are 0.
 template <typename T, int DIM>
-__device__ __forceinline__ void attn_clear_rows(const AttnArgs &a) {
-  int64_t row_lo = a.tokens, row_hi = a.tokens;
-  if (a.requests > 0) {
-    row_lo = min(max(load_int(a.starts, 0, a.len_bytes), int64_t{0}), a.tokens);
-    row_hi = min(max(load_int(a.starts, a.requests, a.len_bytes), row_lo), a.tokens);
-  }
+__device__ __forceinline__ void attn_clear_rows(const AttnArgs &a, int64_t row_lo, int64_t row_hi) {
   const int64_t none = row_lo + a.tokens - row_hi;
   if (none <= 0) return;
   const int64_t row16 = static_cast<int64_t>(a.heads) * DIM / 8;  // pieces of 16 bytes
@@ -556,7 +567,7 @@ __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at
   }
 }
 
-// Clears what belongs to no request, and puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
+// Puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
 // rows to join (a grid that has a workgroup for each row that there could be takes longer to start than to run). Where they
 // are few, a workgroup takes one at a time, its teams of DIM / 4 threads a part each; else every team takes a row.
 constexpr int kMostGroups = 256 * 4;
@@ -569,7 +580,6 @@ __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, co
   __shared__ uint32_t scan[4];
   __shared__ f32x4 acc_shared[kTeams][kLanes];
   __shared__ float top_shared[kTeams], sum_shared[kTeams];
-  attn_clear_rows<T, DIM>(a);
   uint32_t rows[kEach], mine = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {

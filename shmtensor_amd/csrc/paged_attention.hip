@@ -29,6 +29,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   };
   __shared__ Shared shared;
   __shared__ Found found;
+  __shared__ int64_t row_range[2];  // rows of any request
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
   const int kv_heads = a.v.kv_heads;
@@ -36,18 +37,27 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   // Where this workgroup's units begin: each thread counts a run of requests.
   const int64_t each = (a.requests + 255) / 256, b_lo = min(threadIdx.x * each, a.requests), b_hi = min(b_lo + each, a.requests);
   int64_t mine = 0;
-  for (int64_t i = b_lo; i < b_hi; ++i) mine += attn_units<kRows>(a, attn_request(a, i)) * kv_heads;
+  if (threadIdx.x == 0) row_range[0] = row_range[1] = a.requests > 0 ? 0 : a.tokens;
+  __syncthreads();
+  for (int64_t i = b_lo; i < b_hi; ++i) {
+    const Request r = attn_request(a, i);
+    mine += attn_units<kRows>(a, r) * kv_heads;
+    if (i == 0) row_range[0] = r.first_row;
+    if (i == a.requests - 1) row_range[1] = r.first_row + r.queries;
+  }
   uint64_t total;
   const int64_t at =
       static_cast<int64_t>(block_exclusive_scan<uint64_t, 256>(static_cast<uint64_t>(mine), shared.scan, &total));
   const int64_t U = same(static_cast<int64_t>(total));
+  attn_clear_rows<T, DIM>(a, row_range[0], row_range[1]);
   // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same lines of scales and
   // of the table. With fewer units than workgroups each has one, on all XCDs.
   const int64_t G = min(int64_t{gridDim.x}, U);
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
   if (threadIdx.x == 0) records[wg].first = -1;
   if (wg >= G) return;
-  const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
+  const Shares shares(U, G);
+  const int64_t u_begin = shares.begin(wg), u_end = shares.begin(wg + 1);
   if (at <= u_begin && u_begin < at + mine) {
     int64_t before = at;
     for (int64_t i = b_lo;; ++i) {
@@ -65,7 +75,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
   int row0 = 0;
   Request req = same(found.req);
   const int64_t per_head = same(found.units);
-  int head = same(static_cast<int>((u_begin - u_item) / per_head));
+  int head = same(static_cast<int>(divide(u_begin - u_item, per_head)));
   u_item += head * per_head;
   Span span = same(attn_span<kRows>(a, req, 0));
   while (u_item + span.units <= u_begin) {
@@ -270,8 +280,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       }
     }
     if (!begins && ends && threadIdx.x == 0) {
-      // begun by the last workgroup whose units begin at the item's first unit or before it
-      records[wg] = JoinRecord{static_cast<int32_t>(((u_item + 1) * G - 1) / U), head, rows, row0, req.first_row};
+      records[wg] = JoinRecord{static_cast<int32_t>(shares.owner(u_item)), head, rows, row0, req.first_row};
     }
     if (u >= u_end) break;
     // the next item
@@ -338,7 +347,8 @@ void launch_attention(const AttnArgs &a, int dim, int elem_type, const AttnShape
   s.first_item = reinterpret_cast<int32_t *>(at += shape.item_bytes);
   s.room = shape.items;
   // no more workgroups than there can be units
-  const int64_t units = (a.tokens * a.group / shape.rows + a.requests) * a.v.kv_heads * (a.limit / kUnit + 1);
+  const int64_t units = (a.tokens * a.group / shape.rows + a.requests) * a.v.kv_heads *
+                        (a.limit / kUnit + 1 + item_cost(shape.rows));
   const unsigned groups = static_cast<unsigned>(std::min(shape.groups, std::max<int64_t>(units, 1)));
   if (shape.many) launch_attention_many(a, dim, elem_type, groups, s, stream);
   else if (elem_type == SHMT_F16) launch_few<_Float16>(a, dim, shape.rows, groups, s, stream);

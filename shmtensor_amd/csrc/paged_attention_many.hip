@@ -90,6 +90,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   __shared__ ManyStage<DIM> stage[2];
   __shared__ Found found;
   __shared__ uint64_t scan[4];
+  __shared__ int64_t row_range[2];  // rows of any request
   __shared__ int32_t first_item[256];
   __shared__ int again_at[2], wild_any;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -99,15 +100,24 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   int64_t per_head, count;
   if (items) {
     count = same(*item_count), per_head = same(items[count].unit);
+    const Request r0 = attn_request(a, 0), r1 = attn_request(a, a.requests - 1);
+    attn_clear_rows<T, DIM>(a, r0.first_row, r1.first_row + r1.queries);
   } else {
+    if (threadIdx.x == 0) row_range[0] = row_range[1] = a.tokens;
+    __syncthreads();
     Request r{};
-    if (threadIdx.x < a.requests) r = attn_request(a, threadIdx.x);
+    if (threadIdx.x < a.requests) {
+      r = attn_request(a, threadIdx.x);
+      if (threadIdx.x == 0) row_range[0] = r.first_row;
+      if (threadIdx.x == a.requests - 1) row_range[1] = r.first_row + r.queries;
+    }
     const uint64_t mine = (r.queries * a.group + kRows - 1) / kRows;
     uint64_t all;
     const uint64_t at = block_exclusive_scan<uint64_t, 256>(mine, scan, &all);
     first_item[threadIdx.x] = static_cast<int32_t>(at);
     count = same(static_cast<int64_t>(all));
     __syncthreads();
+    attn_clear_rows<T, DIM>(a, row_range[0], row_range[1]);
     per_head = 0;
   }
   // Item i of a head, without the list.
@@ -139,8 +149,9 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
   if (threadIdx.x == 0) records[wg].first = -1;
   if (wg >= G) return;
-  const int64_t u_begin = same(wg * U / G), u_end = same((wg + 1) * U / G);
-  int head = same(static_cast<int>(u_begin / per_head));
+  const Shares shares(U, G);
+  const int64_t u_begin = shares.begin(wg), u_end = shares.begin(wg + 1);
+  int head = same(static_cast<int>(divide(u_begin, per_head)));
   const int64_t x = u_begin - head * per_head;  // within one head's units
   int64_t b, u_item;                            // the item's request and first unit
   int row0;
@@ -497,8 +508,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     }
     __syncthreads();  // wild_any has been read
     if (!begins && ends && threadIdx.x == 0) {
-      // begun by the last workgroup whose units begin at the item's first unit or before it
-      records[wg] = JoinRecord{static_cast<int32_t>(((u_item + 1) * G - 1) / U), head, rows, row0, req.first_row};
+      records[wg] = JoinRecord{static_cast<int32_t>(shares.owner(u_item)), head, rows, row0, req.first_row};
     }
     if (u >= u_end) break;
     // the next item
