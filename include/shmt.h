@@ -710,8 +710,8 @@ int shmt_page_set(const shmt_paged_cache *cache, const void *slots,
                   const void *values, int64_t value_token_stride,
                   int64_t value_head_stride, int elem_type, void *stream);
 /* The reverse: the values that the rows at `slots` stand for, rounded to
- * elem_type, into contiguous keys and values [n, kv_heads, dim]. Rows of slots
- * outside the cache are 0.                                                  */
+ * elem_type, into contiguous keys and values [n, kv_heads, dim]; what is
+ * beyond the type's range is infinite. Rows of slots outside the cache are 0. */
 int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
                     int slot_bytes, int64_t n, void *keys, void *values,
                     int elem_type, void *stream);

@@ -303,7 +303,12 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, in
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
   const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
-  s.many = rows > 32;
+  // Which kernel. 32 rows at a time, read anew for each 32, against 128 rows that share what is decoded: measured at 8 heads of
+  // 128, bfloat16, 16 requests of 8,000 tokens, 64 / 96 / 128 rows a request take 68 / 100 / 114 us and 106 / 108 / 113 us (256
+  // dimensions: 178 / 280 us and 259 / 259 us); one request of 8,000 tokens, 256 rows: 34 and 44 us, 512 rows: 53 and 51 us.
+  // Few items of 128 rows leave most of the card idle.
+  const int64_t items_of_128 = tokens * group * kv_heads / kManyRows;
+  s.many = rows > 256 || (rows > (dim == 256 ? 64 : 96) && items_of_128 >= 128);
   s.rows = s.many ? kManyRows : rows <= 16 ? 16 : 32;
   s.groups = s.many ? attn_many_groups(dim) : 256 * attn_waves(dim, s.rows / 16);
   s.items = s.many ? tokens * group / s.rows + requests : 0;

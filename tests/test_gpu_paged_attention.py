@@ -333,3 +333,31 @@ def test_refusals(capi):
     no(">= 0", sinks=-2)
     no(">= 0", max_query_len=-1)
     no("finite", softmax_scale=float("inf"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows(capi, dtype, dim):
+    """Requests of hundreds of rows: not a number in some rows' sight, one token that takes all weight, parts to join."""
+    b = Batch(dim + 1, [700, 300, 5], [290, 300, 5], 6, 2, dim, 16, dtype)
+    at = lambda r, j: int(b.table[r, j // 16])
+    b.scales[at(0, 520), 0, 1, 1, 520 % 16] = 255                      # a value's block that the later rows see
+    b.scales[at(0, 690), 1, 0, 0, 690 % 16] = 255                      # a key that the last rows see
+    b.scales[at(1, 3), 1, 1, 0, 3] = 250 if dtype == torch.bfloat16 else 140   # values near the end of the type's range
+    b.query[7] *= 2.0 ** 9
+    b.query[400, 1] *= -2.0 ** 9
+    want = b.want()
+    assert np.isnan(want[0]).any() and not np.isnan(want[0]).all()
+    _check(capi, b)
+    _check(capi, b, window=130, sinks=20)
+    _check(capi, Batch(3, [2300, 40], [280, 1], 2, 1, dim, 32, dtype))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_more_requests_than_threads(capi, dim):
+    rng = np.random.default_rng(dim)
+    lens = rng.integers(0, 24, 600)
+    q = np.minimum(rng.integers(0, 5, 600), lens)
+    b = Batch(dim, lens, q, 2, 1, dim, 16, torch.bfloat16)
+    for hint in (4, 1000):                                             # the kernels for few rows and for many
+        _check(capi, b, max_query_len=hint)
