@@ -3,6 +3,8 @@
 // reference; what they compute is in include/shmt.h). Host C++ only: tensors
 // are checked here, outputs and scratch come from torch's caching allocator,
 // the work goes to torch's current stream and nothing waits for it.
+#include <ATen/hip/EmptyTensor.h>
+
 #include <cmath>
 
 #include "shim.h"
@@ -10,6 +12,11 @@
 namespace shim {
 
 namespace {
+
+// A new contiguous tensor on the device of `like`, without the dispatcher's round (a small call makes five of them).
+torch::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor &like) {
+  return torch::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
 
 int elem_type(at::ScalarType t, const char *name) {
   if (t == torch::kFloat32) return SHMT_F32;
@@ -105,11 +112,10 @@ std::vector<torch::Tensor> page_plan(torch::Tensor cached_lens, torch::Tensor ne
   TORCH_CHECK(max_tokens >= 0 && max_tokens < (int64_t{1} << 31), "max_tokens must be in [0, 2^31)");
   TORCH_CHECK(page > 0 && page <= 256, "a page must hold 16, 32, 64, 128 or 256 tokens, not ", page);
   free_pages = free_pages.contiguous();
-  const auto i32 = block_table.options();
-  const auto i64 = i32.dtype(torch::kInt64);
-  torch::Tensor starts = torch::empty({n + 1}, i32), kv_lens = torch::empty({n}, i32);
-  torch::Tensor positions = torch::empty({max_tokens}, i32), slots = torch::empty({max_tokens}, i64);
-  torch::Tensor counts = torch::empty({2}, i64);
+  auto empty = [&](int64_t size, at::ScalarType type) { return new_tensor({size}, type, block_table); };
+  torch::Tensor starts = empty(n + 1, torch::kInt32), kv_lens = empty(n, torch::kInt32);
+  torch::Tensor positions = empty(max_tokens, torch::kInt32), slots = empty(max_tokens, torch::kInt64);
+  torch::Tensor counts = empty(2, torch::kInt64);
   const int64_t scratch_bytes = shmt_page_plan_scratch_bytes(n);
   torch::Tensor scratch = scratch_bytes > 0 ? device_bytes(scratch_bytes) : torch::Tensor();
   check(shmt_page_plan(cached_lens.data_ptr(), new_lens.data_ptr(), static_cast<int>(cached_lens.element_size()), n,
@@ -130,7 +136,8 @@ void page_set(const torch::Tensor &cache, const torch::Tensor &scales, torch::Te
   check_device(keys, cache, "keys");
   check_device(values, cache, "values");
   const int64_t n = slots.numel();
-  const std::vector<int64_t> shape{n, c.kv_heads, c.dim};
+  const int64_t sizes[3] = {n, c.kv_heads, c.dim};
+  const at::IntArrayRef shape(sizes);
   TORCH_CHECK(keys.sizes() == shape && values.sizes() == shape, "keys and values must be [slots, kv_heads, dim] = ",
               shape, ", got ", keys.sizes(), " and ", values.sizes());
   TORCH_CHECK(keys.scalar_type() == values.scalar_type(), "keys and values must have one type");
@@ -150,9 +157,8 @@ std::vector<torch::Tensor> page_fetch(const torch::Tensor &cache, const torch::T
   slots = cuda_ids(slots, "slots");
   check_device(slots, cache, "slots");
   const int type = elem_type(dtype, "dtype");
-  const auto options = cache.options().dtype(dtype);
-  torch::Tensor keys = torch::empty({slots.numel(), c.kv_heads, c.dim}, options);
-  torch::Tensor values = torch::empty_like(keys);
+  torch::Tensor keys = new_tensor({slots.numel(), c.kv_heads, c.dim}, dtype, cache);
+  torch::Tensor values = new_tensor({slots.numel(), c.kv_heads, c.dim}, dtype, cache);
   check(shmt_page_fetch(&c, slots.data_ptr(), static_cast<int>(slots.element_size()), slots.numel(), keys.data_ptr(),
                         values.data_ptr(), type, current_stream()));
   return {keys, values};
@@ -182,16 +188,16 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
   TORCH_CHECK(query_starts.dim() == 1 && query_starts.numel() == n + 1 && kv_lens.dim() == 1 && kv_lens.numel() == n,
               "block_table has ", n, " requests: query_starts must hold one entry more, kv_lens as many");
   TORCH_CHECK(window >= 0 && sinks >= 0 && max_query_len >= 0, "window, sinks and max_query_len must be >= 0");
-  torch::Tensor out = torch::empty({tokens, heads, c.dim}, query.options().memory_format(at::MemoryFormat::Contiguous));
+  torch::Tensor out = new_tensor({tokens, heads, c.dim}, query.scalar_type(), query);
   torch::Tensor lse;
-  if (return_lse) lse = torch::empty({tokens, heads}, query.options().dtype(torch::kFloat32));
+  if (return_lse) lse = new_tensor({tokens, heads}, torch::kFloat32, query);
   if (tokens > 0) {
     query = rows_on_16(query);
     const int64_t scratch_bytes = shmt_page_attention_scratch_bytes(tokens, static_cast<int>(heads), c.kv_heads, c.dim,
                                                                     elem_type(query.scalar_type(), "query"), n,
                                                                     max_query_len);
     TORCH_CHECK(scratch_bytes >= 0, shmt_last_error());
-    torch::Tensor scratch = device_bytes(scratch_bytes);
+    torch::Tensor scratch = new_tensor({scratch_bytes}, torch::kUInt8, cache);
     const float scale = softmax_scale ? static_cast<float>(*softmax_scale)
                                       : 1.0f / std::sqrt(static_cast<float>(c.dim));
     check(shmt_page_attention(&c, query.data_ptr(), stride_of(query, 0), stride_of(query, 1),

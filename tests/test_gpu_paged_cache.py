@@ -214,3 +214,23 @@ def test_refusals(capi):
     no("a page must hold", capi.page_plan, i, i, t, i, 20, 4)
     no("contiguous", capi.page_plan, i, i, torch.zeros((2, 3), dtype=torch.int32, device=DEV).t(), i, 16, 4)
     no("overlap", capi.page_plan, i, i, t[:1].expand(3, 2), i, 16, 4)
+
+
+@pytest.mark.parametrize("room", [1.0, 0.9, 1.2])
+def test_plan_of_long_prompts(capi, room):
+    """Hundreds of thousands of tokens: four in a row to a thread, across the ends of requests and pages."""
+    rng = np.random.default_rng(5)
+    cached, new = rng.integers(0, 100, 50), rng.integers(0, 9000, 50)
+    new[3], new[4], new[5], new[20] = 1, 0, 2, 0
+    end = -(-(cached + new) // 16)
+    table = np.full((50, int(end.max()) - 3), -1, np.int32)                # the longest requests outgrow it
+    table[:, :7] = rng.permutation(1 << 20)[:350].reshape(50, 7)
+    free = rng.permutation(1 << 20)[:int((end - -(-cached // 16)).sum()) - 9].astype(np.int32)
+    tokens = int(new.sum() * room) | 1
+    dev_table = torch.from_numpy(table.copy()).to(DEV)
+    want = paged.plan(cached, new, table, free, 16, tokens)
+    got = capi.page_plan(torch.from_numpy(cached).to(DEV), torch.from_numpy(new).to(DEV), dev_table,
+                         torch.from_numpy(free).to(DEV), 16, tokens)
+    for g, w in zip(got, want):
+        assert np.array_equal(g.cpu().numpy(), w)
+    assert np.array_equal(dev_table.cpu().numpy(), table)
