@@ -733,9 +733,12 @@ int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
  * tokens can be joined. out: contiguous, of query's type. query_starts must
  * not descend; starts and kv_lens are len_bytes in {4,8} wide. max_query_len:
  * the most queries of a request, if known (0: not known): it only chooses the
- * kernel. scratch: shmt_page_attention_scratch_bytes(...) bytes of device
- * memory, 16-byte aligned, free again when the work queued has run. Sums and
- * the softmax are held in 32 bits.                                          */
+ * kernel. A row of the table has room for 2^30 tokens at most, and tokens *
+ * heads are below 2^30. scratch: shmt_page_attention_scratch_bytes(...) bytes
+ * of device memory, 16-byte aligned, free again when the work queued has run.
+ * Sums and the softmax are held in 32 bits; the weights meet the values as
+ * bfloat16 (float16 queries: as the sum of two). The same call gives the same
+ * bits. Values of 2^80 and more may overflow where they would not have to.   */
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads,
                                           int kv_heads, int dim, int elem_type,
                                           int64_t requests,

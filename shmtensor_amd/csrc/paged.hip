@@ -104,7 +104,8 @@ __device__ __forceinline__ void plan_entries(const PlanArgs &a, int64_t b, const
 }
 
 // Up to kPlanOne requests, in one launch: every workgroup adds up all lengths for itself (they are few, and it costs less than
-// a second launch), keeps the sums in LDS and takes its share of the tokens and of the requests' table rows. No workgroup
+// a second launch: 7 / 1,024 / 301 requests 3.6 / 6.5 / 7.6 us on the GPU, with sums, table and tokens in three launches 6 / 10
+// / 13 us), keeps the sums in LDS and takes its share of the tokens and of the requests' table rows. No workgroup
 // reads a table entry that another writes: tokens on new pages take them from the list of free pages.
 constexpr int kPlanOne = 2048;
 
@@ -252,7 +253,10 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
 // A workgroup takes PASSES * 2048 / DIM tokens in a row of one head's keys or values: DIM / 8 lanes a token, eight values a
 // lane, four lanes a block of 32 that shares a scale. Tokens in a row mostly lie in a row in their page too, so the codes
 // leave (or come) as one piece, and the scale bytes, which lie token by token, meet in one L2. All of a lane's rows are in
-// flight together. Bound by HBM.
+// flight together. Bound by HBM: 65,536 tokens of 8 heads x 128 in bfloat16 (268 MB in, 71 MB out, or the reverse) take 70 us
+// to set and 55 us to fetch, 4.8 and 6.2 TB/s; a copy of 2 GiB moves 4.9. Rows are read and written past the caches, which a
+// row is not read from again: without that, 81 and 90 us. With a lane for 8 values of any token in turn, and 64-bit divisions
+// for its place, 90 and 94 us.
 template <int DIM, int PASSES>
 struct RowPlace {
   static constexpr int kLanes = DIM / 8;

@@ -1,5 +1,14 @@
 // Attention over the paged key/value cache held in 4 bits (shmt_page_attention): the kernel for few rows a request (decode,
 // a few speculated tokens), in which the waves of a workgroup share the tokens, and the entry point.
+//
+// The work: every token that a request holds is read once for each of its heads, dim bytes and dim / 16 scale bytes, and a
+// decode step is bound by that. A wave takes 32 tokens a step, 2,176 or 4,352 bytes at 64 or 128 dimensions, while the next 32
+// are on their way; three waves a SIMD keep 52 KB of a compute unit's share of HBM in flight. Units of 128 tokens are dealt out
+// evenly (paged_attention.h), so a batch of ragged requests, one long request and anything between are one case. Measured, 32
+// requests of 8,000 tokens, 8 heads of 128, bfloat16: 56 us, 5.0 TB/s, what a copy reaches; 64 ragged requests of 1,000 to
+// 16,000 tokens 84 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 47 us, 3.0 TB/s, of which the join 7 us.
+// At 64 dimensions half the bytes come with the same softmax, and the vector units are what it waits for: 96 requests with a
+// window of 4,000 tokens, float16, 67 us, 3.1 TB/s (214 vector instructions for 32 tokens of a wave).
 #include "paged_attention.h"
 #include "paged_host.h"
 
@@ -391,7 +400,8 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_
                "%d query heads do not share %d heads of the cache evenly", heads, cache->kv_heads);
   SHMT_REQUIRE(tokens * heads < (int64_t{1} << 30), "query rows x heads must be below 2^30");
   SHMT_REQUIRE(requests >= 0 && requests < (int64_t{1} << 31), "the number of requests must be in [0, 2^31)");
-  SHMT_REQUIRE(width >= 0 && width < (int64_t{1} << 31) / cache->page, "the block table holds too many tokens");
+  SHMT_REQUIRE(width >= 0 && width <= (int64_t{1} << 30) / cache->page,
+               "the block table holds too many tokens: more than 2^30 a request");
   SHMT_REQUIRE(width_ok(len_bytes), "query_starts and kv_lens can only be int32 or int64");
   SHMT_REQUIRE(window >= 0 && sinks >= 0 && max_query_len >= 0, "window, sinks and max_query_len must be >= 0");
   SHMT_REQUIRE(softmax_scale == softmax_scale && softmax_scale - softmax_scale == 0, "softmax_scale must be finite");
