@@ -151,12 +151,12 @@ __device__ __forceinline__ void attn_clear_rows(const AttnArgs &a, int64_t row_l
   const int64_t none = row_lo + a.tokens - row_hi;
   if (none <= 0) return;
   const int64_t row16 = static_cast<int64_t>(a.heads) * DIM / 8;  // pieces of 16 bytes
-  for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * row16; i += int64_t{gridDim.x} * 256) {
+  for (int64_t i = int64_t{blockIdx.x} * blockDim.x + threadIdx.x; i < none * row16; i += int64_t{gridDim.x} * blockDim.x) {
     const int64_t row = i / row16;
     reinterpret_cast<uint4 *>(a.out)[(row < row_lo ? row : row - row_lo + row_hi) * row16 + i % row16] = uint4{0, 0, 0, 0};
   }
   if (!a.lse) return;
-  for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none * a.heads; i += int64_t{gridDim.x} * 256) {
+  for (int64_t i = int64_t{blockIdx.x} * blockDim.x + threadIdx.x; i < none * a.heads; i += int64_t{gridDim.x} * blockDim.x) {
     const int64_t row = i / a.heads;
     a.lse[(row < row_lo ? row : row - row_lo + row_hi) * a.heads + i % a.heads] = kNothing;
   }

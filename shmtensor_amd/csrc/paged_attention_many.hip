@@ -48,7 +48,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
   }
 }
 
-// A workgroup's item is 128 rows, 32 (two 16s) to a wave. The four waves decode a tile of tokens together, a quarter each,
+// A workgroup's item is 128 rows, 32 (two 16s) to each of four waves. They decode a tile of tokens together, a quarter each,
 // into LDS as bfloat16 fragments of the two products (a kilobyte each, lane by lane, so that reading and writing them is
 // free of bank conflicts), and each multiplies its own rows with all of it. While a tile is multiplied the next one is
 // decoded into the other half of the LDS and the one behind it is on its way from memory; a tile costs one barrier.
@@ -61,15 +61,18 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // no maximum from tile to tile, 1.23. Products and softmaxes ordered by hand to run beside each other lost (1.71 against
 // 1.56), priorities for the products brought nothing; products on the 4-bit keys themselves would need the queries in 8 bits,
 // and lose bits of sums whose terms differ by much (2^-14 of the terms' sizes, measured).
+// At 256 dimensions 32 rows leave room for one wave on a SIMD only; eight waves of 16 rows read the LDS twice as often but
+// wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (680 TFLOP/s) against 1.02 with four waves and tiles of
+// 32 tokens and 0.95 with eight and 32; chunks of 17 to 2,000 tokens behind a window 87 us against 95 and 92.
 template <int DIM>
 struct ManyShape {
-  static constexpr int kTile = DIM == 256 ? 32 : 64;  // tokens
+  static constexpr int kTile = 64;  // tokens
   static constexpr int kHalves = kTile / 16, kGroups = kTile / 32;
   static constexpr int kKeyFrags = DIM / 32, kValueFrags = DIM / 16;  // of 16 tokens; of 32 tokens
-  static constexpr int kKeyWords = kKeyFrags < 4 ? kKeyFrags : 4;      // of 8 codes: a wave's share of the keys
+  static constexpr int kWaves = DIM == 256 ? 8 : 4, kThreads = kWave * kWaves;
+  static constexpr int NT = kManyRows / 16 / kWaves;                     // 16 rows each of a wave
+  static constexpr int kKeyWords = kHalves * kKeyFrags / kWaves;         // of 8 codes: a wave's share of the keys
 };
-
-constexpr int many_waves(int dim) { return dim == 256 ? 1 : 2; }
 
 // A wave's share of a tile, as it comes from memory: keys of 16 tokens (at 256 dimensions half of each lane's quarter), values
 // of 32 tokens.
@@ -88,18 +91,18 @@ struct ManyStage {
 };
 
 template <typename T, int DIM>
-__global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kernel(AttnArgs a, const AttnItem *items,
-                                                                                  const int32_t *item_count, float *parts,
-                                                                                  float *part_stats, JoinRecord *records) {
+__global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_many_kernel(
+    AttnArgs a, const AttnItem *items, const int32_t *item_count, float *parts, float *part_stats, JoinRecord *records) {
   using Shape = ManyShape<DIM>;
-  constexpr int kRows = kManyRows, NT = 2, kSteps = DIM / 32, kTile = Shape::kTile, kHalves = Shape::kHalves;
+  constexpr int kThreads = Shape::kThreads;
+  constexpr int kRows = kManyRows, NT = Shape::NT, kSteps = DIM / 32, kTile = Shape::kTile, kHalves = Shape::kHalves;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
   constexpr int kSub = kUnit / kTile;  // tiles of a unit
   __shared__ ManyStage<DIM> stage[2];
   __shared__ Found found;
-  __shared__ uint64_t scan[4];
+  __shared__ uint64_t scan[Shape::kWaves];
   __shared__ int64_t row_range[2];  // rows of any request
-  __shared__ int32_t first_item[256];
+  __shared__ int32_t first_item[kThreads];
   __shared__ int again_at[2], wild_any;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
@@ -121,7 +124,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     }
     const uint64_t mine = (r.queries * a.group + kRows - 1) / kRows;
     uint64_t all;
-    const uint64_t at = block_exclusive_scan<uint64_t, 256>(mine, scan, &all);
+    const uint64_t at = block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all);
     first_item[threadIdx.x] = static_cast<int32_t>(at);
     count = same(static_cast<int64_t>(all));
     __syncthreads();
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     return lo;
   };
   if (!items)
-    for (int64_t base = 0; base < count; base += 256) {
+    for (int64_t base = 0; base < count; base += kThreads) {
       uint64_t mine = 0, all;
       if (base + threadIdx.x < count) {
         Request r;
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
         item_of(base + threadIdx.x, &r, &row0);
         mine = attn_span<kRows>(a, r, row0).units;
       }
-      block_exclusive_scan<uint64_t, 256>(mine, scan, &all);
+      block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all);
       per_head += same(static_cast<int64_t>(all));
     }
   const int64_t U = per_head * a.v.kv_heads;
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   if (items) {
     int64_t item = 0, width = count;  // the item is among [item, item + width)
     while (width > 1) {
-      const int64_t step = (width + 255) / 256;
+      const int64_t step = (width + kThreads - 1) / kThreads;
       const int64_t i = item + threadIdx.x * step, end = min(i + step, item + width);
       if (i < item + width && items[i].unit <= x && x < items[end].unit) found.before = i, found.units = end - i;
       __syncthreads();
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     req = same(attn_request(a, b));
   } else {
     int64_t before = 0;
-    for (int64_t base = 0; base < count; base += 256) {
+    for (int64_t base = 0; base < count; base += kThreads) {
       uint64_t mine = 0, all;
       Request r{};
       int r0 = 0, lo = 0;
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
         lo = item_of(base + threadIdx.x, &r, &r0);
         mine = attn_span<kRows>(a, r, r0).units;
       }
-      const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, 256>(mine, scan, &all));
+      const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all));
       if (at <= x && x < at + static_cast<int64_t>(mine)) found = Found{r, lo, at, r0};
       before += same(static_cast<int64_t>(all));
       if (x < before) break;
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   const int page = 1 << a.v.log2_page;
   // a wave's share of the decoding
   const int key_half = DIM == 256 ? wave >> 1 : wave, key_word0 = DIM == 256 ? 4 * (wave & 1) : 0;
-  const int value_group = kTile == 64 ? wave >> 1 : 0, value_word = DIM == 256 ? wave >> 1 : 0;
+  const int value_group = DIM == 256 ? wave >> 2 : wave >> 1, value_word = DIM == 256 ? wave >> 1 & 1 : 0;
   const uint32_t key_at = n_lane * (DIM / 2) + g * (DIM / 8) + key_word0 * 4;
   const uint32_t key_scale_at = (DIM == 64 ? g >> 1 : g * (DIM / 128) + key_word0 / 4) * page + n_lane;
   const uint32_t value_at = (page + 4 * g) * (DIM / 2) + n_lane * (DIM / 32) + value_word * 4;
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     int see_last[NT], see_after[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = wave * 32 + 16 * n + n_lane;
+      const int r = 16 * (wave * NT + n) + n_lane;
       const int row = row0 + min(r, rows - 1), token = row_token(a, row);
       const int h = head * a.group + row - token * a.group;
       const Sees sees = row_sees(a, r < rows ? req.before + token : -1);
@@ -229,7 +232,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     }
     const int sinks = a.window > 0 ? a.sinks : 0;
     // the first and the last place of the wave's rows, and of the item's
-    const int r_first = min(wave * 32, rows - 1), r_last = min(wave * 32 + 31, rows - 1);
+    const int r_first = min(16 * wave * NT, rows - 1), r_last = min(16 * (wave + 1) * NT - 1, rows - 1);
     auto place = [&](int r) { return req.before + row_token(a, row0 + r); };
     auto after = [&](int r) { return a.window > 0 ? max(place(r), -1) - a.window : -1; };
     const int wave_first = same(min(place(r_first), a.limit - 1)), wave_after = same(after(r_last));
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
       const int at = (t - page_base) * kHalves;
       {
         const Place16 x = places.of_lane(at + key_half);
-        if constexpr (DIM == 64) {
+        if constexpr (Shape::kKeyWords == 2) {
           const uint2 y = *reinterpret_cast<const uint2 *>(x.row() + key_at);
           raw.key[0] = y.x, raw.key[1] = y.y;
         } else {
@@ -359,7 +362,8 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
 
     RowState<DIM, NT> st;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) st.top[n] = wave * 32 + 16 * n + n_lane < rows ? kNothing : 0;  // no row waits for nothing
+    for (int n = 0; n < NT; ++n)  // no row waits for nothing
+      st.top[n] = 16 * (wave * NT + n) + n_lane < rows ? kNothing : 0;
     bool waiting = true;
     // A wave's rows and the tile in `from`. Returns whether the item has to be begun again (see raise_reference).
     auto multiply = [&](const Step &s, const ManyStage<DIM> &from) {
@@ -465,7 +469,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
     const bool add_wild = same(wild_any) != 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = wave * 32 + 16 * n + n_lane;
+      const int r = 16 * (wave * NT + n) + n_lane;
       const float total = across_sum(st.sum[n]);
       if (r >= rows) continue;
       const int row = row0 + r, token = row_token(a, row), h = head * a.group + row - token * a.group;
@@ -532,7 +536,7 @@ __global__ __launch_bounds__(256, many_waves(DIM)) void page_attention_many_kern
   }
 }
 
-int attn_many_groups(int dim) { return 256 * many_waves(dim); }
+int attn_many_groups(int dim) { return dim == 256 ? 256 : 512; }
 
 template <typename T, int DIM>
 static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
@@ -543,8 +547,8 @@ static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s
                        s.count);
     items = s.items;
   }
-  hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(256), 0, stream, a, items, s.count, s.parts,
-                     s.stats, s.records);
+  hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(ManyShape<DIM>::kThreads), 0, stream, a, items,
+                     s.count, s.parts, s.stats, s.records);
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, kManyRows>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }
