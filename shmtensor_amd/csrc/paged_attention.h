@@ -682,10 +682,10 @@ struct AttnShape {
   int64_t bytes() const { return parts_bytes + stats_bytes + record_bytes + item_bytes + first_bytes; }
 };
 
-constexpr int kManyRows = 128;
+constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
 // paged_attention_many.hip
 void launch_attention_many(const AttnArgs &a, int dim, int elem_type, unsigned groups, const AttnScratch &s, hipStream_t stream);
-int attn_many_groups(int dim);
+int attn_many_groups();
 
 }  // namespace shmt

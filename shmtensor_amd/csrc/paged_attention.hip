@@ -312,14 +312,17 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, in
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
   const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
-  // Which kernel. 32 rows at a time, read anew for each 32, against 128 rows that share what is decoded: measured at 8 heads of
-  // 128, bfloat16, 16 requests of 8,000 tokens, 64 / 96 / 128 rows a request take 68 / 100 / 114 us and 106 / 108 / 113 us (256
-  // dimensions: 178 / 280 us and 259 / 259 us); one request of 8,000 tokens, 256 rows: 34 and 44 us, 512 rows: 53 and 51 us.
-  // Few items of 128 rows leave most of the card idle.
-  const int64_t items_of_128 = tokens * group * kv_heads / kManyRows;
-  s.many = rows > 256 || (rows > (dim == 256 ? 64 : 96) && items_of_128 >= 128);
-  s.rows = s.many ? kManyRows : rows <= 16 ? 16 : 32;
-  s.groups = s.many ? attn_many_groups(dim) : 256 * attn_waves(dim, s.rows / 16);
+  // Which kernel. 32 rows at a time, read anew for each 32, against 256 (128) rows that share what is decoded, of which a last
+  // item that is not full costs as much as a full one: 16 requests of 8,000 tokens, 8 heads, 128 / 192 / 256 / 320 rows a
+  // request, bfloat16: 108 / 165 / 203 / 269 us and 151 / 155 / 160 / 263 us (float16: 141 / 221 / 269 / 362 and 241 / 244 / 247
+  // / 423; 64 dimensions: 85 / 108 / 150 / 188 and 110 / 112 / 116 / 199; 256 dimensions, 64 / 96 rows: 174 / 281 and 197 / 202).
+  // So an item costs as much as 6 (2) of 32 rows. Where there are few items most of the card idles behind the first of them:
+  // one request of 8,000 tokens, 384 / 512 / 768 rows: 45 / 52 / 67 us and 48 / 50 / 56 us.
+  const int64_t few_items = (rows + 31) / 32, many_items = (rows + many_rows(dim) - 1) / many_rows(dim);
+  s.many = rows > 2 * many_rows(dim) ||
+           (few_items > (dim == 256 ? 2 : 6) * many_items && tokens * group * kv_heads >= 16384);
+  s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;
+  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(dim, s.rows / 16);
   s.items = s.many ? tokens * group / s.rows + requests : 0;
   const int64_t lines = 2 * s.groups * s.rows;
   s.parts_bytes = lines * dim * 4;

@@ -48,29 +48,31 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
   }
 }
 
-// A workgroup's item is 128 rows, 32 (two 16s) to each of four waves. They decode a tile of tokens together, a quarter each,
-// into LDS as bfloat16 fragments of the two products (a kilobyte each, lane by lane, so that reading and writing them is
+// A workgroup's item is 256 rows, 32 (two 16s) to each of eight waves. They decode a tile of 128 tokens together, an eighth
+// each, into LDS as bfloat16 fragments of the two products (a kilobyte each, lane by lane, so that reading and writing them is
 // free of bank conflicts), and each multiplies its own rows with all of it. While a tile is multiplied the next one is
 // decoded into the other half of the LDS and the one behind it is on its way from memory; a tile costs one barrier.
 // The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them.
 // Bound by what the vector units and the matrix cores have to issue: for 64 tokens a wave has 64 products, of which each keeps
-// the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 250 vector
-// instructions, half of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.22 ms, 870
-// TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave its own
-// tokens 2.24 ms; 128 rows, decoded once, 1.63; reading ahead in LDS, 1.56; addresses held by lanes and items weighted, 1.37;
-// no maximum from tile to tile, 1.23. Products and softmaxes ordered by hand to run beside each other lost (1.71 against
-// 1.56), priorities for the products brought nothing; products on the 4-bit keys themselves would need the queries in 8 bits,
-// and lose bits of sums whose terms differ by much (2^-14 of the terms' sizes, measured).
-// At 256 dimensions 32 rows leave room for one wave on a SIMD only; eight waves of 16 rows read the LDS twice as often but
-// wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (680 TFLOP/s) against 1.02 with four waves and tiles of
-// 32 tokens and 0.95 with eight and 32; chunks of 17 to 2,000 tokens behind a window 87 us against 95 and 92.
+// the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 200 vector
+// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.08
+// ms, 985 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
+// its own tokens 2.24 ms; 128 rows and four waves, tiles of 64 decoded once, 1.63; reading ahead in LDS, 1.56; addresses held
+// by lanes and items weighted, 1.37; no maximum from tile to tile, 1.23; 256 rows and tiles of 128, 1.08 (64 dimensions 0.94
+// to 0.82). Products and softmaxes ordered by hand to run beside each other lost (1.71 against 1.56), priorities for the
+// products brought nothing; products on the 4-bit keys themselves would need the queries in 8 bits, and lose bits of sums whose
+// terms differ by much (2^-14 of the terms' sizes, measured).
+// At 256 dimensions 32 rows leave room for one wave on a SIMD only: eight waves of 16 rows and tiles of 64 tokens, as the LDS
+// has room for. They read it twice as often but wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (680
+// TFLOP/s) against 1.02 with four waves of 32 rows and tiles of 32 tokens and 0.95 with eight and 32; chunks of 17 to 2,000
+// tokens behind a window 87 us against 95 and 92.
 template <int DIM>
 struct ManyShape {
-  static constexpr int kTile = 64;  // tokens
+  static constexpr int kTile = DIM == 256 ? 64 : 128;  // tokens
   static constexpr int kHalves = kTile / 16, kGroups = kTile / 32;
   static constexpr int kKeyFrags = DIM / 32, kValueFrags = DIM / 16;  // of 16 tokens; of 32 tokens
-  static constexpr int kWaves = DIM == 256 ? 8 : 4, kThreads = kWave * kWaves;
-  static constexpr int NT = kManyRows / 16 / kWaves;                     // 16 rows each of a wave
+  static constexpr int kRows = many_rows(DIM), kWaves = 8, kThreads = kWave * kWaves;
+  static constexpr int NT = kRows / 16 / kWaves;                         // 16 rows each of a wave
   static constexpr int kKeyWords = kHalves * kKeyFrags / kWaves;         // of 8 codes: a wave's share of the keys
 };
 
@@ -95,7 +97,7 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
     AttnArgs a, const AttnItem *items, const int32_t *item_count, float *parts, float *part_stats, JoinRecord *records) {
   using Shape = ManyShape<DIM>;
   constexpr int kThreads = Shape::kThreads;
-  constexpr int kRows = kManyRows, NT = Shape::NT, kSteps = DIM / 32, kTile = Shape::kTile, kHalves = Shape::kHalves;
+  constexpr int kRows = Shape::kRows, NT = Shape::NT, kSteps = DIM / 32, kTile = Shape::kTile, kHalves = Shape::kHalves;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
   constexpr int kSub = kUnit / kTile;  // tiles of a unit
   __shared__ ManyStage<DIM> stage[2];
@@ -536,20 +538,20 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
   }
 }
 
-int attn_many_groups(int dim) { return dim == 256 ? 256 : 512; }
+int attn_many_groups() { return 256; }
 
 template <typename T, int DIM>
 static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
   // A list of items costs a launch; every workgroup counts for itself where that takes no longer.
   const AttnItem *items = nullptr;
   if (a.requests > 256 || s.room > 1024) {
-    hipLaunchKernelGGL(page_attention_items_kernel<kManyRows>, dim3(1), dim3(1024), 0, stream, a, s.first_item, s.items, s.room,
+    hipLaunchKernelGGL(page_attention_items_kernel<many_rows(DIM)>, dim3(1), dim3(1024), 0, stream, a, s.first_item, s.items, s.room,
                        s.count);
     items = s.items;
   }
   hipLaunchKernelGGL((page_attention_many_kernel<T, DIM>), dim3(groups), dim3(ManyShape<DIM>::kThreads), 0, stream, a, items,
                      s.count, s.parts, s.stats, s.records);
-  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, kManyRows>), dim3(2048), dim3(256), 0, stream, a,
+  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, many_rows(DIM)>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }
 

@@ -361,3 +361,21 @@ def test_more_requests_than_threads(capi, dim):
     b = Batch(dim, lens, q, 2, 1, dim, 16, torch.bfloat16)
     for hint in (4, 1000):                                             # the kernels for few rows and for many
         _check(capi, b, max_query_len=hint)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (1, 1), (7, 3), (64, 0), (100, 50), (200, 300)])
+def test_ragged_requests_in_the_kernel_for_many_rows(capi, dtype, dim, window, sinks):
+    """A hint that is too great: single tokens, chunks and prompts as items of many rows; pages missing or given back; values
+    that are not a number where some rows, all or none see them."""
+    b = Batch(dim + window, [1, 400, 77, 260, 500, 34, 150], [1, 1, 77, 50, 3, 0, 129], 9, 3, dim, 32, dtype)
+    _check(capi, b, window=window, sinks=sinks, max_query_len=4000)
+    at = lambda r, j: int(b.table[r, j // 32])
+    b.scales[at(6, 75), 1, 1, 0, 75 % 32] = 255                        # a value that later rows see, and windows pass
+    b.scales[at(3, 2), 0, 1, 1, 2] = 255
+    b.scales[at(2, 40), 2, 0, 1, 40 % 32] = 255                        # a key
+    b.table[1, 2:5] = -1
+    b.table[4, 0], b.table[4, 9] = len(b.cache), 2**31 - 1
+    b.table[5, :] = -1
+    _check(capi, b, window=window, sinks=sinks, max_query_len=4000)
