@@ -104,7 +104,7 @@ __device__ __forceinline__ void plan_entries(const PlanArgs &a, int64_t b, const
 }
 
 // Up to kPlanOne requests, in one launch: every workgroup adds up all lengths for itself (they are few, and it costs less than
-// a second launch: 7 / 1,024 / 301 requests 3.6 / 6.5 / 7.6 us on the GPU, with sums, table and tokens in three launches 6 / 10
+// a second launch: 7 / 1,024 / 301 requests 3.6 / 6.5 / 7.6 us on the GPU, with sums, table and tokens in three launches 6 / 11
 // / 13 us), keeps the sums in LDS and takes its share of the tokens and of the requests' table rows. No workgroup
 // reads a table entry that another writes: tokens on new pages take them from the list of free pages.
 constexpr int kPlanOne = 2048;
@@ -289,7 +289,7 @@ struct RowPlace {
   __device__ __forceinline__ uint32_t *codes(const RowsArgs &a, int p) const {
     const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
     return reinterpret_cast<uint32_t *>(a.v.cache + at * a.v.cache_stride +
-                                        ((int64_t{2} * head + which << a.v.log2_page) + off) * (DIM / 2) + piece * 4);
+                                        (((int64_t{2} * head + which) << a.v.log2_page) + off) * (DIM / 2) + piece * 4);
   }
   __device__ __forceinline__ uint8_t *scale(const RowsArgs &a, int p) const {
     const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
