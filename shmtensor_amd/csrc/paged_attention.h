@@ -39,7 +39,7 @@ struct AttnArgs {
 constexpr int kUnit = 128;  // tokens: four waves of 32
 constexpr int kWaveTokens = 32;
 constexpr float kNothing = -__builtin_inff();
-constexpr float kLowest = -3.0e38f;  // subtracted instead of kNothing, so that nothing stays nothing
+constexpr float kLowest = -3.40282347e38f;  // the lowest float, subtracted instead of kNothing, so that nothing stays nothing
 
 // Beginning and ending an item costs about as much as this many units: so many are added to each, without tokens in them, for
 // the sake of even shares.
@@ -343,14 +343,15 @@ struct Sight {
   int begin, end, sink_end;  // no row of the item sees any outside of [begin, end) and [0, sink_end)
 };
 
-// The weights of eight scores of a row, relative to its reference, as the right operand of V^T P^T.
+// The weights of eight scores of a row, in units of `unit` powers of two, relative to its reference, as the right operand of
+// V^T P^T.
 template <int PARTS, int NT>
-__device__ __forceinline__ void weights(const f32x4 (&s)[2], float scale2, float top, float &sum, u32x4 (&w)[PARTS][NT], int n) {
+__device__ __forceinline__ void weights(const f32x4 (&s)[2], float unit, float top, float &sum, u32x4 (&w)[PARTS][NT], int n) {
   const float base = fmaxf(top, kLowest);
   float e[8], add = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], scale2, -base));
+    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], unit, -base));
     add += e[j];
   }
   sum += add;
@@ -365,44 +366,67 @@ __device__ __forceinline__ void weights(const f32x4 (&s)[2], float scale2, float
 
 // References. Weights are taken relative to the maximum of the first tile in which a row sees anything: with floats' exponents
 // any reference near the true maximum does as well as that, so there is no maximum to follow from tile to tile and nothing to
-// rescale. Only a sum of weights above 2^40, which takes scores that ordinary ones do not come near, makes a wave begin its
-// tokens again, with a greater reference.
+// rescale (kFirst). Two things make that too little. A row's later scores may be so much greater that its weights sum up to more
+// than 2^40. And a weight comes from the product score * scale as it is, the reference is that product rounded: from 2^30 on,
+// half a unit in its last place is more than an exponent of 2 may move by, and weights would be anything. Where either happens
+// (the second from 2^12 on) the tokens are gone through twice more, with scores in powers of two that are rounded: once for each
+// row's maximum (kMaximum), once with that as the reference (kRounded), to which no weight is above 1. So there are three passes
+// at most, whatever the scores are. Waves that share a row may have weighted it either way: below 2^12 that makes a difference
+// of 2^-13 of a weight, and scores that are tied stay tied above.
+enum : int { kFirst, kMaximum, kRounded };
 constexpr float kPassed = 1099511627776.0f;  // 2^40
+constexpr float kFar = 4096.0f;
 
 template <int NT>
-__device__ __forceinline__ float most_of(const f32x4 (&s)[NT][2], int n, float scale2) {
+__device__ __forceinline__ float most_of(const f32x4 (&s)[NT][2], int n) {
   float x = s[n][0][0];
 #pragma unroll
   for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n][j / 4][j % 4]);
-  return across_max(x) * scale2;
+  return across_max(x);
 }
 
-// Rows without a reference take this tile's maximum. Returns whether any is still without.
-template <int NT, typename State>
-__device__ __forceinline__ bool first_reference(const f32x4 (&s)[NT][2], float scale2, State &st) {
-  bool none = false;
+// What softmax_scale makes of scores, in powers of two. A negative scale goes to the queries' signs; a scale of 0 becomes the
+// smallest number, with which a masked score stays where it is.
+__device__ __forceinline__ float powers_of_two(const AttnArgs &a) {
+  return fmaxf(fabsf(a.scale) * 1.44269504088896340736f, __uint_as_float(1u));
+}
+
+// Rows without a reference take this tile's maximum. Returns whether any is still without; `again` is set for one that is far
+// from 0.
+template <int NT, typename State, typename Flag>
+__device__ __forceinline__ bool first_reference(const f32x4 (&s)[NT][2], float scale2, State &st, Flag &again) {
+  bool none = false, far = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float most = most_of<NT>(s, n, scale2);
+    const float most = most_of<NT>(s, n) * scale2;
     st.top[n] = st.top[n] == kNothing ? most : st.top[n];
     none |= st.top[n] == kNothing;
+    far |= st.top[n] != kNothing && fabsf(st.top[n]) >= kFar;
   }
+  if (__ballot(far)) again = 1;
   return __ballot(none) != 0;
 }
 
-// Where a row's sum has passed 2^40: a reference that is greater by 2^20 at least. Returns whether there is such a row.
+// Scores in powers of two, rounded; and, on the way to the maximum, that as far as it is known.
 template <int NT, typename State>
-__device__ __forceinline__ bool raise_reference(const f32x4 (&s)[NT][2], float scale2, State &st) {
+__device__ __forceinline__ void round_scores(f32x4 (&s)[NT][2], float scale2, State &st, int pass) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[n][j / 4][j % 4] = s[n][j / 4][j % 4] * scale2;
+  if (pass != kMaximum) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) st.top[n] = fmaxf(st.top[n], most_of<NT>(s, n));
+}
+
+// Whether a row's sum has passed 2^40.
+template <int NT, typename State>
+__device__ __forceinline__ bool sum_passed(const State &st) {
   bool passed = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) passed |= st.sum[n] > kPassed;
-  if (!__ballot(passed)) return false;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const float most = most_of<NT>(s, n, scale2);
-    if (across_max(st.sum[n]) > kPassed) st.top[n] = fmaxf(st.top[n] + 20.0f, most);
-  }
-  return true;
+  return __ballot(passed) != 0;
 }
 
 // Scale bytes from here on make values that are infinite in bfloat16, or not a number.
@@ -417,11 +441,11 @@ constexpr uint32_t kWild = 253;
 // result's own rounding.
 // `whole`: all rows see all tokens. Otherwise scores are masked; and values that are not finite in bfloat16 must not meet the
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
-// Returns whether the item has to be begun again (see below).
-template <int DIM, int NT, int PARTS>
+// FIRST: `pass` is kFirst; rows may be `waiting` for a reference. Returns whether the wave has to begin its tokens again.
+template <bool FIRST, int DIM, int NT, int PARTS>
 __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
-                                            float scale2, int lane, bool whole, int token0, bool there0, bool there1,
-                                            const Sight<NT> &sight, bool &wild, bool &waiting) {
+                                            float scale2, int pass, int lane, bool whole, int token0, bool there0,
+                                            bool there1, const Sight<NT> &sight, bool &wild, bool &waiting) {
   const int g = lane >> 4;
   f32x4 s[NT][2];
 #pragma unroll
@@ -464,11 +488,13 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
         wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
       }
   }
-  if (waiting) waiting = first_reference<NT>(s, scale2, st);
+  bool again = false;
+  if constexpr (!FIRST) round_scores<NT>(s, scale2, st, pass);
+  else if (waiting) waiting = first_reference<NT>(s, scale2, st, again);
   u32x4 w[PARTS][NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) weights<PARTS>(s[n], scale2, st.top[n], st.sum[n], w, n);
-  const bool again = raise_reference<NT>(s, scale2, st);
+  for (int n = 0; n < NT; ++n) weights<PARTS>(s[n], FIRST ? scale2 : 1.0f, st.top[n], st.sum[n], w, n);
+  if constexpr (FIRST) again |= sum_passed<NT>(st);
   // The conversion reads nothing of a scale but its exponent field, so the byte need not be cut out.
   float f[8];
 #pragma unroll
@@ -544,6 +570,7 @@ __device__ float score_of(const T *q, const uint8_t *codes, const uint8_t *scale
 template <typename T, int DIM>
 __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at, int j0, const T *q_row, const Sees &sees,
                                              float scale2, float base, int d0, f32x4 (&o)[DIM / 64]) {
+#pragma clang fp contract(off)
   if (at < 0) return;
   const int page = 1 << a.v.log2_page, off = j0 & (page - 1);
   const int64_t tile = int64_t{2} * head << a.v.log2_page;
@@ -556,7 +583,7 @@ __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at
     const uint32_t byte = sc[(DIM / 32 + d0 / 32) * page + i];
     if (byte < kWild || j > sees.last || (j <= sees.after && j >= sinks)) continue;
     const float x = score_of<T, DIM>(q_row, codes + i * (DIM / 2), sc + i, page);
-    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(a.scale < 0 ? -x : x, scale2, -base));
+    const float e = __builtin_amdgcn_exp2f((a.scale < 0 ? -x : x) * scale2 - base);  // scores rounded, as in kRounded
     const uint8_t *v = codes + (page + i) * (DIM / 2) + d0 / 2;
 #pragma unroll
     for (int d = 0; d < DIM / 16; d += 2) {

@@ -93,9 +93,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
     span = same(attn_span<kRows>(a, req, row0));
   }
 
-  // scores in powers of two; a negative scale goes to the queries' signs
-  // (a scale of 0 becomes the smallest number, with which a masked score stays where it is)
-  const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, __uint_as_float(1u));
+  const float scale2 = powers_of_two(a);
   const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
   const LaneOffsets offsets = lane_offsets<DIM>(lane, 1 << a.v.log2_page);
   for (int64_t u = u_begin; u < u_end;) {
@@ -175,25 +173,27 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       load_half<DIM>(places.of_lane(at + 1), 1 << a.v.log2_page, offsets, 1, ahead);
       return Step{token_of(k), present_of(k)};
     };
-    bool wild = false, again, waiting = true;
+    bool wild = false, waiting = true;
     RowState<DIM, NT> st;
 #pragma unroll
     for (int n = 0; n < NT; ++n) st.top[n] = 16 * n + n_lane < rows ? kNothing : 0;  // what is not a row waits for nothing
-    // Nothing in this loop changes the accumulators but the products, on every way through it: only so do they stay in one
-    // place.
-    do {
-      again = false;
+    // A pass over the tokens (see kFirst); returns whether the later passes have to follow. They are a loop of their own, which
+    // costs the first one no registers. Nothing in the loop changes the accumulators but the products, on every way through it:
+    // only so do they stay in one place.
+    auto go = [&](auto is_first, int pass) {
+      constexpr bool kIsFirst = decltype(is_first)::value;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (!kIsFirst && pass == kMaximum) st.top[n] = kNothing;
         st.sum[n] = 0;
 #pragma unroll
         for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
       }
       look_up(first);
       int k = find(first);
-      if (k >= last) break;
+      if (k >= last) return false;
       Step next = fetch(k);
-      bool more;
+      bool more, again;
       do {
         const Step now = next;
         KvTile<DIM> t = ahead;
@@ -201,10 +201,13 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
         more = k < last;
         if (more) next = fetch(k);
         const bool whole = tile_whole(now.token0, now.there);
-        again = attend_tile<DIM, NT, kParts>(t, q, st, scale2, lane, whole, now.token0, now.there & 1, now.there & 2, sight,
-                                             wild, waiting);
+        again = attend_tile<kIsFirst, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
+                                                       now.there & 2, sight, wild, waiting);
       } while (more && !again);
-    } while (again);
+      return again;
+    };
+    if (go(std::true_type{}, kFirst))
+      for (int pass = kMaximum; pass <= kRounded; ++pass) go(std::false_type{}, pass);
     u = u_item + last;
 
     // The four waves' states, 16 rows at a time, into the result or into a part.

@@ -202,9 +202,6 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
     req = same(found.req);
   }
 
-  // scores in powers of two; a negative scale goes to the queries' signs
-  // (a scale of 0 becomes the smallest number, with which a masked score stays where it is)
-  const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, __uint_as_float(1u));
   const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
   const int page = 1 << a.v.log2_page;
   // a wave's share of the decoding
@@ -367,10 +364,10 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
     for (int n = 0; n < NT; ++n)  // no row waits for nothing
       st.top[n] = 16 * (wave * NT + n) + n_lane < rows ? kNothing : 0;
     bool waiting = true;
-    // A wave's rows and the tile in `from`. Returns whether the item has to be begun again (see raise_reference).
-    auto multiply = [&](const Step &s, const ManyStage<DIM> &from) {
+    // A wave's rows and the tile in `from`, in pass `pass` (see kFirst), which takes scores in units of `unit` powers of two.
+    // `again` is set if the item has to be begun again.
+    auto multiply = [&](const Step &s, const ManyStage<DIM> &from, int pass, float unit, int &again) {
       const bool whole = sees_all(s.token0, s.there, wave_first, wave_after);
-      bool passed = false;
       // All fragments of a product are on their way from LDS before it begins: those of the values under the softmax, those
       // of the next keys under the values' product. Reads of LDS keep their place at the fences, all else may move.
       auto fence = [] { __builtin_amdgcn_sched_barrier(0x67f); };
@@ -409,11 +406,14 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
               x[n][j / 4][j % 4] = sees ? x[n][j / 4][j % 4] : kNothing;
             }
         }
-        if (waiting) waiting = first_reference<NT>(x, scale2, st);
+        if (waiting) {  // in the later passes always
+          if (pass == kFirst) waiting = first_reference<NT>(x, unit, st, again);
+          else round_scores<NT>(x, powers_of_two(a), st, pass);
+        }
         u32x4 w[kParts][NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) weights<kParts>(x[n], scale2, st.top[n], st.sum[n], w, n);
-        passed |= raise_reference<NT>(x, scale2, st);
+        for (int n = 0; n < NT; ++n) weights<kParts>(x[n], unit, st.top[n], st.sum[n], w, n);
+        if (sum_passed<NT>(st)) again = 1;
         if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
         for (int i = 0; i < Shape::kValueFrags; ++i)
@@ -422,15 +422,18 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
 #pragma unroll
             for (int p = 0; p < kParts; ++p) st.acc[n][i] = mfma(values[i], w[p][n], st.acc[n][i]);
       }
-      return passed;
     };
 
-    bool again;
     if (threadIdx.x == 0) again_at[0] = again_at[1] = wild_any = 0;
-    do {
-      again = false;
+    // The passes share one loop: with a second one for the later passes, registers of the first were spilled (1.17 ms instead of
+    // 1.08 for the two prompts).
+    for (int pass = kFirst;; ++pass) {
+      const float unit = pass == kFirst ? powers_of_two(a) : 1.0f;
+      bool again = false;
+      waiting = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (pass == kMaximum) st.top[n] = kNothing;
         st.sum[n] = 0;
 #pragma unroll
         for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
@@ -450,19 +453,16 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
         decode(next, stage[~k & 1]);
         const int t_then = more ? find(t + 1) : last;
         const Step then = fetch(t_then < last ? t_then : page_base);
-        if (multiply(now, stage[k & 1])) again_at[k & 1] = 1;
+        multiply(now, stage[k & 1], pass, unit, again_at[k & 1]);
         __syncthreads();
         // This word is written again two tiles on only, behind the next barrier: all waves read the same.
-        again = again_at[k & 1] != 0;
+        again = pass == kFirst && again_at[k & 1] != 0;
         if (!more || again) break;
         now = next, next = then, t = t_then;
         more = t < last;
       }
-      if (again) {
-        __syncthreads();
-        if (threadIdx.x == 0) again_at[0] = again_at[1] = 0;
-      }
-    } while (again);
+      if (pass == kFirst ? !again : pass == kRounded) break;
+    }
     u = u_item + last / kSub;
 
     // Each wave's rows into the result or into a part.
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
 #pragma unroll 1
             for (int half = 0; half < kHalves; ++half) {
               const int j0 = token_of(t) + 16 * half;
-              add_left_out<T, DIM>(a, head, page_at(a, table, span, j0), j0, q_row, sees, scale2, base, d0, o);
+              add_left_out<T, DIM>(a, head, page_at(a, table, span, j0), j0, q_row, sees, powers_of_two(a), base, d0, o);
             }
           }
         }
