@@ -542,9 +542,9 @@ int attn_many_groups() { return 256; }
 
 template <typename T, int DIM>
 static void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  // A list of items costs a launch; every workgroup counts for itself where that takes no longer.
+  // A list of items costs a launch; every workgroup counts for itself where that takes no longer, or there is nothing to count.
   const AttnItem *items = nullptr;
-  if (a.requests > 256 || s.room > 1024) {
+  if (a.requests > 256 || (a.requests > 0 && s.room > 1024)) {
     hipLaunchKernelGGL(page_attention_items_kernel<many_rows(DIM)>, dim3(1), dim3(1024), 0, stream, a, s.first_item, s.items, s.room,
                        s.count);
     items = s.items;
