@@ -532,10 +532,11 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
   return again;
 }
 
-// Eight values of a query row as a fragment: bfloat16 as they are, float16 as the sum of two.
+// Eight values of a query row as a fragment: bfloat16 as they are, float16 as the sum of two. What is not a row is 0: its
+// scores are its reference then, whatever the rows beside it score.
 template <typename T>
-__device__ __forceinline__ void query_fragment(const T *src, uint32_t flip, u32x4 &y, u32x4 &z) {
-  y = *reinterpret_cast<const u32x4 *>(src) ^ flip;
+__device__ __forceinline__ void query_fragment(const T *src, bool there, uint32_t flip, u32x4 &y, u32x4 &z) {
+  y = (*reinterpret_cast<const u32x4 *>(src) ^ flip) & (there ? 0xffffffffu : 0u);
   if constexpr (std::is_same<T, _Float16>::value) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       for (int i = 0; i < kSteps; ++i) {
         if (Q::kShared && ((n * kSteps + i) & 3) != wave) continue;  // the waves fill LDS together
         u32x4 y, z;
-        query_fragment<T>(src + 8 * i, flip, y, z);
+        query_fragment<T>(src + 8 * i, r < rows, flip, y, z);
         if constexpr (Q::kShared) {
           shared.queries[(n * kSteps + i) * kWave + lane] = y;
           if constexpr (kParts == 2) shared.queries[((NT + n) * kSteps + i) * kWave + lane] = z;

@@ -227,7 +227,7 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
       const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
                      g * (DIM / 4);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) query_fragment<T>(src + 8 * i, flip, q[0][n][i], q[kParts - 1][n][i]);
+      for (int i = 0; i < kSteps; ++i) query_fragment<T>(src + 8 * i, r < rows, flip, q[0][n][i], q[kParts - 1][n][i]);
     }
     const int sinks = a.window > 0 ? a.sinks : 0;
     // the first and the last place of the wave's rows, and of the item's
@@ -406,14 +406,14 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
               x[n][j / 4][j % 4] = sees ? x[n][j / 4][j % 4] : kNothing;
             }
         }
-        if (waiting) {  // in the later passes always
+        if (__builtin_expect(waiting, 0)) {  // in the later passes always
           if (pass == kFirst) waiting = first_reference<NT>(x, unit, st, again);
           else round_scores<NT>(x, powers_of_two(a), st, pass);
         }
         u32x4 w[kParts][NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) weights<kParts>(x[n], unit, st.top[n], st.sum[n], w, n);
-        if (sum_passed<NT>(st)) again = 1;
+        if (__builtin_expect(sum_passed<NT>(st), 0)) again = 1;
         if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
         for (int i = 0; i < Shape::kValueFrags; ++i)

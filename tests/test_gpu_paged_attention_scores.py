@@ -81,3 +81,32 @@ def test_ordinary_rows_with_enormous_scores_stay_finite(capi, power, rows, dim, 
     got, _ = _check(capi, b, max_query_len=hint)
     assert bool(got.isfinite().all())
     assert float(got.abs().max()) <= 6.0 * 1.01                        # values are 6 at most: weights sum up to 1
+
+
+@pytest.mark.parametrize("requests, q, group, kv_heads", [(32, 1, 4, 8), (16, 7, 3, 8), (8, 180, 3, 1)])
+def test_a_constant_in_all_scores_costs_nothing(capi, requests, q, group, kv_heads):
+    """A score's distance from 0 is nothing that a softmax depends on. Items have lanes that hold no row (12 of 16, 11 of 32,
+    the most of the last 256): what those make of scores must not send the item's rows through their tokens again, which takes
+    half as long again at least. A quarter is allowed, of the least of many times, three times over."""
+    b = Batch(1, [4000] * requests, [q] * requests, group * kv_heads, kv_heads, 128, 16, torch.bfloat16)
+    b.cache[:, :, 0, :, 0] = b.cache[:, :, 0, :, 0] & 0xF0 | 2         # dimension 0 of every key: 1
+    live = b.scales[:, :, 0, 0] != 255
+    b.scales[:, :, 0, 0] = torch.where(live, torch.tensor(127, dtype=torch.uint8), b.scales[:, :, 0, 0])
+    args = b.args()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+
+    def least(constant):
+        args[0][..., 0] = constant / b.scale
+        times = []
+        for _ in range(30):
+            begin.record()
+            for _ in range(10):
+                capi.page_attention(*args, b.scale, max_query_len=q)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+
+    least(0)
+    pairs = [(least(0), least(40)) for _ in range(3)]
+    assert any(far < 1.25 * near for near, far in pairs), pairs
