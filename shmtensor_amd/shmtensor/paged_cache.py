@@ -16,6 +16,8 @@ import torch
 
 from . import capi
 
+_STEPS_AHEAD = 32
+
 
 class Step:
     """One step's plan, all on the GPU but the counts: query_starts [requests + 1], kv_lens [requests], positions and
@@ -29,7 +31,7 @@ class Step:
 class PagedCache:
     """`requests` places for requests of up to `max_len` tokens, sharing `pages` pages of `page` tokens. All layers use
     the same block table. The host keeps the requests' lengths and how many pages are free, so that no step waits for
-    the GPU; which pages they are is known to the GPU only."""
+    the GPU (until it is _STEPS_AHEAD steps behind); which pages they are is known to the GPU only."""
 
     def __init__(self, pages, kv_heads, dim, requests, max_len, layers=1, page=16, device="cuda"):
         self.page, self.max_len = page, max_len
@@ -42,6 +44,11 @@ class PagedCache:
         self._dropped = [(0, 0)] * requests          # pages [from, to) of a request that trim() gave back
         self._free = torch.arange(pages, dtype=torch.int32, device=device)
         self._kv_lens = torch.zeros(requests, dtype=torch.int32, device=device)
+        # New lengths on their way to the GPU: from memory that is not pinned a copy waits for all that is queued, and so does
+        # pinning memory. A place is written again when its copy has run.
+        self._staging = torch.empty((_STEPS_AHEAD, requests), dtype=torch.int32, pin_memory=True)
+        self._copied = [None] * _STEPS_AHEAD
+        self._turn = 0
 
     @property
     def free_pages(self):
@@ -49,6 +56,17 @@ class PagedCache:
 
     def _pages(self, tokens):
         return -(-tokens // self.page)
+
+    def _to_device(self, lens):
+        at = self._turn = (self._turn + 1) % _STEPS_AHEAD
+        if self._copied[at] is None:
+            self._copied[at] = torch.cuda.Event()
+        else:
+            self._copied[at].synchronize()
+        self._staging[at].numpy()[:] = lens
+        there = self._staging[at].to(self._free.device, non_blocking=True)
+        self._copied[at].record()
+        return there
 
     def plan(self, new_lens):
         """Pages and slots for new_lens[r] further tokens of every request r (host integers). Raises RuntimeError, and
@@ -62,7 +80,7 @@ class PagedCache:
         need = int((self._pages(total) - self._pages(self.lens)).sum())
         if need > self.free_pages:
             raise RuntimeError("%d pages needed, %d free" % (need, self.free_pages))
-        device_new = torch.from_numpy(new.astype(np.int32)).to(self._free.device)
+        device_new = self._to_device(new)
         starts, kv_lens, positions, slots, _ = capi.page_plan(self._kv_lens, device_new, self.block_table, self._free,
                                                               self.page, int(new.sum()))
         self._free, self._kv_lens, self.lens = self._free[need:], kv_lens, total
@@ -85,8 +103,12 @@ class PagedCache:
 
     def _give_back(self, request, first, end):
         if first < end:
-            self._free = torch.cat([self._free, self.block_table[request, first:end]])
-            self.block_table[request, first:end] = -1
+            pages, n = self.block_table[request, first:end], self.free_pages
+            free = self._free.new_empty(n + end - first)     # (torch.cat pins memory for its arguments, and may wait for that)
+            free[:n].copy_(self._free)
+            free[n:].copy_(pages)
+            self._free = free
+            pages.fill_(-1)
 
     def release(self, request):
         """The request is done; its place is empty again."""
@@ -96,7 +118,7 @@ class PagedCache:
         self._dropped[request] = (0, 0)
         self.lens[request] = 0
         self._kv_lens = self._kv_lens.clone()        # a step that is still in use keeps its own
-        self._kv_lens[request] = 0
+        self._kv_lens[request:request + 1].zero_()
 
     def trim(self, request, window, sinks=0):
         """Gives back the pages that no further query of the request can see with this window and these sinks."""
