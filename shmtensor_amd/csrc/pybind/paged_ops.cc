@@ -30,6 +30,12 @@ void check_device(const torch::Tensor &t, const torch::Tensor &like, const char 
   TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", the cache on ", like.device());
 }
 
+// Nothing is learned through the rounded rows of a cache: a gradient that somebody waits for is refused, not lost.
+void check_no_grad(const torch::Tensor &t, const char *name) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
+              " requires a gradient, which the paged cache does not give: call it under torch.no_grad() or detach() first");
+}
+
 bool page_contiguous(const torch::Tensor &t) {
   int64_t want = 1;
   for (int64_t d = 4; d >= 1; --d) {
@@ -135,6 +141,8 @@ void page_set(const torch::Tensor &cache, const torch::Tensor &scales, torch::Te
   check_device(slots, cache, "slots");
   check_device(keys, cache, "keys");
   check_device(values, cache, "values");
+  check_no_grad(keys, "keys");
+  check_no_grad(values, "values");
   const int64_t n = slots.numel();
   const int64_t sizes[3] = {n, c.kv_heads, c.dim};
   const at::IntArrayRef shape(sizes);
@@ -171,6 +179,7 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
                           bool return_lse) {
   const shmt_paged_cache c = describe(cache, scales);
   check_device(query, cache, "query");
+  check_no_grad(query, "query");
   check_device(block_table, cache, "block_table");
   const int64_t stride = table_stride(block_table);
   query_starts = cuda_ids(query_starts, "query_starts");
