@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void page_fetch_kernel(RowsArgs a) {
 
 // 64 tokens a workgroup where that makes enough of them to fill the card, else as few as its lanes can hold.
 template <typename T, int DIM>
-void launch_rows(const RowsArgs &a, bool set, hipStream_t s) {
+void launch_some_rows(const RowsArgs &a, bool set, hipStream_t s) {
   constexpr int kMany = DIM / 32, kOne = 2048 / DIM;  // passes for 64 tokens; tokens of one pass
   const int64_t tiles = 2 * a.v.kv_heads, many = (a.tokens + 63) / 64 * tiles, few = (a.tokens + kOne - 1) / kOne * tiles;
   const dim3 block(256);
@@ -371,6 +371,20 @@ void launch_rows(const RowsArgs &a, bool set, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(few));
     if (set) hipLaunchKernelGGL((page_set_kernel<T, DIM, 1>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((page_fetch_kernel<T, DIM, 1>), grid, block, 0, s, a);
+  }
+}
+
+// A launch has less than 2^32 threads; more rows are more launches.
+template <typename T, int DIM>
+void launch_rows(const RowsArgs &all, bool set, hipStream_t s) {
+  const int64_t each = ((int64_t{1} << 24) - 1) / (2 * all.v.kv_heads) * 64;
+  RowsArgs a = all;
+  for (int64_t t0 = 0; t0 < all.tokens; t0 += each) {
+    a.tokens = std::min(each, all.tokens - t0);
+    a.slots = static_cast<const char *>(all.slots) + t0 * all.slot_bytes;
+    a.keys = static_cast<const T *>(all.keys) + t0 * all.key_token;
+    a.values = static_cast<const T *>(all.values) + t0 * all.value_token;
+    launch_some_rows<T, DIM>(a, set, s);
   }
 }
 
