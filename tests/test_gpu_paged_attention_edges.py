@@ -1,8 +1,11 @@
 """Attention over the paged 4-bit cache at the edges of its calls."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
+
+from test_gpu_paged_attention import Batch, _check
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,3 +37,30 @@ def test_no_requests(capi, cabi, tokens, heads, kv_heads, dim):
     assert rc == 0, lib.shmt_last_error()
     torch.cuda.synchronize()
     assert bool((got == 0).all()) and bool(lse.isneginf().all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_more_items_than_one_round_of_the_list(capi, dim):
+    """1,500 requests in the kernel for many rows: the list of items takes two rounds of 1,024, finding a workgroup's first
+    item in it takes two of 512."""
+    rng = np.random.default_rng(dim)
+    q = rng.integers(1, 4, 1500)
+    lens = q + rng.integers(0, 20, 1500)
+    b = Batch(dim, lens, q, 2, 1, dim, 16, torch.bfloat16)
+    _check(capi, b, max_query_len=2000)
+    _check(capi, b, max_query_len=2000, window=5, sinks=1)
+
+
+@pytest.mark.parametrize("dim, items", [(64, 518), (128, 518), (256, 780)])
+def test_more_items_than_threads_without_a_list(capi, dim, items):
+    """256 requests of two items and more: every workgroup counts them in two rounds of 512."""
+    rng = np.random.default_rng(dim)
+    q = np.full(256, 33)
+    q[rng.permutation(256)[:6]] = 65
+    assert (-(-q * 8 // (128 if dim == 256 else 256))).sum() == items
+    lens = q + rng.integers(0, 9, 256)
+    b = Batch(dim, lens, q, 8, 1, dim, 16, torch.bfloat16)
+    _check(capi, b, window=20, sinks=2)
+    got = [capi.page_attention(*b.args(), b.scale, max_query_len=hint, return_lse=True) for hint in (65, 1)]
+    for x, y in zip(*got):                                             # the kernel for few rows counts otherwise; each within 2^-7
+        assert bool(((x - y).abs() <= 2.0 ** -6 * (1 + y.abs())).all())
