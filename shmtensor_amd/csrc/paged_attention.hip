@@ -6,9 +6,9 @@
 // are on their way; three waves a SIMD keep 52 KB of a compute unit's share of HBM in flight. Units of 128 tokens are dealt out
 // evenly (paged_attention.h), so a batch of ragged requests, one long request and anything between are one case. Measured, 32
 // requests of 8,000 tokens, 8 heads of 128, bfloat16: 56 us, 5.0 TB/s, what a copy reaches; 64 ragged requests of 1,000 to
-// 16,000 tokens 84 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 47 us, 3.0 TB/s, of which the join 7 us.
+// 16,000 tokens 84 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 46 us, 3.1 TB/s, of which the join 7 us.
 // At 64 dimensions half the bytes come with the same softmax, and the vector units are what it waits for: 96 requests with a
-// window of 4,000 tokens, float16, 67 us, 3.1 TB/s (214 vector instructions for 32 tokens of a wave).
+// window of 4,000 tokens, float16, 66 us, 3.1 TB/s (some 230 vector instructions for 32 tokens of a wave).
 #include "paged_attention.h"
 #include "paged_host.h"
 
@@ -317,10 +317,10 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, in
   AttnShape s;
   // Which kernel. 32 rows at a time, read anew for each 32, against 256 (128) rows that share what is decoded, of which a last
   // item that is not full costs as much as a full one: 16 requests of 8,000 tokens, 8 heads, 128 / 192 / 256 / 320 rows a
-  // request, bfloat16: 108 / 165 / 203 / 269 us and 151 / 155 / 160 / 263 us (float16: 141 / 221 / 269 / 362 and 241 / 244 / 247
-  // / 423; 64 dimensions: 85 / 108 / 150 / 188 and 110 / 112 / 116 / 199; 256 dimensions, 64 / 96 rows: 174 / 281 and 197 / 202).
+  // request, bfloat16: 114 / 165 / 203 / 267 us and 142 / 147 / 152 / 257 us (float16: 143 / 210 / 264 / 343 and 216 / 220 / 225
+  // / 401; 64 dimensions: 87 / 111 / 153 / 191 and 103 / 106 / 110 / 186; 256 dimensions, 64 / 96 rows: 173 / 275 and 185 / 190).
   // So an item costs as much as 6 (2) of 32 rows. Where there are few items most of the card idles behind the first of them:
-  // one request of 8,000 tokens, 384 / 512 / 768 rows: 45 / 52 / 67 us and 48 / 50 / 56 us.
+  // one request of 8,000 tokens, 384 / 512 / 768 rows: 45 / 53 / 67 us and 45 / 53 / 59 us.
   const int64_t few_items = (rows + 31) / 32, many_items = (rows + many_rows(dim) - 1) / many_rows(dim);
   s.many = rows > 2 * many_rows(dim) ||
            (few_items > (dim == 256 ? 2 : 6) * many_items && tokens * group * kv_heads >= 16384);

@@ -55,17 +55,18 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them.
 // Bound by what the vector units and the matrix cores have to issue: for 64 tokens a wave has 64 products, of which each keeps
 // the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 200 vector
-// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.08
-// ms, 985 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
+// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.10
+// ms, 962 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
 // its own tokens 2.24 ms; 128 rows and four waves, tiles of 64 decoded once, 1.63; reading ahead in LDS, 1.56; addresses held
 // by lanes and items weighted, 1.37; no maximum from tile to tile, 1.23; 256 rows and tiles of 128, 1.08 (64 dimensions 0.94
-// to 0.82). Products and softmaxes ordered by hand to run beside each other lost (1.71 against 1.56), priorities for the
-// products brought nothing; products on the 4-bit keys themselves would need the queries in 8 bits, and lose bits of sums whose
-// terms differ by much (2^-14 of the terms' sizes, measured).
+// to 0.82); passes that may follow for large scores in the same loop, 1.10 (0.78). Products and softmaxes ordered by hand to
+// run beside each other lost (1.71 against 1.56), priorities for the products brought nothing; products on the 4-bit keys
+// themselves would need the queries in 8 bits, and lose bits of sums whose terms differ by much (2^-14 of the terms' sizes,
+// measured).
 // At 256 dimensions 32 rows leave room for one wave on a SIMD only: eight waves of 16 rows and tiles of 64 tokens, as the LDS
-// has room for. They read it twice as often but wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (680
-// TFLOP/s) against 1.02 with four waves of 32 rows and tiles of 32 tokens and 0.95 with eight and 32; chunks of 17 to 2,000
-// tokens behind a window 87 us against 95 and 92.
+// has room for. They read it twice as often but wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (0.76
+// now, 710 TFLOP/s) against 1.02 with four waves of 32 rows and tiles of 32 tokens and 0.95 with eight and 32; chunks of 17 to
+// 2,000 tokens behind a window 87 us against 95 and 92.
 template <int DIM>
 struct ManyShape {
   static constexpr int kTile = DIM == 256 ? 64 : 128;  // tokens
