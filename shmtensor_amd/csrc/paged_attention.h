@@ -367,13 +367,14 @@ __device__ __forceinline__ void weights(const f32x4 (&s)[2], float unit, float t
 // References. Weights are taken relative to the maximum of the first tile in which a row sees anything: with floats' exponents
 // any reference near the true maximum does as well as that, so there is no maximum to follow from tile to tile and nothing to
 // rescale (kFirst). Two things make that too little. A row's later scores may be so much greater that its weights sum up to more
-// than 2^40. And a weight comes from the product score * scale as it is, the reference is that product rounded: from 2^30 on,
-// half a unit in its last place is more than an exponent of 2 may move by, and weights would be anything. Where either happens
-// (the second from 2^12 on) the tokens are gone through twice more, with scores in powers of two that are rounded: once for each
-// row's maximum (kMaximum), once with that as the reference (kRounded), to which no weight is above 1. So there are three passes
-// at most, whatever the scores are. Waves that share a row may have weighted it either way: below 2^12 that makes a difference
-// of 2^-13 of a weight, and scores that are tied stay tied above.
-enum : int { kFirst, kMaximum, kRounded };
+// than 2^40: then the tokens are begun again, with a reference that is greater by as much (kRaised). And a weight comes
+// from the product score * scale as it is, the reference is that product rounded: from 2^30 on, half a unit in its last place
+// is more than an exponent of 2 may move by, and weights would be anything. Where a reference is far from 0 (2^12), or
+// raising it once was not enough, the tokens are gone through twice, with scores in powers of two that are rounded: once for
+// each row's maximum (kMaximum), once with that as the reference (kRounded), to which no weight is above 1. So there are four
+// passes at most, whatever the scores are. Waves that share a row may have weighted it either way: below 2^12 that makes a
+// difference of 2^-13 of a weight, and scores that are tied stay tied above.
+enum : int { kFirst, kRaised, kMaximum, kRounded };
 constexpr float kPassed = 1099511627776.0f;  // 2^40
 constexpr float kFar = 4096.0f;
 
@@ -391,19 +392,19 @@ __device__ __forceinline__ float powers_of_two(const AttnArgs &a) {
   return fmaxf(fabsf(a.scale) * 1.44269504088896340736f, __uint_as_float(1u));
 }
 
-// Rows without a reference take this tile's maximum. Returns whether any is still without; `again` is set for one that is far
-// from 0.
+// Rows without a reference take this tile's maximum. Returns whether any is still without; `again` and `far` are set for one
+// that is far from 0.
 template <int NT, typename State, typename Flag>
-__device__ __forceinline__ bool first_reference(const f32x4 (&s)[NT][2], float scale2, State &st, Flag &again) {
-  bool none = false, far = false;
+__device__ __forceinline__ bool first_reference(const f32x4 (&s)[NT][2], float scale2, State &st, Flag &again, Flag &far) {
+  bool none = false, is_far = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float most = most_of<NT>(s, n) * scale2;
     st.top[n] = st.top[n] == kNothing ? most : st.top[n];
     none |= st.top[n] == kNothing;
-    far |= st.top[n] != kNothing && fabsf(st.top[n]) >= kFar;
+    is_far |= st.top[n] != kNothing && fabsf(st.top[n]) >= kFar;
   }
-  if (__ballot(far)) again = 1;
+  if (__ballot(is_far)) again = far = 1;
   return __ballot(none) != 0;
 }
 
@@ -420,13 +421,26 @@ __device__ __forceinline__ void round_scores(f32x4 (&s)[NT][2], float scale2, St
   for (int n = 0; n < NT; ++n) st.top[n] = fmaxf(st.top[n], most_of<NT>(s, n));
 }
 
-// Whether a row's sum has passed 2^40.
-template <int NT, typename State>
-__device__ __forceinline__ bool sum_passed(const State &st) {
+// Where a row's sum has passed 2^40: a reference that is greater by the sum's logarithm, so that no weight so far is above 1 to
+// it, and a new sum, which is for the rest of the pass to see whether that is enough. `again` is set if there is such a row,
+// `far` if its reference is far from 0 (an infinite sum has an infinite logarithm).
+template <int NT, typename State, typename Flag>
+__device__ __forceinline__ void raise_reference(State &st, Flag &again, Flag &far) {
   bool passed = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) passed |= st.sum[n] > kPassed;
-  return __ballot(passed) != 0;
+  if (__builtin_expect(__ballot(passed) == 0, 1)) return;
+  bool is_far = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float sum = across_max(st.sum[n]);
+    if (sum > kPassed) {
+      st.top[n] += __builtin_log2f(sum), st.sum[n] = 0;
+      is_far |= fabsf(st.top[n]) >= kFar;
+    }
+  }
+  again = 1;
+  if (__ballot(is_far)) far = 1;
 }
 
 // Scale bytes from here on make values that are infinite in bfloat16, or not a number.
@@ -441,11 +455,13 @@ constexpr uint32_t kWild = 253;
 // result's own rounding.
 // `whole`: all rows see all tokens. Otherwise scores are masked; and values that are not finite in bfloat16 must not meet the
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
-// FIRST: `pass` is kFirst; rows may be `waiting` for a reference. Returns whether the wave has to begin its tokens again.
+// FIRST: `pass` is kFirst or kRaised; rows may be `waiting` for a reference. `again` is set if the wave has to begin its tokens
+// again, `far` if with rounded scores.
 template <bool FIRST, int DIM, int NT, int PARTS>
-__device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
+__device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int pass, int lane, bool whole, int token0, bool there0,
-                                            bool there1, const Sight<NT> &sight, bool &wild, bool &waiting) {
+                                            bool there1, const Sight<NT> &sight, bool &wild, bool &waiting, bool &again,
+                                            bool &far) {
   const int g = lane >> 4;
   f32x4 s[NT][2];
 #pragma unroll
@@ -488,13 +504,12 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
         wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
       }
   }
-  bool again = false;
   if constexpr (!FIRST) round_scores<NT>(s, scale2, st, pass);
-  else if (waiting) waiting = first_reference<NT>(s, scale2, st, again);
+  else if (waiting) waiting = first_reference<NT>(s, scale2, st, again, far);
   u32x4 w[PARTS][NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) weights<PARTS>(s[n], FIRST ? scale2 : 1.0f, st.top[n], st.sum[n], w, n);
-  if constexpr (FIRST) again |= sum_passed<NT>(st);
+  if constexpr (FIRST) raise_reference<NT>(st, again, far);
   // The conversion reads nothing of a scale but its exponent field, so the byte need not be cut out.
   float f[8];
 #pragma unroll
@@ -529,7 +544,6 @@ __device__ __forceinline__ bool attend_tile(KvTile<DIM> &t, const Queries<DIM, N
       two(std::integral_constant<int, 3>{});
     }
   }
-  return again;
 }
 
 // Eight values of a query row as a fragment: bfloat16 as they are, float16 as the sum of two. What is not a row is 0: its

@@ -173,12 +173,12 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       load_half<DIM>(places.of_lane(at + 1), 1 << a.v.log2_page, offsets, 1, ahead);
       return Step{token_of(k), present_of(k)};
     };
-    bool wild = false, waiting = true;
+    bool wild = false, waiting = true, far = false;
     RowState<DIM, NT> st;
 #pragma unroll
     for (int n = 0; n < NT; ++n) st.top[n] = 16 * n + n_lane < rows ? kNothing : 0;  // what is not a row waits for nothing
-    // A pass over the tokens (see kFirst); returns whether the later passes have to follow. They are a loop of their own, which
-    // costs the first one no registers. Nothing in the loop changes the accumulators but the products, on every way through it:
+    // A pass over the tokens (see kFirst); returns whether another has to follow. The last two are a loop of their own, which
+    // costs the first ones no registers. Nothing in the loop changes the accumulators but the products, on every way through it:
     // only so do they stay in one place.
     auto go = [&](auto is_first, int pass) {
       constexpr bool kIsFirst = decltype(is_first)::value;
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
       int k = find(first);
       if (k >= last) return false;
       Step next = fetch(k);
-      bool more, again;
+      bool more, again = false;
       do {
         const Step now = next;
         KvTile<DIM> t = ahead;
@@ -201,12 +201,14 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
         more = k < last;
         if (more) next = fetch(k);
         const bool whole = tile_whole(now.token0, now.there);
-        again = attend_tile<kIsFirst, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
-                                                       now.there & 2, sight, wild, waiting);
+        attend_tile<kIsFirst, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1, now.there & 2,
+                                               sight, wild, waiting, again, far);
       } while (more && !again);
       return again;
     };
-    if (go(std::true_type{}, kFirst))
+    bool again = true;
+    for (int pass = kFirst; pass <= kRaised && again && !far; ++pass) again = go(std::true_type{}, pass);
+    if (again)
       for (int pass = kMaximum; pass <= kRounded; ++pass) go(std::false_type{}, pass);
     u = u_item + last;
 

@@ -55,11 +55,11 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them.
 // Bound by what the vector units and the matrix cores have to issue: for 64 tokens a wave has 64 products, of which each keeps
 // the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 200 vector
-// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.10
-// ms, 962 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
+// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.05
+// ms, 1,010 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
 // its own tokens 2.24 ms; 128 rows and four waves, tiles of 64 decoded once, 1.63; reading ahead in LDS, 1.56; addresses held
 // by lanes and items weighted, 1.37; no maximum from tile to tile, 1.23; 256 rows and tiles of 128, 1.08 (64 dimensions 0.94
-// to 0.82); passes that may follow for large scores in the same loop, 1.10 (0.78). Products and softmaxes ordered by hand to
+// to 0.82); what follows for large scores in the same loop but out of the way, 1.05 (0.78). Products and softmaxes ordered by hand to
 // run beside each other lost (1.71 against 1.56), priorities for the products brought nothing; products on the 4-bit keys
 // themselves would need the queries in 8 bits, and lose bits of sums whose terms differ by much (2^-14 of the terms' sizes,
 // measured).
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
   __shared__ uint64_t scan[Shape::kWaves];
   __shared__ int64_t row_range[2];  // rows of any request
   __shared__ int32_t first_item[kThreads];
-  __shared__ int again_at[2], wild_any;
+  __shared__ int again_at[2], far_any, wild_any;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_lane = lane & 15, g = lane >> 4;
   // The units of one head, and, later, the item that holds a given one of them: from the list of items, or, without one (not
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
       st.top[n] = 16 * (wave * NT + n) + n_lane < rows ? kNothing : 0;
     bool waiting = true;
     // A wave's rows and the tile in `from`, in pass `pass` (see kFirst), which takes scores in units of `unit` powers of two.
-    // `again` is set if the item has to be begun again.
+    // `again` is set if the item has to be begun again, far_any if with rounded scores.
     auto multiply = [&](const Step &s, const ManyStage<DIM> &from, int pass, float unit, int &again) {
       const bool whole = sees_all(s.token0, s.there, wave_first, wave_after);
       // All fragments of a product are on their way from LDS before it begins: those of the values under the softmax, those
@@ -407,14 +407,14 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
               x[n][j / 4][j % 4] = sees ? x[n][j / 4][j % 4] : kNothing;
             }
         }
-        if (__builtin_expect(waiting, 0)) {  // in the later passes always
-          if (pass == kFirst) waiting = first_reference<NT>(x, unit, st, again);
+        if (__builtin_expect(waiting, 0)) {  // in the last passes always
+          if (pass < kMaximum) waiting = first_reference<NT>(x, unit, st, again, far_any);
           else round_scores<NT>(x, powers_of_two(a), st, pass);
         }
         u32x4 w[kParts][NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) weights<kParts>(x[n], unit, st.top[n], st.sum[n], w, n);
-        if (__builtin_expect(sum_passed<NT>(st), 0)) again = 1;
+        raise_reference<NT>(st, again, far_any);
         if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
         for (int i = 0; i < Shape::kValueFrags; ++i)
@@ -425,13 +425,13 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
       }
     };
 
-    if (threadIdx.x == 0) again_at[0] = again_at[1] = wild_any = 0;
-    // The passes share one loop: with a second one for the later passes, registers of the first were spilled (1.17 ms instead of
+    if (threadIdx.x == 0) again_at[0] = again_at[1] = far_any = wild_any = 0;
+    // The passes share one loop: with a second one for the last two, registers of the first were spilled (1.17 ms instead of
     // 1.08 for the two prompts).
-    for (int pass = kFirst;; ++pass) {
-      const float unit = pass == kFirst ? powers_of_two(a) : 1.0f;
+    for (int pass = kFirst;;) {
+      const float unit = pass < kMaximum ? powers_of_two(a) : 1.0f;
       bool again = false;
-      waiting = true;
+      waiting |= pass >= kMaximum;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (pass == kMaximum) st.top[n] = kNothing;
@@ -457,12 +457,15 @@ __global__ __launch_bounds__(ManyShape<DIM>::kThreads, 2) void page_attention_ma
         multiply(now, stage[k & 1], pass, unit, again_at[k & 1]);
         __syncthreads();
         // This word is written again two tiles on only, behind the next barrier: all waves read the same.
-        again = pass == kFirst && again_at[k & 1] != 0;
+        again = pass < kMaximum && again_at[k & 1] != 0;
         if (!more || again) break;
         now = next, next = then, t = t_then;
         more = t < last;
       }
-      if (pass == kFirst ? !again : pass == kRounded) break;
+      if (pass < kMaximum ? !again : pass == kRounded) break;
+      __syncthreads();  // all have read again_at
+      if (threadIdx.x == 0) again_at[0] = again_at[1] = 0;
+      pass = pass == kFirst && far_any == 0 ? kRaised : std::max<int>(pass + 1, kMaximum);
     }
     u = u_item + last / kSub;
 

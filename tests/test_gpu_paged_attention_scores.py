@@ -83,6 +83,29 @@ def test_ordinary_rows_with_enormous_scores_stay_finite(capi, power, rows, dim, 
     assert float(got.abs().max()) <= 6.0 * 1.01                        # values are 6 at most: weights sum up to 1
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", range(len(ROWS)))
+@pytest.mark.parametrize("levels", [(2,), (4,), (2, 4, 6), (6, 2)])
+@pytest.mark.parametrize("lead", [20, 25, 45, 64, 130, 1100, 3000])
+def test_a_few_tokens_far_above_all_others(capi, lead, levels, rows, dim, dtype):
+    """One token, or one after another, lead by 2^20 to 2^18,000: what one raise of the reference settles, what a second one
+    would have to, sums beyond the floats, references far from 0."""
+    lens, q, hint = ROWS[rows]
+    b = Batch(lead + dim + rows, lens, q, 4, 2, dim, 16, dtype)
+    b.query[:] = 0
+    b.query[..., 2] = 1
+    b.cache[:, :, 0, :, 1] = b.cache[:, :, 0, :, 1] & 0xF0             # dimension 2 of every key: 0
+    b.scales[:, :, 0, 0] = torch.where(b.scales[:, :, 0, 0] != 255, torch.tensor(127, dtype=torch.uint8), b.scales[:, :, 0, 0])
+    for r, n in enumerate(lens):
+        for i, level in enumerate(levels):
+            j = int(n * (0.5 + 0.4 * i / len(levels)))
+            b.cache[int(b.table[r, j // 16]), :, 0, j % 16, 1] |= {2: 4, 4: 6, 6: 7}[level]
+    b.scale = lead / 2 * np.log(2)
+    _exact(capi, b, hint)
+    _exact(capi, b, hint, window=200, sinks=3)
+
+
 @pytest.mark.parametrize("requests, q, group, kv_heads", [(32, 1, 4, 8), (16, 7, 3, 8), (8, 180, 3, 1)])
 def test_a_constant_in_all_scores_costs_nothing(capi, requests, q, group, kv_heads):
     """A score's distance from 0 is nothing that a softmax depends on. Items have lanes that hold no row (12 of 16, 11 of 32,
