@@ -55,11 +55,11 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them.
 // Bound by what the vector units and the matrix cores have to issue: for 64 tokens a wave has 64 products, of which each keeps
 // the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 200 vector
-// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.05
-// ms, 1,010 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
+// instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.06
+// ms, 1,004 TFLOP/s; a library's product of 8,192^3 reaches 1,206 here. Measured on the way, same case: 64 rows and every wave
 // its own tokens 2.24 ms; 128 rows and four waves, tiles of 64 decoded once, 1.63; reading ahead in LDS, 1.56; addresses held
 // by lanes and items weighted, 1.37; no maximum from tile to tile, 1.23; 256 rows and tiles of 128, 1.08 (64 dimensions 0.94
-// to 0.82); what follows for large scores in the same loop but out of the way, 1.05 (0.78). Products and softmaxes ordered by hand to
+// to 0.82); what follows for large scores in the same loop but out of the way, 1.06 (0.78). Products and softmaxes ordered by hand to
 // run beside each other lost (1.71 against 1.56), priorities for the products brought nothing; products on the 4-bit keys
 // themselves would need the queries in 8 bits, and lose bits of sums whose terms differ by much (2^-14 of the terms' sizes,
 // measured).
