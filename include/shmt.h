@@ -736,10 +736,9 @@ int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
  * kernel. A row of the table has room for 2^30 tokens at most, and tokens *
  * heads are below 2^30. scratch: shmt_page_attention_scratch_bytes(...) bytes
  * of device memory, 16-byte aligned, free again when the work queued has run.
- * Sums and the softmax are held in 32 bits; the weights meet the values as
- * bfloat16 (float16 queries: as the sum of two), which may move a result by
- * 2^-8 sum_j w_j |V[j]| (2^-16) besides its own rounding. The same call gives
- * the same bits. softmax_scale q . K[j] log2(e) has to lie within the range of
+ * Sums and the softmax are held in 32 bits; the weights meet the values in 16
+ * bits, for many rows of bfloat16 in 8, which may move a result by 2^-16 (2^-8)
+ * sum_j w_j |V[j]| besides its own rounding. The same call gives the same bits. softmax_scale q . K[j] log2(e) has to lie within the range of
  * 32-bit floats. Values of 2^80 and more may overflow where they would not have
  * to. No gradient goes through a cache.                                      */
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads,

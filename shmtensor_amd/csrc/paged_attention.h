@@ -450,9 +450,11 @@ constexpr uint32_t kWild = 253;
 //   S^T = K Q^T, 16 tokens x 16 rows at a time: lane (n, g) gets the scores of row n with tokens 4g .. 4g + 3, which is
 //   the place that the weights need to have as the right operand of O^T += V^T P^T (contraction over tokens, which may be
 //   numbered in any order as long as both operands agree): nothing crosses lanes but the maximum.
-// Keys and values become bfloat16 exactly. The weights of float16 queries are held as the sum of two bfloat16 (16 bits), as
-// are the queries themselves; with bfloat16 queries the weights are rounded to bfloat16, an error of the size of the
-// result's own rounding.
+// Keys and values become bfloat16 exactly. Weights are held as the sum of two bfloat16 (16 bits), as are float16 queries.
+// Rounded to one, the weights of bfloat16 queries would save half of the second product and move results by as much as their
+// own rounding does (64 ragged decodes: 2.3e-3 off instead of 1.66e-3, which is the result's rounding alone). That buys
+// nothing where HBM is the bound (these 84.5 us either way, 32 decodes of 8,000 tokens with 128 / 256 dimensions 57 / 113 us
+// against 57 / 113, with 64 41 against 38; 7 tokens each of 16 requests 45 against 40).
 // `whole`: all rows see all tokens. Otherwise scores are masked; and values that are not finite in bfloat16 must not meet the
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
 // FIRST: `pass` is kFirst or kRaised; rows may be `waiting` for a reference. `again` is set if the wave has to begin its tokens
@@ -506,9 +508,9 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
   }
   if constexpr (!FIRST) round_scores<NT>(s, scale2, st, pass);
   else if (waiting) waiting = first_reference<NT>(s, scale2, st, again, far);
-  u32x4 w[PARTS][NT];
+  u32x4 w[2][NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) weights<PARTS>(s[n], FIRST ? scale2 : 1.0f, st.top[n], st.sum[n], w, n);
+  for (int n = 0; n < NT; ++n) weights<2>(s[n], FIRST ? scale2 : 1.0f, st.top[n], st.sum[n], w, n);
   if constexpr (FIRST) raise_reference<NT>(st, again, far);
   // The conversion reads nothing of a scale but its exponent field, so the byte need not be cut out.
   float f[8];
@@ -532,7 +534,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
+        for (int p = 0; p < 2; ++p) {
           st.acc[n][8 * word + 2 * B] = mfma(lo, w[p][n], st.acc[n][8 * word + 2 * B]);
           st.acc[n][8 * word + 2 * B + 1] = mfma(hi, w[p][n], st.acc[n][8 * word + 2 * B + 1]);
         }
