@@ -313,19 +313,22 @@ __global__ __launch_bounds__(256, attn_waves(DIM, NT)) void page_attention_kerne
 
 // ---- launch ------------------------------------------------------------------------
 
-inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, int64_t requests, int64_t max_query_len) {
+inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int dim, int elem_type, int64_t requests,
+                            int64_t max_query_len) {
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
   const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
   // Which kernel. 32 rows at a time, read anew for each 32, against 256 (128) rows that share what is decoded, of which a last
-  // item that is not full costs as much as a full one: 16 requests of 8,000 tokens, 8 heads, 128 / 192 / 256 / 320 rows a
-  // request, bfloat16: 114 / 165 / 203 / 267 us and 142 / 147 / 152 / 257 us (float16: 143 / 210 / 264 / 343 and 216 / 220 / 225
-  // / 401; 64 dimensions: 87 / 111 / 153 / 191 and 103 / 106 / 110 / 186; 256 dimensions, 64 / 96 rows: 173 / 275 and 185 / 190).
-  // So an item costs as much as 6 (2) of 32 rows. Where there are few items most of the card idles behind the first of them:
-  // one request of 8,000 tokens, 384 / 512 / 768 rows: 45 / 53 / 67 us and 45 / 53 / 59 us.
+  // item that is not full costs as much as a full one. 16 requests of 8,000 tokens, 8 heads, us by the kernels for few and for many:
+  //   128 dimensions, bfloat16: 128 rows a request 130 and 135, 160 rows 167 and 136, 256 rows 236 and 144, 288 rows 277 and 243;
+  //   float16: 192 rows 208 and 212, 224 rows 245 and 214, 352 rows 376 and 386, 384 rows 405 and 388;
+  //   64 dimensions: bfloat16 128 rows 102 and 105, 160 rows 123 and 106; float16 192 rows 141 and 152, 224 rows 176 and 153;
+  //   256 dimensions: 64 rows 179 and 185, 96 rows 293 and 191; float16 64 rows 193 and 277, 96 rows 312 and 282.
+  // So an item costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the card idles
+  // behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
   const int64_t few_items = (rows + 31) / 32, many_items = (rows + many_rows(dim) - 1) / many_rows(dim);
-  s.many = rows > 2 * many_rows(dim) ||
-           (few_items > (dim == 256 ? 2 : 6) * many_items && tokens * group * kv_heads >= 16384);
+  const int64_t worth = dim == 256 ? 2 : elem_type == SHMT_F16 ? 6 : 4;
+  s.many = rows > 2 * many_rows(dim) || (few_items > worth * many_items && tokens * group * kv_heads >= 16384);
   s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;
   s.groups = s.many ? attn_many_groups() : 256 * attn_waves(dim, s.rows / 16);
   s.items = s.many ? tokens * group / s.rows + requests : 0;
@@ -390,7 +393,7 @@ int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads, int kv_head
     set_error("bad arguments for the attention's scratch size");
     return -1;
   }
-  return attn_shape(tokens, heads, kv_heads, dim, requests, max_query_len).bytes();
+  return attn_shape(tokens, heads, kv_heads, dim, elem_type, requests, max_query_len).bytes();
 }
 
 int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_t query_token_stride,
@@ -420,7 +423,7 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_
   SHMT_REQUIRE(((reinterpret_cast<int64_t>(query) | query_token_stride * 2 | query_head_stride * 2) & 15) == 0,
                "every row of query has to begin on 16 bytes");
   SHMT_REQUIRE((reinterpret_cast<int64_t>(out) & 15) == 0, "out has to begin on 16 bytes");
-  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, cache->dim, requests, max_query_len);
+  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, cache->dim, elem_type, requests, max_query_len);
   if (scratch_bytes < shape.bytes() || !scratch) {
     set_error("scratch too small: %lld bytes, needed %lld", static_cast<long long>(scratch_bytes),
               static_cast<long long>(shape.bytes()));
