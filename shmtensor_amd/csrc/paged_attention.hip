@@ -5,8 +5,8 @@
 // decode step is bound by that. A wave takes 32 tokens a step, 2,176 or 4,352 bytes at 64 or 128 dimensions, while the next 32
 // are on their way; three waves a SIMD keep 52 KB of a compute unit's share of HBM in flight. Units of 128 tokens are dealt out
 // evenly (paged_attention.h), so a batch of ragged requests, one long request and anything between are one case. Measured, 32
-// requests of 8,000 tokens, 8 heads of 128, bfloat16: 56 us, 5.0 TB/s, what a copy reaches; 64 ragged requests of 1,000 to
-// 16,000 tokens 84 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 46 us, 3.1 TB/s, of which the join 7 us.
+// requests of 8,000 tokens, 8 heads of 128, bfloat16: 57 us, 4.9 TB/s, what a copy reaches; 64 ragged requests of 1,000 to
+// 16,000 tokens 85 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 46 us, 3.1 TB/s, of which the join 7 us.
 // At 64 dimensions half the bytes come with the same softmax, and the vector units are what it waits for: 96 requests with a
 // window of 4,000 tokens, float16, 66 us, 3.1 TB/s (some 230 vector instructions for 32 tokens of a wave).
 #include "paged_attention.h"
