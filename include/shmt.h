@@ -636,7 +636,7 @@ int shmt_subcsr_copy_rows(const void *indptr, const void *indices,
                           void *cache_indices, void *stream);
 
 /* ------------------------------------------------------------------ */
-/* Paged key/value cache of a language model, held in 4 bits. No counterpart
+/* Paged key/value cache of a language model, held in 4 (or 8) bits. No counterpart
  * in the reference: its caches hold rows bit for bit (src/cache_feature_set.cu,
  * src/cache_feature_fetch.cu), under slots that a map gives; here a row is
  * rounded, and its slot comes from a block table.
@@ -715,6 +715,70 @@ int shmt_page_set(const shmt_paged_cache *cache, const void *slots,
 int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
                     int slot_bytes, int64_t n, void *keys, void *values,
                     int elem_type, void *stream);
+
+/* The same over a cache that holds its values in `bits` = 4 or 8 bits. In 8
+ * bits a value is a float of 8 bits (sign, 4 exponent bits, 3 mantissa bits,
+ * no infinities, 2^-9 .. 448 in size):
+ *   cache   uint8 [pages][kv_heads][2][page][dim]
+ * and the power of two of 32 values the smallest with max |x| < 464 * 2^e. All
+ * else is as in 4 bits. A cache is written and read with one number of bits.  */
+int shmt_page_set_as(const shmt_paged_cache *cache, int bits,
+                     const void *slots, int slot_bytes, int64_t n,
+                     const void *keys, int64_t key_token_stride,
+                     int64_t key_head_stride, const void *values,
+                     int64_t value_token_stride, int64_t value_head_stride,
+                     int elem_type, void *stream);
+int shmt_page_fetch_as(const shmt_paged_cache *cache, int bits,
+                       const void *slots, int slot_bytes, int64_t n, void *keys,
+                       void *values, int elem_type, void *stream);
+
+/* Trees of drafted tokens. A step's new tokens of request b, rows
+ * query_starts[b] .. query_starts[b + 1), are the nodes of a tree (or of
+ * several): parents[row] is the parent's index among the request's nodes, in
+ * front of the node's own, or -1 (as any other value is taken). Node i is the
+ * request's token kv_lens[b] - n + i for the cache, n being its nodes: it has
+ * that token's slot, but the position in the text is
+ *   positions[row] = kv_lens[b] - n + depth of the node   (a root's depth is 0)
+ * nodes[row] are four words, which the attention reads:
+ *   the node's number in preorder, children and roots in ascending order;
+ *   the nodes of its subtree, itself among them; its depth;
+ *   the least depth from this node to the request's last one.
+ * Rows of no request get -1. nodes: int32 [tokens][4], on 16 bytes. A tree is
+ * as large as it likes to be; those of up to 64 nodes, and chains, are the
+ * quick ones. query_starts must not descend; starts and kv_lens are len_bytes in
+ * {4,8} wide.                                                               */
+int shmt_page_tree(const int32_t *parents, const void *query_starts,
+                   const void *kv_lens, int len_bytes, int64_t requests,
+                   int64_t tokens, int32_t *nodes, int32_t *positions,
+                   void *stream);
+
+/* The end of a step over trees: of each request the path that the model agrees
+ * with, and its rows where they would lie had nothing else been drafted.
+ * tokens[row] is a node's token, picked[row] the model's choice behind it
+ * (token_bytes in {4,8} wide). The first given[b] nodes (given NULL: 1; at
+ * least 1, at most n) are not drafts but stand as they are, one behind the
+ * other; from the last of them on, the path goes on to the first child whose
+ * token is the one that was picked at its parent, as long as there is one.
+ *   counts[b]            nodes on the path
+ *   path[row of node k]  the k-th of them, k < counts[b]; behind that, and in
+ *                        rows of no request, -1
+ *   next[b]              picked at the path's end (token_bytes wide); -1 for a
+ *                        request without nodes, whose count is 0
+ * and in each of `layers` caches of one layout (strides between them in bytes;
+ * addresses, pages and layers on 16 bytes) the keys and values of the k-th node
+ * are copied to the place of node k, codes and scales as they are. Other rows
+ * are not touched; where a place or a row has no page, nothing is copied. The request
+ * holds kv_lens[b] - n + counts[b] tokens then, at positions without a gap.
+ * Requests must not share pages that are written. cache->cache and
+ * cache->scales are the first layer's.                                      */
+int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers,
+                   int64_t cache_layer_stride, int64_t scales_layer_stride,
+                   const int32_t *block_table, int64_t width,
+                   int64_t table_stride, const void *query_starts,
+                   const void *kv_lens, int len_bytes, int64_t requests,
+                   int64_t rows, const int32_t *parents, const void *tokens,
+                   const void *picked, int token_bytes, const int32_t *given,
+                   int32_t *counts, int32_t *path, void *next, void *stream);
 
 /* Attention over the cache. Request b's queries are rows query_starts[b] ..
  * query_starts[b + 1) of `query` [tokens, heads, dim] (strides in elements, a

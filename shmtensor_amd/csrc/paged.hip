@@ -1,4 +1,4 @@
-// The paged key/value cache held in 4 bits: block tables and slot maps from
+// The paged key/value cache held in 4 or 8 bits: block tables and slot maps from
 // request lengths (shmt_page_plan), rows into the cache (shmt_page_set) and
 // out of it (shmt_page_fetch). The attention that reads it is in
 // paged_attention.hip.
@@ -8,6 +8,7 @@
 #include "wave.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace shmt {
 
@@ -250,6 +251,50 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
   }
 }
 
+// Eight values of a row.
+template <int BITS>
+using Codes = std::conditional_t<BITS == 8, uint64_t, uint32_t>;
+
+// The byte of the smallest power of two with most < 7 * 2^e, in 8 bits 464 * 2^e: nothing is cut by more than half the step at
+// its place (6 is the largest code, 7 the middle between it and the 8 that there is not; 448, 464 and 480).
+template <int BITS>
+__device__ __forceinline__ int power_of(uint32_t most) {
+  if constexpr (BITS == 8) return max(static_cast<int>((most + 0x180000u) >> 23) - 8, 0);
+  else return max(static_cast<int>((most + 0x200000u) >> 23) - 2, 0);
+}
+
+template <int BITS>
+__device__ __forceinline__ Codes<BITS> encode8(const float (&x)[8], float s) {
+  if constexpr (BITS == 8) {
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    i16x2 lo{}, hi{};
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0], x[1], s, false);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2], x[3], s, true);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[4], x[5], s, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[6], x[7], s, true);
+    return static_cast<uint64_t>(__builtin_bit_cast(uint32_t, hi)) << 32 | __builtin_bit_cast(uint32_t, lo);
+  } else {
+    uint32_t codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], s, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], s, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], s, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], s, 3);
+  }
+}
+
+template <int BITS>
+__device__ __forceinline__ void decode8(Codes<BITS> codes, float s, float (&x)[8]) {
+  f32x2 y[4];
+  if constexpr (BITS == 8) {
+    const uint32_t lo = static_cast<uint32_t>(codes), hi = static_cast<uint32_t>(codes >> 32);
+    y[0] = decode2_f32_8<0>(lo, s), y[1] = decode2_f32_8<1>(lo, s), y[2] = decode2_f32_8<0>(hi, s), y[3] = decode2_f32_8<1>(hi, s);
+  } else {
+    y[0] = decode2_f32<0>(codes, s), y[1] = decode2_f32<1>(codes, s), y[2] = decode2_f32<2>(codes, s), y[3] = decode2_f32<3>(codes, s);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = y[j / 2][j % 2];
+}
+
 // A workgroup takes PASSES * 2048 / DIM tokens in a row of one head's keys or values: DIM / 8 lanes a token, eight values a
 // lane, four lanes a block of 32 that shares a scale. Tokens in a row mostly lie in a row in their page too, so the codes
 // leave (or come) as one piece, and the scale bytes, which lie token by token, meet in one L2. All of a lane's rows are in
@@ -257,7 +302,7 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
 // to set and 55 us to fetch, 4.8 and 6.2 TB/s; a copy of 2 GiB moves 4.9. Rows are read and written past the caches, which a
 // row is not read from again: without that, 81 and 90 us. With a lane for 8 values of any token in turn, and 64-bit divisions
 // for its place, 90 and 94 us.
-template <int DIM, int PASSES>
+template <int BITS, int DIM, int PASSES>
 struct RowPlace {
   static constexpr int kLanes = DIM / 8;
   static constexpr int kPasses = PASSES;
@@ -286,10 +331,11 @@ struct RowPlace {
       if (slot[p] < 0 || slot[p] >> a.v.log2_page >= a.v.pages) slot[p] = -1;
   }
   __device__ __forceinline__ int64_t token(int p) const { return token0 + p * (256 / kLanes); }
-  __device__ __forceinline__ uint32_t *codes(const RowsArgs &a, int p) const {
+  __device__ __forceinline__ Codes<BITS> *codes(const RowsArgs &a, int p) const {
     const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
-    return reinterpret_cast<uint32_t *>(a.v.cache + at * a.v.cache_stride +
-                                        (((int64_t{2} * head + which) << a.v.log2_page) + off) * (DIM / 2) + piece * 4);
+    return reinterpret_cast<Codes<BITS> *>(a.v.cache + at * a.v.cache_stride +
+                                           (((int64_t{2} * head + which) << a.v.log2_page) + off) * (DIM * BITS / 8) +
+                                           piece * BITS);
   }
   __device__ __forceinline__ uint8_t *scale(const RowsArgs &a, int p) const {
     const int64_t at = slot[p] >> a.v.log2_page, off = slot[p] & ((1 << a.v.log2_page) - 1);
@@ -298,9 +344,9 @@ struct RowPlace {
   }
 };
 
-template <typename T, int DIM, int PASSES>
+template <typename T, int BITS, int DIM, int PASSES>
 __global__ __launch_bounds__(256) void page_set_kernel(RowsArgs a) {
-  const RowPlace<DIM, PASSES> r(a);
+  const RowPlace<BITS, DIM, PASSES> r(a);
   constexpr int kPasses = PASSES;
   const T *src = r.which ? static_cast<const T *>(a.values) + r.head * a.value_head
                          : static_cast<const T *>(a.keys) + r.head * a.key_head;
@@ -318,26 +364,20 @@ __global__ __launch_bounds__(256) void page_set_kernel(RowsArgs a) {
     for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[p][j]) & 0x7fffffffu);
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 1)));
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 2)));
-    // The smallest power of two with most < 7 * 2^e: nothing is cut by more than half the step at its place (6 is
-    // the largest code, 7 the middle between it and the 8 that there is not).
     const bool broken = most >= 0x7f800000u;
-    const int e = max(static_cast<int>((most + 0x200000u) >> 23) - 2, 0);
-    const float s = scale_operand(static_cast<uint32_t>(e));
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][0], x[p][1], s, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][2], x[p][3], s, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][4], x[p][5], s, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[p][6], x[p][7], s, 3);
-    *r.codes(a, p) = broken ? 0u : codes;
+    const int e = power_of<BITS>(most);
+    const Codes<BITS> codes = encode8<BITS>(x[p], scale_operand(static_cast<uint32_t>(e)));
+    *r.codes(a, p) = broken ? Codes<BITS>{} : codes;
     if ((r.piece & 3) == 0) *r.scale(a, p) = static_cast<uint8_t>(broken ? 255 : e);
   }
 }
 
-template <typename T, int DIM, int PASSES>
+template <typename T, int BITS, int DIM, int PASSES>
 __global__ __launch_bounds__(256) void page_fetch_kernel(RowsArgs a) {
-  const RowPlace<DIM, PASSES> r(a);
+  const RowPlace<BITS, DIM, PASSES> r(a);
   constexpr int kPasses = PASSES;
-  uint32_t codes[kPasses], scale[kPasses];
+  Codes<BITS> codes[kPasses];
+  uint32_t scale[kPasses];
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     codes[p] = scale[p] = 0;
@@ -347,12 +387,8 @@ __global__ __launch_bounds__(256) void page_fetch_kernel(RowsArgs a) {
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     if (r.token(p) >= a.tokens) continue;
-    const float s = scale_operand(scale[p]);
-    const f32x2 y[4] = {decode2_f32<0>(codes[p], s), decode2_f32<1>(codes[p], s), decode2_f32<2>(codes[p], s),
-                        decode2_f32<3>(codes[p], s)};
     float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = y[j / 2][j % 2];
+    decode8<BITS>(codes[p], scale_operand(scale[p]), x);
     store8(dst + r.token(p) * a.key_token, x);
   }
 }
@@ -361,24 +397,24 @@ __global__ __launch_bounds__(256) void page_fetch_kernel(RowsArgs a) {
 // fetch, 8 heads of 128 in bfloat16, with 64 and with 16 tokens: 2,048 tokens (512 workgroups of 64) 4.3 / 4.2 and 4.1 / 4.1
 // us, 4,096 tokens 5.6 / 5.0 and 6.0 / 5.3 us, 16,384 tokens 17 / 12.7 and 21 / 12.5 us; 2 heads of 256, 8,192 tokens (512)
 // 7.0 / 5.4 and 6.1 / 5.2 us.
-template <typename T, int DIM>
+template <typename T, int BITS, int DIM>
 void launch_some_rows(const RowsArgs &a, bool set, hipStream_t s) {
   constexpr int kMany = DIM / 32, kOne = 2048 / DIM;  // passes for 64 tokens; tokens of one pass
   const int64_t tiles = 2 * a.v.kv_heads, many = (a.tokens + 63) / 64 * tiles, few = (a.tokens + kOne - 1) / kOne * tiles;
   const dim3 block(256);
   if (many >= 1024) {
     const dim3 grid(static_cast<unsigned>(many));
-    if (set) hipLaunchKernelGGL((page_set_kernel<T, DIM, kMany>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((page_fetch_kernel<T, DIM, kMany>), grid, block, 0, s, a);
+    if (set) hipLaunchKernelGGL((page_set_kernel<T, BITS, DIM, kMany>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((page_fetch_kernel<T, BITS, DIM, kMany>), grid, block, 0, s, a);
   } else {
     const dim3 grid(static_cast<unsigned>(few));
-    if (set) hipLaunchKernelGGL((page_set_kernel<T, DIM, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((page_fetch_kernel<T, DIM, 1>), grid, block, 0, s, a);
+    if (set) hipLaunchKernelGGL((page_set_kernel<T, BITS, DIM, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((page_fetch_kernel<T, BITS, DIM, 1>), grid, block, 0, s, a);
   }
 }
 
 // A launch has less than 2^32 threads; more rows are more launches.
-template <typename T, int DIM>
+template <typename T, int BITS, int DIM>
 void launch_rows(const RowsArgs &all, bool set, hipStream_t s) {
   const int64_t each = ((int64_t{1} << 24) - 1) / (2 * all.v.kv_heads) * 64;
   RowsArgs a = all;
@@ -387,24 +423,30 @@ void launch_rows(const RowsArgs &all, bool set, hipStream_t s) {
     a.slots = static_cast<const char *>(all.slots) + t0 * all.slot_bytes;
     a.keys = static_cast<const T *>(all.keys) + t0 * all.key_token;
     a.values = static_cast<const T *>(all.values) + t0 * all.value_token;
-    launch_some_rows<T, DIM>(a, set, s);
+    launch_some_rows<T, BITS, DIM>(a, set, s);
   }
 }
 
+template <typename T, int BITS>
+void launch_rows(const RowsArgs &a, int dim, bool set, hipStream_t s) {
+  if (dim == 64) launch_rows<T, BITS, 64>(a, set, s);
+  else if (dim == 128) launch_rows<T, BITS, 128>(a, set, s);
+  else launch_rows<T, BITS, 256>(a, set, s);
+}
+
 template <typename T>
-int launch_rows(const RowsArgs &a, int dim, bool set, hipStream_t s) {
-  if (dim == 64) launch_rows<T, 64>(a, set, s);
-  else if (dim == 128) launch_rows<T, 128>(a, set, s);
-  else launch_rows<T, 256>(a, set, s);
+int launch_rows(const RowsArgs &a, int bits, int dim, bool set, hipStream_t s) {
+  if (bits == 8) launch_rows<T, 8>(a, dim, set, s);
+  else launch_rows<T, 4>(a, dim, set, s);
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;
 }
 
-int rows_entry(const shmt_paged_cache *c, const void *slots, int slot_bytes, int64_t n, const void *keys,
+int rows_entry(const shmt_paged_cache *c, int bits, const void *slots, int slot_bytes, int64_t n, const void *keys,
                int64_t key_token, int64_t key_head, const void *values, int64_t value_token, int64_t value_head,
                int elem_type, bool set, hipStream_t s) {
   PagedView v;
-  const int rc = paged_view(c, &v);
+  const int rc = paged_view(c, bits, &v);
   if (rc != SHMT_OK) return rc;
   SHMT_REQUIRE(n >= 0, "the number of rows must be >= 0");
   SHMT_REQUIRE(width_ok(slot_bytes), "slots can only be int32 or int64");
@@ -414,13 +456,13 @@ int rows_entry(const shmt_paged_cache *c, const void *slots, int slot_bytes, int
   SHMT_REQUIRE(slots && keys && values, "slots, keys or values is null");
   SHMT_REQUIRE(n / 64 < (int64_t{1} << 30) / c->kv_heads, "too many rows in one call");
   const int64_t esize = elem_type == SHMT_F32 ? 4 : 2;
-  const int64_t bits = reinterpret_cast<int64_t>(keys) | reinterpret_cast<int64_t>(values) |
+  const int64_t low = reinterpret_cast<int64_t>(keys) | reinterpret_cast<int64_t>(values) |
                        (key_token | key_head | value_token | value_head) * esize;
-  SHMT_REQUIRE((bits & 15) == 0, "every row of keys and values has to begin on 16 bytes");
+  SHMT_REQUIRE((low & 15) == 0, "every row of keys and values has to begin on 16 bytes");
   const RowsArgs a{v, slots, slot_bytes, n, keys, values, key_token, key_head, value_token, value_head};
-  if (elem_type == SHMT_F32) return launch_rows<float>(a, c->dim, set, s);
-  if (elem_type == SHMT_F16) return launch_rows<_Float16>(a, c->dim, set, s);
-  return launch_rows<__bf16>(a, c->dim, set, s);
+  if (elem_type == SHMT_F32) return launch_rows<float>(a, bits, c->dim, set, s);
+  if (elem_type == SHMT_F16) return launch_rows<_Float16>(a, bits, c->dim, set, s);
+  return launch_rows<__bf16>(a, bits, c->dim, set, s);
 }
 
 }  // namespace shmt
@@ -474,18 +516,30 @@ int shmt_page_plan(const void *cached_lens, const void *new_lens, int len_bytes,
   return SHMT_OK;
 }
 
+int shmt_page_set_as(const shmt_paged_cache *cache, int bits, const void *slots, int slot_bytes, int64_t n, const void *keys,
+                     int64_t key_token_stride, int64_t key_head_stride, const void *values, int64_t value_token_stride,
+                     int64_t value_head_stride, int elem_type, void *stream) {
+  return rows_entry(cache, bits, slots, slot_bytes, n, keys, key_token_stride, key_head_stride, values, value_token_stride,
+                    value_head_stride, elem_type, true, as_stream(stream));
+}
+
+int shmt_page_fetch_as(const shmt_paged_cache *cache, int bits, const void *slots, int slot_bytes, int64_t n, void *keys,
+                       void *values, int elem_type, void *stream) {
+  const int64_t head = cache ? cache->dim : 0, token = cache ? int64_t{cache->kv_heads} * cache->dim : 0;
+  return rows_entry(cache, bits, slots, slot_bytes, n, keys, token, head, values, token, head, elem_type, false,
+                    as_stream(stream));
+}
+
 int shmt_page_set(const shmt_paged_cache *cache, const void *slots, int slot_bytes, int64_t n, const void *keys,
                   int64_t key_token_stride, int64_t key_head_stride, const void *values, int64_t value_token_stride,
                   int64_t value_head_stride, int elem_type, void *stream) {
-  return rows_entry(cache, slots, slot_bytes, n, keys, key_token_stride, key_head_stride, values, value_token_stride,
-                    value_head_stride, elem_type, true, as_stream(stream));
+  return shmt_page_set_as(cache, 4, slots, slot_bytes, n, keys, key_token_stride, key_head_stride, values,
+                          value_token_stride, value_head_stride, elem_type, stream);
 }
 
 int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots, int slot_bytes, int64_t n, void *keys,
                     void *values, int elem_type, void *stream) {
-  const int64_t head = cache ? cache->dim : 0, token = cache ? int64_t{cache->kv_heads} * cache->dim : 0;
-  return rows_entry(cache, slots, slot_bytes, n, keys, token, head, values, token, head, elem_type, false,
-                    as_stream(stream));
+  return shmt_page_fetch_as(cache, 4, slots, slot_bytes, n, keys, values, elem_type, stream);
 }
 
 }  // extern "C"

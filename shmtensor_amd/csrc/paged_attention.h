@@ -59,12 +59,6 @@ struct JoinRecord {
   int64_t first_row;  // the request's first row of `query`
 };
 
-struct Request {
-  int64_t first_row;  // of `query`
-  int32_t queries;
-  int32_t before;  // tokens in front of the first query; negative: the first rows see nothing
-};
-
 struct Span {
   int32_t sink_tiles;  // tiles 0 .. sink_tiles
   int32_t tile0;       // then tiles from here
@@ -85,16 +79,7 @@ __device__ __forceinline__ Span same(Span s) {
 }
 
 __device__ __forceinline__ Request attn_request(const AttnArgs &a, int64_t b) {
-  int64_t lo, hi;
-  load_int_pair(a.starts, b, a.len_bytes, &lo, &hi);
-  const int64_t len = load_int(a.kv_lens, b, a.len_bytes);
-  lo = min(max(lo, int64_t{0}), a.tokens);
-  hi = min(max(hi, lo), a.tokens);
-  Request r;
-  r.first_row = lo;
-  r.queries = static_cast<int32_t>(hi - lo);
-  r.before = static_cast<int32_t>(min(max(len, int64_t{0}), int64_t{0x7fffffff}) - (hi - lo));
-  return r;
+  return load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b);
 }
 
 template <int ROWS>

@@ -403,7 +403,7 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_
                         int64_t sinks, int64_t max_query_len, void *out, float *lse, void *scratch,
                         int64_t scratch_bytes, void *stream) {
   PagedView v;
-  const int rc = paged_view(cache, &v);
+  const int rc = paged_view(cache, 4, &v);
   if (rc != SHMT_OK) return rc;
   SHMT_REQUIRE(elem_type == SHMT_F16 || elem_type == SHMT_BF16, "queries can only be float16 or bfloat16");
   SHMT_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31), "the number of query rows must be in [0, 2^31)");

@@ -1,6 +1,6 @@
-// The paged key/value cache held in 4 bits, as operators of ShmTensorLib:
-// page_plan, page_set, page_fetch, page_attention (no counterpart in the
-// reference; what they compute is in include/shmt.h). Host C++ only: tensors
+// The paged key/value cache held in 4 or 8 bits, as operators of ShmTensorLib:
+// page_plan, page_set, page_fetch, page_attention, page_tree, page_keep (no
+// counterpart in the reference; what they compute is in include/shmt.h). Host C++ only: tensors
 // are checked here, outputs and scratch come from torch's caching allocator,
 // the work goes to torch's current stream and nothing waits for it.
 #include <ATen/hip/EmptyTensor.h>
@@ -36,43 +36,59 @@ void check_no_grad(const torch::Tensor &t, const char *name) {
               " requires a gradient, which the paged cache does not give: call it under torch.no_grad() or detach() first");
 }
 
-bool page_contiguous(const torch::Tensor &t) {
+// Whether the last four of five dimensions (from `from` on) are contiguous.
+bool page_contiguous(const torch::Tensor &t, int64_t from = 0) {
   int64_t want = 1;
-  for (int64_t d = 4; d >= 1; --d) {
+  for (int64_t d = from + 4; d > from; --d) {
     if (t.size(d) > 1 && t.stride(d) != want) return false;
     want *= t.size(d);
   }
   return true;
 }
 
-shmt_paged_cache describe(const torch::Tensor &cache, const torch::Tensor &scales) {
+// A cache, or `layers` of them side by side, and how many bits it holds a value in: uint8 is two codes of 4 bits, float8_e4m3fn is
+// codes of 8.
+struct Cache : shmt_paged_cache {
+  int bits;
+  int64_t layers, cache_layer, scales_layer;  // strides in bytes
+};
+
+Cache describe(const torch::Tensor &cache, const torch::Tensor &scales, bool with_layers = false) {
   TORCH_CHECK(cache.is_cuda(), "cache must be a CUDA tensor");
   TORCH_CHECK(cache.device().index() == c10::hip::current_device(), "cache is on ", cache.device(),
               ", which is not the current device");
   check_device(scales, cache, "scales");
-  TORCH_CHECK(cache.scalar_type() == torch::kUInt8 && scales.scalar_type() == torch::kUInt8,
-              "cache and scales must be uint8 tensors");
-  TORCH_CHECK(cache.dim() == 5 && cache.size(2) == 2, "cache must be [pages, kv_heads, 2, page, dim / 2], got ",
-              cache.sizes());
-  const int64_t pages = cache.size(0), heads = cache.size(1), page = cache.size(3), half = cache.size(4);
-  TORCH_CHECK(half == 32 || half == 64 || half == 128, "a row must have 64, 128 or 256 values, not ", half * 2);
-  TORCH_CHECK(scales.dim() == 5 && scales.size(0) == pages && scales.size(1) == heads && scales.size(2) == 2 &&
-                  scales.size(3) == half / 16 && scales.size(4) == page,
+  const bool eight = cache.scalar_type() == torch::kFloat8_e4m3fn;
+  TORCH_CHECK((eight || cache.scalar_type() == torch::kUInt8) && scales.scalar_type() == torch::kUInt8,
+              "cache and scales must be uint8 tensors, or the cache float8_e4m3fn");
+  const int64_t from = with_layers && cache.dim() == 6 ? 1 : 0;
+  TORCH_CHECK(cache.dim() == from + 5 && cache.size(from + 2) == 2, "cache must be [pages, kv_heads, 2, page, dim",
+              eight ? "" : " / 2", "], got ", cache.sizes());
+  const int64_t pages = cache.size(from), heads = cache.size(from + 1), page = cache.size(from + 3);
+  const int64_t dim = cache.size(from + 4) * (eight ? 1 : 2);
+  TORCH_CHECK(dim == 64 || dim == 128 || dim == 256, "a row must have 64, 128 or 256 values, not ", dim);
+  TORCH_CHECK(scales.dim() == from + 5 && (from == 0 || scales.size(0) == cache.size(0)) && scales.size(from) == pages &&
+                  scales.size(from + 1) == heads && scales.size(from + 2) == 2 && scales.size(from + 3) == dim / 32 &&
+                  scales.size(from + 4) == page,
               "scales must be [pages, kv_heads, 2, dim / 32, page] of the same cache, got ", scales.sizes(), " beside ",
               cache.sizes());
   TORCH_CHECK(page <= 256 && heads >= 1 && heads <= 65535, "a page must hold 16, 32, 64, 128 or 256 tokens of 1 to 65535 heads");
-  // within a page everything is contiguous; pages may lie apart
-  TORCH_CHECK(pages == 0 || (page_contiguous(cache) && page_contiguous(scales)),
+  // within a page everything is contiguous; pages and layers may lie apart
+  TORCH_CHECK(cache.numel() == 0 || (page_contiguous(cache, from) && page_contiguous(scales, from)),
               "the pages of cache and scales must be contiguous");
-  shmt_paged_cache c;
+  Cache c;
   c.cache = cache.data_ptr();
   c.scales = scales.data_ptr();
   c.pages = pages;
-  c.cache_page_stride = pages > 1 ? cache.stride(0) : 0;
-  c.scales_page_stride = pages > 1 ? scales.stride(0) : 0;
+  c.cache_page_stride = pages > 1 ? cache.stride(from) : 0;
+  c.scales_page_stride = pages > 1 ? scales.stride(from) : 0;
   c.kv_heads = static_cast<int>(heads);
-  c.dim = static_cast<int>(half * 2);
+  c.dim = static_cast<int>(dim);
   c.page = static_cast<int>(page);
+  c.bits = eight ? 8 : 4;
+  c.layers = from ? cache.size(0) : 1;
+  c.cache_layer = from && c.layers > 1 ? cache.stride(0) : 0;
+  c.scales_layer = from && c.layers > 1 ? scales.stride(0) : 0;
   return c;
 }
 
@@ -136,7 +152,7 @@ std::vector<torch::Tensor> page_plan(torch::Tensor cached_lens, torch::Tensor ne
 // Rows of keys and values rounded into their slots (shmt_page_set).
 void page_set(const torch::Tensor &cache, const torch::Tensor &scales, torch::Tensor slots, torch::Tensor keys,
               torch::Tensor values) {
-  const shmt_paged_cache c = describe(cache, scales);
+  const Cache c = describe(cache, scales);
   slots = cuda_ids(slots, "slots");
   check_device(slots, cache, "slots");
   check_device(keys, cache, "keys");
@@ -153,7 +169,7 @@ void page_set(const torch::Tensor &cache, const torch::Tensor &scales, torch::Te
   if (n == 0) return;
   keys = rows_on_16(keys);
   values = rows_on_16(values);
-  check(shmt_page_set(&c, slots.data_ptr(), static_cast<int>(slots.element_size()), n, keys.data_ptr(),
+  check(shmt_page_set_as(&c, c.bits, slots.data_ptr(), static_cast<int>(slots.element_size()), n, keys.data_ptr(),
                       stride_of(keys, 0), stride_of(keys, 1), values.data_ptr(), stride_of(values, 0),
                       stride_of(values, 1), type, current_stream()));
 }
@@ -161,13 +177,13 @@ void page_set(const torch::Tensor &cache, const torch::Tensor &scales, torch::Te
 // The values that the rows at `slots` stand for (shmt_page_fetch).
 std::vector<torch::Tensor> page_fetch(const torch::Tensor &cache, const torch::Tensor &scales, torch::Tensor slots,
                                       at::ScalarType dtype) {
-  const shmt_paged_cache c = describe(cache, scales);
+  const Cache c = describe(cache, scales);
   slots = cuda_ids(slots, "slots");
   check_device(slots, cache, "slots");
   const int type = elem_type(dtype, "dtype");
   torch::Tensor keys = new_tensor({slots.numel(), c.kv_heads, c.dim}, dtype, cache);
   torch::Tensor values = new_tensor({slots.numel(), c.kv_heads, c.dim}, dtype, cache);
-  check(shmt_page_fetch(&c, slots.data_ptr(), static_cast<int>(slots.element_size()), slots.numel(), keys.data_ptr(),
+  check(shmt_page_fetch_as(&c, c.bits, slots.data_ptr(), static_cast<int>(slots.element_size()), slots.numel(), keys.data_ptr(),
                         values.data_ptr(), type, current_stream()));
   return {keys, values};
 }
@@ -177,7 +193,8 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
                           const torch::Tensor &block_table, torch::Tensor query_starts, torch::Tensor kv_lens,
                           std::optional<double> softmax_scale, int64_t window, int64_t sinks, int64_t max_query_len,
                           bool return_lse) {
-  const shmt_paged_cache c = describe(cache, scales);
+  const Cache c = describe(cache, scales);
+  TORCH_CHECK(c.bits == 4, "attention reads a cache held in 4 bits only");
   check_device(query, cache, "query");
   check_no_grad(query, "query");
   check_device(block_table, cache, "block_table");
@@ -220,6 +237,75 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
   return py::cast(out);
 }
 
+// Lengths of a step over trees: one entry more than requests in query_starts, one integer type.
+int64_t check_lengths(const torch::Tensor &query_starts, const torch::Tensor &kv_lens) {
+  TORCH_CHECK(query_starts.scalar_type() == kv_lens.scalar_type(), "query_starts and kv_lens must have one type");
+  TORCH_CHECK(query_starts.dim() == 1 && kv_lens.dim() == 1 && query_starts.numel() == kv_lens.numel() + 1,
+              "query_starts must hold one entry more than kv_lens");
+  TORCH_CHECK(query_starts.device() == kv_lens.device(), "all tensors must be on one device");
+  return kv_lens.numel();
+}
+torch::Tensor check_nodes(const torch::Tensor &parents) {
+  TORCH_CHECK(parents.is_cuda(), "parents must be a CUDA tensor");
+  TORCH_CHECK(parents.scalar_type() == torch::kInt32 && parents.dim() == 1,
+              "parents must be a one-dimensional int32 tensor, got ", parents.scalar_type(), " ", parents.sizes());
+  TORCH_CHECK(parents.device().index() == c10::hip::current_device(), "parents is on ", parents.device(),
+              ", which is not the current device");
+  return parents.contiguous();
+}
+
+// A step's trees, numbered, and their nodes' positions (shmt_page_tree).
+std::vector<torch::Tensor> page_tree(torch::Tensor parents, torch::Tensor query_starts, torch::Tensor kv_lens) {
+  parents = check_nodes(parents);
+  query_starts = cuda_ids(query_starts, "query_starts");
+  kv_lens = cuda_ids(kv_lens, "kv_lens");
+  const int64_t n = check_lengths(query_starts, kv_lens), tokens = parents.numel();
+  TORCH_CHECK(query_starts.device() == parents.device(), "all tensors must be on one device");
+  TORCH_CHECK(tokens < (int64_t{1} << 31), "there must be less than 2^31 nodes");
+  torch::Tensor nodes = new_tensor({tokens, 4}, torch::kInt32, parents), positions = new_tensor({tokens}, torch::kInt32, parents);
+  check(shmt_page_tree(parents.data_ptr<int32_t>(), query_starts.data_ptr(), kv_lens.data_ptr(),
+                       static_cast<int>(kv_lens.element_size()), n, tokens, nodes.data_ptr<int32_t>(),
+                       positions.data_ptr<int32_t>(), current_stream()));
+  return {nodes, positions};
+}
+
+// The accepted paths of a step over trees, their rows moved together (shmt_page_keep).
+std::vector<torch::Tensor> page_keep(const torch::Tensor &cache, const torch::Tensor &scales, const torch::Tensor &block_table,
+                                     torch::Tensor query_starts, torch::Tensor kv_lens, torch::Tensor parents,
+                                     torch::Tensor tokens, torch::Tensor picked, std::optional<torch::Tensor> given) {
+  const Cache c = describe(cache, scales, true);
+  check_device(block_table, cache, "block_table");
+  const int64_t stride = table_stride(block_table);
+  query_starts = cuda_ids(query_starts, "query_starts");
+  kv_lens = cuda_ids(kv_lens, "kv_lens");
+  check_device(query_starts, cache, "query_starts");
+  const int64_t n = check_lengths(query_starts, kv_lens);
+  TORCH_CHECK(block_table.size(0) == n, "block_table has ", block_table.size(0), " requests, kv_lens ", n);
+  parents = check_nodes(parents);
+  tokens = cuda_ids(tokens, "tokens");
+  picked = cuda_ids(picked, "picked");
+  for (const auto &t : {parents, tokens, picked}) check_device(t, cache, "parents, tokens or picked");
+  const int64_t rows = parents.numel();
+  TORCH_CHECK(tokens.scalar_type() == picked.scalar_type(), "tokens and picked must have one type");
+  TORCH_CHECK(tokens.dim() == 1 && picked.dim() == 1 && tokens.numel() == rows && picked.numel() == rows,
+              "tokens and picked must hold an entry for each of ", rows, " nodes");
+  if (given) {
+    check_device(*given, cache, "given");
+    TORCH_CHECK(given->scalar_type() == torch::kInt32 && given->dim() == 1 && given->numel() == n,
+                "given must hold an int32 for each of ", n, " requests");
+    given = given->contiguous();
+  }
+  torch::Tensor counts = new_tensor({n}, torch::kInt32, cache), path = new_tensor({rows}, torch::kInt32, cache);
+  torch::Tensor next = new_tensor({n}, tokens.scalar_type(), cache);
+  check(shmt_page_keep(&c, c.bits, c.layers, c.cache_layer, c.scales_layer, block_table.data_ptr<int32_t>(),
+                       block_table.size(1), stride, query_starts.data_ptr(), kv_lens.data_ptr(),
+                       static_cast<int>(kv_lens.element_size()), n, rows, parents.data_ptr<int32_t>(), tokens.data_ptr(),
+                       picked.data_ptr(), static_cast<int>(tokens.element_size()),
+                       given ? given->data_ptr<int32_t>() : nullptr, counts.data_ptr<int32_t>(), path.data_ptr<int32_t>(),
+                       next.data_ptr(), current_stream()));
+  return {counts, path, next};
+}
+
 void register_paged_ops(py::module &m) {
   m.def("page_plan", &page_plan, py::arg("cached_lens"), py::arg("new_lens"), py::arg("block_table"),
         py::arg("free_pages"), py::arg("page"), py::arg("max_tokens"),
@@ -228,7 +314,8 @@ void register_paged_ops(py::module &m) {
         "without a page have slot -1.");
   m.def("page_set", &page_set, py::arg("cache"), py::arg("scales"), py::arg("slots"), py::arg("keys"),
         py::arg("values"),
-        "Rounds rows of keys and values [n, kv_heads, dim] to 4 bits and writes them to their slots (-1: nowhere).");
+        "Rounds rows of keys and values [n, kv_heads, dim] to the cache's 4 or 8 bits and writes them to their slots (-1: "
+        "nowhere).");
   m.def("page_fetch", &page_fetch, py::arg("cache"), py::arg("scales"), py::arg("slots"), py::arg("dtype"),
         "[keys, values]: what the rows at `slots` stand for, in `dtype`; 0 for slots outside the cache.");
   m.def("page_attention", &page_attention, py::arg("query"), py::arg("cache"), py::arg("scales"),
@@ -236,6 +323,14 @@ void register_paged_ops(py::module &m) {
         py::arg("window") = 0, py::arg("sinks") = 0, py::arg("max_query_len") = 0, py::arg("return_lse") = false,
         "Attention of each request's new tokens (the last of its kv_lens tokens) over what the cache holds for it, or "
         "over a window of it and the first `sinks` tokens. out [tokens, heads, dim], with return_lse (out, lse).");
+  m.def("page_tree", &page_tree, py::arg("parents"), py::arg("query_starts"), py::arg("kv_lens"),
+        "[nodes, positions] of a step whose new tokens are trees: parents[t] is the parent's index among its request's "
+        "nodes, or -1. `nodes` is for page_attention, positions = tokens in front + the node's depth.");
+  m.def("page_keep", &page_keep, py::arg("cache"), py::arg("scales"), py::arg("block_table"), py::arg("query_starts"),
+        py::arg("kv_lens"), py::arg("parents"), py::arg("tokens"), py::arg("picked"), py::arg("given") = py::none(),
+        "[counts, path, next]: of each request's tree the nodes along which `picked` (the model's choice behind each node) "
+        "agrees with `tokens`, their rows moved to the request's first new places in every layer of the cache ([layers, "
+        "pages, ...] or one layer's), and what was picked behind the last of them.");
 }
 
 }  // namespace shim
