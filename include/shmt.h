@@ -819,6 +819,38 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query,
                         int64_t max_query_len, void *out, float *lse,
                         void *scratch, int64_t scratch_bytes, void *stream);
 
+/* The same over a cache of `bits` = 4 or 8, with another rule of what a row
+ * sees:
+ *   SHMT_SEEN_CAUSAL  as above
+ *   SHMT_SEEN_TREE    the request's new tokens are trees, `nodes` what
+ *     shmt_page_tree made of them for the same starts and lengths. With c =
+ *     kv_lens[b] - queries, a row has position p = c + its node's depth and sees,
+ *     of the tokens j < c, those that shmt_page_attention lets it see, and of
+ *     the new ones its own and those of the nodes above it; with a window those
+ *     of them only whose position c + depth is > p - window or < sinks.
+ *   SHMT_SEEN_ALL     every row sees all kv_lens[b] tokens (an encoder's states,
+ *     which are as many as they are, however many rows look at them); no window.
+ * nodes: int32 [tokens][4] on 16 bytes, not read unless trees are asked for.
+ * scratch: shmt_page_attention_as_scratch_bytes(...) bytes.                  */
+#define SHMT_SEEN_CAUSAL 0
+#define SHMT_SEEN_TREE 1
+#define SHMT_SEEN_ALL 2
+int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads,
+                                             int kv_heads, int bits, int dim,
+                                             int elem_type, int64_t requests,
+                                             int64_t max_query_len);
+int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen,
+                           const int32_t *nodes, const void *query,
+                           int64_t query_token_stride,
+                           int64_t query_head_stride, int elem_type,
+                           int64_t tokens, int heads,
+                           const int32_t *block_table, int64_t width,
+                           int64_t table_stride, const void *query_starts,
+                           const void *kv_lens, int len_bytes, int64_t requests,
+                           float softmax_scale, int64_t window, int64_t sinks,
+                           int64_t max_query_len, void *out, float *lse,
+                           void *scratch, int64_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

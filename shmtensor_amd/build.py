@@ -21,7 +21,8 @@ ORACLE_DIR = os.path.join(ROOT, "oracle")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "liboracle.so")
 
 HIP_SOURCES = ["hashmap.hip", "fetch.hip", "scan.hip", "relabel.hip", "sample.hip", "misc.hip",
-               "paged.hip", "paged_tree.hip", "paged_attention.hip", "paged_attention_many.hip", "host_mem.hip", "errors.cc"]
+               "paged.hip", "paged_tree.hip", "paged_attention.hip", "paged_attention_few.hip", "paged_attention_many.hip",
+               "paged_attention_tree.hip", "paged_attention_8.hip", "paged_attention_8_tree.hip", "host_mem.hip", "errors.cc"]
 
 MODULE_SOURCES = ["module.cc", "batch_driver.cc", "batch_sampler.cc", "host_tensors.cc", "paged_ops.cc"]
 

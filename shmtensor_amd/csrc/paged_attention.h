@@ -1,5 +1,5 @@
-// What the two attention kernels over the paged 4-bit cache share: how the work is cut and numbered, how tokens are read and
-// decoded, the join of parts.
+// What the two attention kernels over the paged cache share: how the work is cut and numbered, how tokens are read and
+// decoded (BITS: 4 or 8 a value), what a row sees (TREE: its request's new tokens are trees), the join of parts.
 #pragma once
 #include "common.h"
 #include "paged_dev.h"
@@ -26,6 +26,8 @@ struct AttnArgs {
   int32_t limit;  // tokens that a row of the table has room for
   void *out;
   float *lse;
+  int32_t step;       // -1: a row's place moves on with its token; 0: all rows are at the last one (they see all)
+  const int4 *nodes;  // trees: number, size, depth and least depth of each row's node
 };
 
 // ---- items and units -------------------------------------------------------------
@@ -79,18 +81,39 @@ __device__ __forceinline__ Span same(Span s) {
 }
 
 __device__ __forceinline__ Request attn_request(const AttnArgs &a, int64_t b) {
-  return load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b);
+  Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b);
+  r.before += (r.queries - 1) & ~a.step;  // all rows at the last token
+  return r;
 }
 
-template <int ROWS>
+// The place that a row of the request's query `token` looks from. Of trees, the furthest that it may be.
+__device__ __forceinline__ int place_of(const AttnArgs &a, const Request &r, int token) { return r.before + (token & a.step); }
+
+// The last token that every row from `token` on sees, but for windows: trees, the last that was there before.
+template <bool TREE>
+__device__ __forceinline__ int seen_by_all(const AttnArgs &a, const Request &r, int token) {
+  return min(TREE ? r.before - 1 : place_of(a, r, token), a.limit - 1);
+}
+
+template <bool TREE, int ROWS>
 __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, int row0) {
   const int all = r.queries * a.group;
   const int t_first = static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group));
   const int t_last =
       static_cast<int>(static_cast<uint32_t>(min(row0 + ROWS, all) - 1) / static_cast<uint32_t>(a.group));
   Span s;
-  s.end = max(min(r.before + t_last + 1, a.limit), 0);
-  s.begin = a.window > 0 ? max(min(max(r.before + t_first, -1) - a.window + 1, s.end), 0) : 0;
+  s.end = max(min(place_of(a, r, t_last) + 1, a.limit), 0);
+  if constexpr (TREE) {
+    // A node's place is its depth's, which is at most its token's: what is behind the least place's window in tokens holds all
+    // that a window shows. First tokens may be nodes, too.
+    s.begin = 0;
+    if (a.window > 0) {
+      s.begin = max(min(max(r.before + a.nodes[r.first_row + t_first].w, -1) - a.window + 1, s.end), 0);
+      if (a.sinks > r.before) s.begin = min(s.begin, max(r.before, 0));
+    }
+  } else {
+    s.begin = a.window > 0 ? max(min(max(place_of(a, r, t_first), -1) - a.window + 1, s.end), 0) : 0;
+  }
   s.tile0 = s.begin / kUnit;
   s.sink_end = min(a.sinks, s.begin);
   s.sink_tiles = min((s.sink_end + kUnit - 1) / kUnit, s.tile0);
@@ -99,11 +122,11 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
 }
 
 // Units of a request for one head.
-template <int ROWS>
+template <bool TREE, int ROWS>
 __device__ __forceinline__ int64_t attn_units(const AttnArgs &a, const Request &r) {
   int64_t n = 0;
   const int all = r.queries * a.group;
-  for (int row0 = 0; row0 < all; row0 += ROWS) n += attn_span<ROWS>(a, r, row0).units;
+  for (int row0 = 0; row0 < all; row0 += ROWS) n += attn_span<TREE, ROWS>(a, r, row0).units;
   return n;
 }
 
@@ -163,12 +186,35 @@ __device__ __forceinline__ int page_at(const AttnArgs &a, const int32_t *table, 
   return p >= 0 && p < a.v.pages ? p : -1;
 }
 
-// What a row at place `pos` sees: tokens up to `last` that are behind `after`, or first ones.
+// What a row sees: tokens up to `last` that are behind `after`, or first ones; of trees, new tokens in `last`'s place whose node
+// is the row's own, `number`, or above it and whose place is behind `after` or among the first.
 struct Sees {
   int last, after;
+  int number;
 };
-__device__ __forceinline__ Sees row_sees(const AttnArgs &a, int pos) {
-  return {min(max(pos, -1), a.limit - 1), a.window > 0 && pos >= 0 ? pos - a.window : -1};
+template <bool TREE>
+__device__ __forceinline__ Sees row_sees(const AttnArgs &a, const Request &r, int token, bool there) {
+  if constexpr (TREE) {
+    if (!there) return {-1, 0x7fffffff, -1};
+    const int4 node = a.nodes[r.first_row + token];
+    const int64_t after = int64_t{r.before} + node.z - a.window;
+    return {min(r.before - 1, a.limit - 1), a.window > 0 ? static_cast<int>(max(after, int64_t{-0x7fffffff})) : -0x7fffffff, node.x};
+  } else {
+    const int pos = there ? place_of(a, r, token) : -1;
+    return {min(max(pos, -1), a.limit - 1), a.window > 0 && pos >= 0 ? pos - a.window : -1, 0};
+  }
+}
+// Whether a row whose node has this number is, or lies below, a node of these words.
+__device__ __forceinline__ bool is_above(const int4 &node, int number) {
+  return static_cast<uint32_t>(number - node.x) < static_cast<uint32_t>(node.y);
+}
+template <bool TREE>
+__device__ __forceinline__ bool sees_token(const AttnArgs &a, const Request &r, const Sees &s, int j, int sinks) {
+  if (j <= s.last) return j > s.after || j < sinks;
+  if (!TREE || j < r.before || j >= r.before + r.queries) return false;
+  const int4 node = a.nodes[r.first_row + (j - r.before)];
+  const int place = r.before + node.z;
+  return is_above(node, s.number) && (place > s.after || place < sinks);
 }
 
 // ---- arithmetic of a tile ------------------------------------------------------------
@@ -214,11 +260,11 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 
 // 32 tokens of one head as a wave holds them: lane (m, g) = (lane % 16, lane / 16) has, of the key of token m of each
 // 16, the quarter g; of the values of tokens 4g .. 4g + 3 of each 16, the sixteenth m.
-template <int DIM>
+template <int BITS, int DIM>
 struct KvTile {
-  static constexpr int kKeyWords = DIM / 32;                       // of 8 codes
+  static constexpr int kKeyWords = DIM * BITS / 128;  // of 8 codes, or 4
   static constexpr int kKeyScales = DIM / 128 > 0 ? DIM / 128 : 1;
-  static constexpr int kValueWords = DIM / 128 > 0 ? DIM / 128 : 1;  // at 64 dimensions: half a word
+  static constexpr int kValueWords = DIM * BITS / 512 > 0 ? DIM * BITS / 512 : 1;  // 4 bits and 64 dimensions: half a word
   uint32_t key[2][kKeyWords];
   uint32_t key_scale[2][kKeyScales];
   uint32_t value[2][4][kValueWords];
@@ -229,13 +275,13 @@ struct KvTile {
 struct LaneOffsets {
   uint32_t key, key_scale, value, value_scale;
 };
-template <int DIM>
+template <int BITS, int DIM>
 __device__ __forceinline__ LaneOffsets lane_offsets(int lane, int page) {
   const int m = lane & 15, g = lane >> 4;
   LaneOffsets o;
-  o.key = m * (DIM / 2) + g * (DIM / 8);
+  o.key = m * (DIM * BITS / 8) + g * (DIM * BITS / 32);
   o.key_scale = (DIM == 64 ? g >> 1 : g * (DIM / 128)) * page + m;
-  o.value = (page + 4 * g) * (DIM / 2) + m * (DIM / 32);
+  o.value = (page + 4 * g) * (DIM * BITS / 8) + m * (DIM * BITS / 128);
   o.value_scale = (DIM / 32 + m * (DIM / 16) / 32) * page + 4 * g;
   return o;
 }
@@ -257,43 +303,61 @@ struct Place16 {
   }
 };
 // Those of page `at` from the place of token j on.
-template <int DIM>
+template <int BITS, int DIM>
 __device__ __forceinline__ Place16 place16(const PagedView &v, int head, int at, int j) {
   const int off = j & ((1 << v.log2_page) - 1);
   const int64_t tile = int64_t{2} * head << v.log2_page;
-  const uint64_t row = reinterpret_cast<uint64_t>(v.cache + at * v.cache_stride + (tile + off) * (DIM / 2));
+  const uint64_t row = reinterpret_cast<uint64_t>(v.cache + at * v.cache_stride + (tile + off) * (DIM * BITS / 8));
   const uint64_t scale = reinterpret_cast<uint64_t>(v.scales + at * v.scales_stride + tile * (DIM / 32) + off);
   return {static_cast<uint32_t>(row), static_cast<uint32_t>(row >> 32), static_cast<uint32_t>(scale),
           static_cast<uint32_t>(scale >> 32)};
 }
 
-// Loads 16 tokens.
-template <int DIM>
-__device__ __forceinline__ void load_half(const Place16 &at, int page, const LaneOffsets &o, int half, KvTile<DIM> &t) {
-  const uint8_t *rows = at.row(), *sc = at.scale();
-  if constexpr (DIM == 64) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(rows + o.key);
-    t.key[half][0] = x.x, t.key[half][1] = x.y;
-    t.key_scale[half][0] = sc[o.key_scale];
+// W words in a row; half a word if there are none.
+template <int W>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *x) {
+  if constexpr (W == 0) {
+    x[0] = *reinterpret_cast<const uint16_t *>(p);
+  } else if constexpr (W == 1) {
+    x[0] = *reinterpret_cast<const uint32_t *>(p);
+  } else if constexpr (W == 2) {
+    const uint2 y = *reinterpret_cast<const uint2 *>(p);
+    x[0] = y.x, x[1] = y.y;
   } else {
 #pragma unroll
-    for (int i = 0; i < DIM / 128; ++i) {
-      const uint4 x = *reinterpret_cast<const uint4 *>(rows + o.key + 16 * i);
-      t.key[half][4 * i] = x.x, t.key[half][4 * i + 1] = x.y, t.key[half][4 * i + 2] = x.z, t.key[half][4 * i + 3] = x.w;
-      t.key_scale[half][i] = sc[o.key_scale + i * page];
+    for (int i = 0; i < W / 4; ++i) {
+      const uint4 y = *reinterpret_cast<const uint4 *>(p + 16 * i);
+      x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
     }
   }
+}
+
+// Loads 16 tokens.
+template <int BITS, int DIM>
+__device__ __forceinline__ void load_half(const Place16 &at, int page, const LaneOffsets &o, int half, KvTile<BITS, DIM> &t) {
+  const uint8_t *rows = at.row(), *sc = at.scale();
+  using Tile = KvTile<BITS, DIM>;
+  load_words<Tile::kKeyWords>(rows + o.key, t.key[half]);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const uint8_t *p = rows + o.value + r * (DIM / 2);
-    if constexpr (DIM == 64) t.value[half][r][0] = *reinterpret_cast<const uint16_t *>(p);
-    else if constexpr (DIM == 128) t.value[half][r][0] = *reinterpret_cast<const uint32_t *>(p);
-    else {
-      const uint2 x = *reinterpret_cast<const uint2 *>(p);
-      t.value[half][r][0] = x.x, t.value[half][r][1] = x.y;
-    }
-  }
+  for (int i = 0; i < Tile::kKeyScales; ++i) t.key_scale[half][i] = sc[o.key_scale + i * page];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) load_words<DIM * BITS / 512>(rows + o.value + r * (DIM * BITS / 8), t.value[half][r]);
   t.value_scale[half] = *reinterpret_cast<const uint32_t *>(sc + o.value_scale);
+}
+
+// Eight values from codes: a word of them in 4 bits, two in 8.
+template <int BITS>
+__device__ __forceinline__ u32x4 decode_fragment(const uint32_t *c, float f) {
+  if constexpr (BITS == 8)
+    return u32x4{decode2_bf16_8<0>(c[0], f), decode2_bf16_8<1>(c[0], f), decode2_bf16_8<0>(c[1], f), decode2_bf16_8<1>(c[1], f)};
+  else
+    return u32x4{decode2_bf16<0>(c[0], f), decode2_bf16<1>(c[0], f), decode2_bf16<2>(c[0], f), decode2_bf16<3>(c[0], f)};
+}
+// The I-th two values of a word.
+template <int BITS, int I>
+__device__ __forceinline__ uint32_t decode_two(uint32_t c, float f) {
+  if constexpr (BITS == 8) return decode2_bf16_8<I>(c, f);
+  else return decode2_bf16<I>(c, f);
 }
 
 // Softmax state and weighted values of NT x 16 rows: lane (n, g) has row n of each 16, and the dimensions
@@ -326,6 +390,9 @@ struct Sight {
   int after[NT];  // ... from behind here, or
   int sinks;      // before here
   int begin, end, sink_end;  // no row of the item sees any outside of [begin, end) and [0, sink_end)
+  int number[NT];            // trees: the rows' nodes,
+  int fresh;                 // the first token that is one,
+  const int4 *node;          // and what would be token 0's
 };
 
 // The weights of eight scores of a row, in units of `unit` powers of two, relative to its reference, as the right operand of
@@ -428,8 +495,9 @@ __device__ __forceinline__ void raise_reference(State &st, Flag &again, Flag &fa
   if (__ballot(is_far)) far = 1;
 }
 
-// Scale bytes from here on make values that are infinite in bfloat16, or not a number.
-constexpr uint32_t kWild = 253;
+// Scale bytes from here on make values that are infinite in bfloat16, or not a number: 6 * 2^126, 256 * 2^120.
+template <int BITS>
+constexpr uint32_t kWild = BITS == 8 ? 247 : 253;
 
 // One wave's step over 32 tokens.
 //   S^T = K Q^T, 16 tokens x 16 rows at a time: lane (n, g) gets the scores of row n with tokens 4g .. 4g + 3, which is
@@ -444,8 +512,8 @@ constexpr uint32_t kWild = 253;
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
 // FIRST: `pass` is kFirst or kRaised; rows may be `waiting` for a reference. `again` is set if the wave has to begin its tokens
 // again, `far` if with rounded scores.
-template <bool FIRST, int DIM, int NT, int PARTS>
-__device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
+template <bool FIRST, int BITS, bool TREE, int DIM, int NT, int PARTS>
+__device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int pass, int lane, bool whole, int token0, bool there0,
                                             bool there1, const Sight<NT> &sight, bool &wild, bool &waiting, bool &again,
                                             bool &far) {
@@ -459,8 +527,7 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const float f = scale_operand(t.key_scale[half][i / 4]);
-      const uint32_t c = t.key[half][i];
-      k[half] = u32x4{decode2_bf16<0>(c, f), decode2_bf16<1>(c, f), decode2_bf16<2>(c, f), decode2_bf16<3>(c, f)};
+      k[half] = decode_fragment<BITS>(&t.key[half][i * BITS / 4], f);
     }
     if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -474,22 +541,48 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
   }
   if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
   if (!whole) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+    if (TREE && token0 + kWaveTokens > sight.fresh) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
-        const bool sees = (j < 4 ? there0 : there1) && token <= sight.last[n] &&
-                          (token > sight.after[n] || token < sight.sinks);
-        s[n][j / 4][j % 4] = sees ? s[n][j / 4][j % 4] : kNothing;
+        const bool there = j < 4 ? there0 : there1;
+        int4 node = make_int4(0, 0, 0, 0);  // nobody is below it
+        if (token >= sight.fresh && token < sight.end) node = sight.node[token];
+        const int place = sight.fresh + node.z;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bool old = token <= sight.last[n] && (token > sight.after[n] || token < sight.sinks);
+          const bool own = is_above(node, sight.number[n]) && (place > sight.after[n] || place < sight.sinks);
+          s[n][j / 4][j % 4] = there && (old || own) ? s[n][j / 4][j % 4] : kNothing;
+        }
       }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
+          const bool sees = (j < 4 ? there0 : there1) && token <= sight.last[n] &&
+                            (token > sight.after[n] || token < sight.sinks);
+          s[n][j / 4][j % 4] = sees ? s[n][j / 4][j % 4] : kNothing;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if ((t.value_scale[j / 4] >> (8 * (j % 4)) & 255u) >= kWild) {
+      if ((t.value_scale[j / 4] >> (8 * (j % 4)) & 255u) >= kWild<BITS>) {
         const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
         t.value_scale[j / 4] &= ~(255u << (8 * (j % 4)));
         wild |= (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
       }
+    if constexpr (BITS == 8) {  // two codes of 8 bits are not numbers: where nobody looks they may stand, and must not meet a 0
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
+        const bool seen = (j < 4 ? there0 : there1) && token < sight.end && (token >= sight.begin || token < sight.sink_end);
+#pragma unroll
+        for (int i = 0; i < KvTile<BITS, DIM>::kValueWords; ++i) t.value[j / 4][j % 4][i] = seen ? t.value[j / 4][j % 4][i] : 0;
+      }
+    }
   }
   if constexpr (!FIRST) round_scores<NT>(s, scale2, st, pass);
   else if (waiting) waiting = first_reference<NT>(s, scale2, st, again, far);
@@ -503,30 +596,31 @@ __device__ __forceinline__ void attend_tile(KvTile<DIM> &t, const Queries<DIM, N
   for (int j = 0; j < 8; ++j)
     f[j] = __uint_as_float(j % 4 == 3 ? t.value_scale[j / 4] >> 1 : t.value_scale[j / 4] << (23 - 8 * (j % 4)));
 #pragma unroll
-  for (int word = 0; word < KvTile<DIM>::kValueWords; ++word) {
-    auto two = [&](auto byte) {  // dimensions 2 B and 2 B + 1 of this lane's
+  for (int word = 0; word < KvTile<BITS, DIM>::kValueWords; ++word) {
+    auto two = [&](auto pair) {  // dimensions 2 I and 2 I + 1 of this lane's in the word
       if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
-      constexpr int B = decltype(byte)::value;
+      constexpr int I = decltype(pair)::value;
       uint32_t x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = decode2_bf16<B>(t.value[j / 4][j % 4][word], f[j]);
+      for (int j = 0; j < 8; ++j) x[j] = decode_two<BITS, I>(t.value[j / 4][j % 4][word], f[j]);
       u32x4 lo, hi;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         lo[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
         hi[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
       }
+      const int at = 32 / BITS * word + 2 * I;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          st.acc[n][8 * word + 2 * B] = mfma(lo, w[p][n], st.acc[n][8 * word + 2 * B]);
-          st.acc[n][8 * word + 2 * B + 1] = mfma(hi, w[p][n], st.acc[n][8 * word + 2 * B + 1]);
+          st.acc[n][at] = mfma(lo, w[p][n], st.acc[n][at]);
+          st.acc[n][at + 1] = mfma(hi, w[p][n], st.acc[n][at + 1]);
         }
     };
     two(std::integral_constant<int, 0>{});
     two(std::integral_constant<int, 1>{});
-    if constexpr (DIM > 64) {
+    if constexpr (BITS == 4 && DIM > 64) {
       two(std::integral_constant<int, 2>{});
       two(std::integral_constant<int, 3>{});
     }
@@ -552,44 +646,54 @@ __device__ __forceinline__ void query_fragment(const T *src, bool there, uint32_
   }
 }
 
+// The two values from dimension d on, of a row's codes.
+template <int BITS>
+__device__ __forceinline__ f32x2 decode_at(const uint8_t *codes, int d, float f) {
+  if constexpr (BITS == 8) return decode2_f32_8<0>(*reinterpret_cast<const uint16_t *>(codes + d), f);
+  else return decode2_f32<0>(codes[d / 2], f);
+}
+
 // q . K[j] of one row and token, element by element.
-template <typename T, int DIM>
+template <typename T, int BITS, int DIM>
 __device__ float score_of(const T *q, const uint8_t *codes, const uint8_t *scales, int page) {
   float s = 0;
 #pragma unroll 1
   for (int p = 0; p < DIM / 8; ++p) {
-    const uint32_t c = reinterpret_cast<const uint32_t *>(codes)[p];
     const float f = scale_operand(scales[p / 4 * page]);
-    const f32x2 x[4] = {decode2_f32<0>(c, f), decode2_f32<1>(c, f), decode2_f32<2>(c, f), decode2_f32<3>(c, f)};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += static_cast<float>(q[8 * p + i]) * x[i / 2][i % 2];
+    for (int i = 0; i < 8; i += 2) {
+      const f32x2 x = decode_at<BITS>(codes, 8 * p + i, f);
+      s += static_cast<float>(q[8 * p + i]) * x[0];
+      s += static_cast<float>(q[8 * p + i + 1]) * x[1];
+    }
   }
   return s;
 }
 
 // Adds, for one row and DIM / 16 of its dimensions from d0 on, the values of the 16 tokens from j0 on (page `at`) that the
 // products left out: those that are not finite in bfloat16 and that the row sees.
-template <typename T, int DIM>
-__device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at, int j0, const T *q_row, const Sees &sees,
-                                             float scale2, float base, int d0, f32x4 (&o)[DIM / 64]) {
+template <typename T, int BITS, bool TREE, int DIM>
+__device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at, int j0, const T *q_row, const Request &req,
+                                             const Sees &sees, float scale2, float base, int d0, f32x4 (&o)[DIM / 64]) {
 #pragma clang fp contract(off)
   if (at < 0) return;
+  constexpr int kRow = DIM * BITS / 8;
   const int page = 1 << a.v.log2_page, off = j0 & (page - 1);
   const int64_t tile = int64_t{2} * head << a.v.log2_page;
-  const uint8_t *codes = a.v.cache + at * a.v.cache_stride + (tile + off) * (DIM / 2);
+  const uint8_t *codes = a.v.cache + at * a.v.cache_stride + (tile + off) * kRow;
   const uint8_t *sc = a.v.scales + at * a.v.scales_stride + tile * (DIM / 32) + off;
   const int sinks = a.window > 0 ? a.sinks : 0;
 #pragma unroll 1
   for (int i = 0; i < 16; ++i) {
     const int j = j0 + i;
     const uint32_t byte = sc[(DIM / 32 + d0 / 32) * page + i];
-    if (byte < kWild || j > sees.last || (j <= sees.after && j >= sinks)) continue;
-    const float x = score_of<T, DIM>(q_row, codes + i * (DIM / 2), sc + i, page);
+    if (byte < kWild<BITS> || !sees_token<TREE>(a, req, sees, j, sinks)) continue;
+    const float x = score_of<T, BITS, DIM>(q_row, codes + i * kRow, sc + i, page);
     const float e = __builtin_amdgcn_exp2f((a.scale < 0 ? -x : x) * scale2 - base);  // scores rounded, as in kRounded
-    const uint8_t *v = codes + (page + i) * (DIM / 2) + d0 / 2;
+    const uint8_t *v = codes + (page + i) * kRow;
 #pragma unroll
     for (int d = 0; d < DIM / 16; d += 2) {
-      const f32x2 y = decode2_f32<0>(v[d / 2], scale_operand(byte));
+      const f32x2 y = decode_at<BITS>(v, d0 + d, scale_operand(byte));
       o[d / 4][d % 4] += e * y[0];
       o[d / 4][d % 4 + 1] += e * y[1];
     }
@@ -713,8 +817,15 @@ struct AttnShape {
 
 constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
-// paged_attention_many.hip
+// Waves per SIMD that the registers of the kernel for few rows are meant for.
+constexpr int attn_waves(int bits, int dim, int tiles) { return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2; }
+
+// paged_attention_few.h, paged_attention_many.h
+template <int BITS, bool TREE>
+void launch_attention_few(const AttnArgs &a, int dim, int elem_type, int rows, unsigned groups, const AttnScratch &s,
+                          hipStream_t stream);
+template <int BITS, bool TREE>
 void launch_attention_many(const AttnArgs &a, int dim, int elem_type, unsigned groups, const AttnScratch &s, hipStream_t stream);
-int attn_many_groups();
+constexpr int attn_many_groups() { return 256; }
 
 }  // namespace shmt

@@ -1,0 +1,8 @@
+// Attention over the paged cache in 4 bits: few rows a request.
+#include "paged_attention_few.h"
+
+namespace shmt {
+
+template void launch_attention_few<4, false>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &, hipStream_t);
+
+}  // namespace shmt

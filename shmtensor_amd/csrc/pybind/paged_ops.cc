@@ -188,13 +188,12 @@ std::vector<torch::Tensor> page_fetch(const torch::Tensor &cache, const torch::T
   return {keys, values};
 }
 
-// Attention of the requests' new tokens over the cache (shmt_page_attention).
+// Attention of the requests' new tokens over the cache (shmt_page_attention_as).
 py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const torch::Tensor &scales,
                           const torch::Tensor &block_table, torch::Tensor query_starts, torch::Tensor kv_lens,
                           std::optional<double> softmax_scale, int64_t window, int64_t sinks, int64_t max_query_len,
-                          bool return_lse) {
+                          bool return_lse, std::optional<torch::Tensor> tree, bool causal) {
   const Cache c = describe(cache, scales);
-  TORCH_CHECK(c.bits == 4, "attention reads a cache held in 4 bits only");
   check_device(query, cache, "query");
   check_no_grad(query, "query");
   check_device(block_table, cache, "block_table");
@@ -214,24 +213,35 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
   TORCH_CHECK(query_starts.dim() == 1 && query_starts.numel() == n + 1 && kv_lens.dim() == 1 && kv_lens.numel() == n,
               "block_table has ", n, " requests: query_starts must hold one entry more, kv_lens as many");
   TORCH_CHECK(window >= 0 && sinks >= 0 && max_query_len >= 0, "window, sinks and max_query_len must be >= 0");
+  TORCH_CHECK(causal || window == 0, "without causal every row sees all: there is no window");
+  if (tree) {
+    TORCH_CHECK(causal, "a tree says what a row sees: it does not go with causal = False");
+    check_device(*tree, cache, "tree");
+    TORCH_CHECK(tree->scalar_type() == torch::kInt32 && tree->dim() == 2 && tree->size(0) == tokens && tree->size(1) == 4,
+                "tree must be the int32 [", tokens, ", 4] that page_tree makes, got ", tree->scalar_type(), " ", tree->sizes());
+    tree = tree->contiguous();
+    if (reinterpret_cast<intptr_t>(tree->data_ptr()) & 15) tree = tree->clone();
+  }
   torch::Tensor out = new_tensor({tokens, heads, c.dim}, query.scalar_type(), query);
   torch::Tensor lse;
   if (return_lse) lse = new_tensor({tokens, heads}, torch::kFloat32, query);
   if (tokens > 0) {
     query = rows_on_16(query);
-    const int64_t scratch_bytes = shmt_page_attention_scratch_bytes(tokens, static_cast<int>(heads), c.kv_heads, c.dim,
-                                                                    elem_type(query.scalar_type(), "query"), n,
-                                                                    max_query_len);
+    const int64_t scratch_bytes = shmt_page_attention_as_scratch_bytes(tokens, static_cast<int>(heads), c.kv_heads, c.bits,
+                                                                       c.dim, elem_type(query.scalar_type(), "query"), n,
+                                                                       max_query_len);
     TORCH_CHECK(scratch_bytes >= 0, shmt_last_error());
     torch::Tensor scratch = new_tensor({scratch_bytes}, torch::kUInt8, cache);
     const float scale = softmax_scale ? static_cast<float>(*softmax_scale)
                                       : 1.0f / std::sqrt(static_cast<float>(c.dim));
-    check(shmt_page_attention(&c, query.data_ptr(), stride_of(query, 0), stride_of(query, 1),
-                              elem_type(query.scalar_type(), "query"), tokens, static_cast<int>(heads),
-                              block_table.data_ptr<int32_t>(), block_table.size(1), stride, query_starts.data_ptr(),
-                              kv_lens.data_ptr(), static_cast<int>(kv_lens.element_size()), n, scale, window, sinks,
-                              max_query_len, out.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
-                              scratch.data_ptr(), scratch_bytes, current_stream()));
+    check(shmt_page_attention_as(&c, c.bits, tree ? SHMT_SEEN_TREE : causal ? SHMT_SEEN_CAUSAL : SHMT_SEEN_ALL,
+                                 tree ? tree->data_ptr<int32_t>() : nullptr, query.data_ptr(), stride_of(query, 0),
+                                 stride_of(query, 1), elem_type(query.scalar_type(), "query"), tokens,
+                                 static_cast<int>(heads), block_table.data_ptr<int32_t>(), block_table.size(1), stride,
+                                 query_starts.data_ptr(), kv_lens.data_ptr(), static_cast<int>(kv_lens.element_size()), n,
+                                 scale, window, sinks, max_query_len, out.data_ptr(),
+                                 return_lse ? lse.data_ptr<float>() : nullptr, scratch.data_ptr(), scratch_bytes,
+                                 current_stream()));
   }
   if (return_lse) return py::make_tuple(out, lse);
   return py::cast(out);
@@ -321,8 +331,11 @@ void register_paged_ops(py::module &m) {
   m.def("page_attention", &page_attention, py::arg("query"), py::arg("cache"), py::arg("scales"),
         py::arg("block_table"), py::arg("query_starts"), py::arg("kv_lens"), py::arg("softmax_scale") = py::none(),
         py::arg("window") = 0, py::arg("sinks") = 0, py::arg("max_query_len") = 0, py::arg("return_lse") = false,
+        py::arg("tree") = py::none(), py::arg("causal") = true,
         "Attention of each request's new tokens (the last of its kv_lens tokens) over what the cache holds for it, or "
-        "over a window of it and the first `sinks` tokens. out [tokens, heads, dim], with return_lse (out, lse).");
+        "over a window of it and the first `sinks` tokens. With `tree` (the nodes of page_tree) the new tokens see what was "
+        "there before them, themselves and the nodes above them; with causal = False every row sees all kv_lens tokens, as "
+        "those of a decoder see an encoder's states. out [tokens, heads, dim], with return_lse (out, lse).");
   m.def("page_tree", &page_tree, py::arg("parents"), py::arg("query_starts"), py::arg("kv_lens"),
         "[nodes, positions] of a step whose new tokens are trees: parents[t] is the parent's index among its request's "
         "nodes, or -1. `nodes` is for page_attention, positions = tokens in front + the node's depth.");
