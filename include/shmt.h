@@ -836,8 +836,9 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query,
 #define SHMT_SEEN_TREE 1
 #define SHMT_SEEN_ALL 2
 int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads,
-                                             int kv_heads, int bits, int dim,
-                                             int elem_type, int64_t requests,
+                                             int kv_heads, int bits, int seen,
+                                             int dim, int elem_type,
+                                             int64_t requests,
                                              int64_t max_query_len);
 int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen,
                            const int32_t *nodes, const void *query,

@@ -93,7 +93,7 @@ SIGNATURES = {
     "shmt_page_tree": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _vp, _vp]),
     "shmt_page_keep": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _int, _i64, _i64, _vp, _vp, _vp,
                               _int, _vp, _vp, _vp, _vp, _vp]),
-    "shmt_page_attention_as_scratch_bytes": (_i64, [_i64, _int, _int, _int, _int, _int, _i64, _i64]),
+    "shmt_page_attention_as_scratch_bytes": (_i64, [_i64, _int, _int, _int, _int, _int, _int, _i64, _i64]),
     "shmt_page_attention_as": (_int, [_vp, _int, _int, _vp, _vp, _i64, _i64, _int, _i64, _int, _vp, _i64, _i64, _vp, _vp,
                                       _int, _i64, _c.c_float, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "shmt_page_attention_scratch_bytes": (_i64, [_i64, _int, _int, _int, _int, _i64, _i64]),

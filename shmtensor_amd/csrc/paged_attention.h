@@ -332,17 +332,21 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *x) {
   }
 }
 
-// Loads 16 tokens.
+// Loads 16 tokens' keys, and values.
 template <int BITS, int DIM>
-__device__ __forceinline__ void load_half(const Place16 &at, int page, const LaneOffsets &o, int half, KvTile<BITS, DIM> &t) {
-  const uint8_t *rows = at.row(), *sc = at.scale();
+__device__ __forceinline__ void load_keys(const Place16 &at, int page, const LaneOffsets &o, int half, KvTile<BITS, DIM> &t) {
   using Tile = KvTile<BITS, DIM>;
-  load_words<Tile::kKeyWords>(rows + o.key, t.key[half]);
+  load_words<Tile::kKeyWords>(at.row() + o.key, t.key[half]);
+  const uint8_t *sc = at.scale() + o.key_scale;
 #pragma unroll
-  for (int i = 0; i < Tile::kKeyScales; ++i) t.key_scale[half][i] = sc[o.key_scale + i * page];
+  for (int i = 0; i < Tile::kKeyScales; ++i) t.key_scale[half][i] = sc[i * page];
+}
+template <int BITS, int DIM>
+__device__ __forceinline__ void load_values(const Place16 &at, const LaneOffsets &o, int half, KvTile<BITS, DIM> &t) {
+  const uint8_t *rows = at.row() + o.value;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) load_words<DIM * BITS / 512>(rows + o.value + r * (DIM * BITS / 8), t.value[half][r]);
-  t.value_scale[half] = *reinterpret_cast<const uint32_t *>(sc + o.value_scale);
+  for (int r = 0; r < 4; ++r) load_words<DIM * BITS / 512>(rows + r * (DIM * BITS / 8), t.value[half][r]);
+  t.value_scale[half] = *reinterpret_cast<const uint32_t *>(at.scale() + o.value_scale);
 }
 
 // Eight values from codes: a word of them in 4 bits, two in 8.
@@ -512,11 +516,12 @@ constexpr uint32_t kWild = BITS == 8 ? 247 : 253;
 // weight 0 of a row that does not see them: they are left out (`wild` says so) and added at the end of the item.
 // FIRST: `pass` is kFirst or kRaised; rows may be `waiting` for a reference. `again` is set if the wave has to begin its tokens
 // again, `far` if with rounded scores.
-template <bool FIRST, int BITS, bool TREE, int DIM, int NT, int PARTS>
+// `keys_done` and `values_done` are called when the tile's keys and values are not needed any more.
+template <bool FIRST, int BITS, bool TREE, int DIM, int NT, int PARTS, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int pass, int lane, bool whole, int token0, bool there0,
                                             bool there1, const Sight<NT> &sight, bool &wild, bool &waiting, bool &again,
-                                            bool &far) {
+                                            bool &far, KeysDone keys_done, ValuesDone values_done) {
   const int g = lane >> 4;
   f32x4 s[NT][2];
 #pragma unroll
@@ -540,6 +545,7 @@ __device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<
       }
   }
   if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
+  keys_done();
   if (!whole) {
     if (TREE && token0 + kWaveTokens > sight.fresh) {
 #pragma unroll
@@ -625,6 +631,7 @@ __device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<
       two(std::integral_constant<int, 3>{});
     }
   }
+  values_done();
 }
 
 // Eight values of a query row as a fragment: bfloat16 as they are, float16 as the sum of two. What is not a row is 0: its
@@ -817,8 +824,15 @@ struct AttnShape {
 
 constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
-// Waves per SIMD that the registers of the kernel for few rows are meant for.
-constexpr int attn_waves(int bits, int dim, int tiles) { return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2; }
+// Waves per SIMD that the registers of the kernel for few rows are meant for. Trees and 8 bits take more registers, and fewer waves
+// that spill none are quicker. us with one wave more a SIMD and as it is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in
+// 4 bits, 64 dimensions bfloat16 36 and 30, 128 dimensions 40 and 35, float16 46 and 36; in 8 bits, 64 dimensions float16 43 and
+// 34, 128 dimensions 66 and 54, 256 dimensions 141 and 114 (bfloat16 115 with one wave, 119 with two, but 59 and 57 where
+// requests are short); 32 rows of 256 dimensions 144 and 116.
+constexpr int attn_waves(int bits, bool tree, bool f16, int dim, int tiles) {
+  if (bits == 8 || tree) return dim == 256 ? (tiles == 1 && !f16 ? 2 : 1) : tiles * dim <= 64 ? 3 : 2;
+  return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2;
+}
 
 // paged_attention_few.h, paged_attention_many.h
 template <int BITS, bool TREE>

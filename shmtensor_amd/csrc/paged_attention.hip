@@ -8,7 +8,7 @@ namespace shmt {
 
 // ---- launch ------------------------------------------------------------------------
 
-inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, int dim, int elem_type, int64_t requests,
+inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, int seen, int dim, int elem_type, int64_t requests,
                             int64_t max_query_len) {
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
   const int64_t group = heads / kv_heads, rows = longest * group;
@@ -21,11 +21,21 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   //   256 dimensions: 64 rows 179 and 185, 96 rows 293 and 191; float16 64 rows 193 and 277, 96 rows 312 and 282.
   // So an item costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the card idles
   // behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
-  const int64_t few_items = (rows + 31) / 32, many_items = (rows + many_rows(dim) - 1) / many_rows(dim);
-  const int64_t worth = dim == 256 ? 2 : elem_type == SHMT_F16 ? 6 : 4;
-  s.many = rows > 2 * many_rows(dim) || (few_items > worth * many_items && tokens * group * kv_heads >= 16384);
+  // Chains in 4 bits keep that rule, and with it their results. Otherwise a last item of half the rows or fewer is told apart: the
+  // waves that have none of them only decode. Trees, as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and
+  // 119, 128 rows 129 and 121, 160 rows 169 and 146; 8 bits, 64 rows 87 and 122, 96 rows 137 and 124; float16: 4 bits, 128 rows 141
+  // and 164, 192 rows 216 and 224, 224 rows 251 and 228, 320 rows 344 and 409; 64 dimensions, bfloat16: 96 rows 91 and 90, 128 rows
+  // 104 and 90; 256 dimensions, bfloat16: 64 rows 155 and 157, in 8 bits 175 and 167, 96 rows 240 and 203; float16: 64 rows 187 and
+  // 232, 96 rows 289 and 280, in 8 bits 96 rows 357 and 363, 128 rows 402 and 374.
+  const bool f16 = elem_type == SHMT_F16;
+  const int64_t few_items = (rows + 31) / 32, whole = rows / many_rows(dim), rest = rows % many_rows(dim);
+  const int64_t worth = dim == 256 ? 2 + (f16 && bits == 8) : f16 ? 6 : 4;
+  int64_t last = rest > 0 ? worth : 0;  // what the last item is worth
+  if (rest > 0 && rest <= many_rows(dim) / 2 && (bits == 8 || seen != SHMT_SEEN_CAUSAL))
+    last = dim == 256 ? 1 + f16 : f16 ? 4 : bits == 8 && dim == 128 ? 2 : 3;
+  s.many = rows > 2 * many_rows(dim) || (few_items > worth * whole + last && tokens * group * kv_heads >= 16384);
   s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;
-  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(bits, dim, s.rows / 16);
+  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(bits, seen == SHMT_SEEN_TREE, f16, dim, s.rows / 16);
   s.items = s.many ? tokens * group / s.rows + requests : 0;
   const int64_t lines = 2 * s.groups * s.rows;
   s.parts_bytes = lines * dim * 4;
@@ -69,19 +79,19 @@ using namespace shmt;
 
 extern "C" {
 
-int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads, int kv_heads, int bits, int dim, int elem_type,
+int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads, int kv_heads, int bits, int seen, int dim, int elem_type,
                                              int64_t requests, int64_t max_query_len) {
-  if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (bits != 4 && bits != 8) || (dim != 64 && dim != 128 && dim != 256) ||
+  if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (bits != 4 && bits != 8) || seen < SHMT_SEEN_CAUSAL || seen > SHMT_SEEN_ALL || (dim != 64 && dim != 128 && dim != 256) ||
       (elem_type != SHMT_F16 && elem_type != SHMT_BF16) || requests < 0 || max_query_len < 0) {
     set_error("bad arguments for the attention's scratch size");
     return -1;
   }
-  return attn_shape(tokens, heads, kv_heads, bits, dim, elem_type, requests, max_query_len).bytes();
+  return attn_shape(tokens, heads, kv_heads, bits, seen, dim, elem_type, requests, max_query_len).bytes();
 }
 
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads, int kv_heads, int dim, int elem_type,
                                           int64_t requests, int64_t max_query_len) {
-  return shmt_page_attention_as_scratch_bytes(tokens, heads, kv_heads, 4, dim, elem_type, requests, max_query_len);
+  return shmt_page_attention_as_scratch_bytes(tokens, heads, kv_heads, 4, SHMT_SEEN_CAUSAL, dim, elem_type, requests, max_query_len);
 }
 
 int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_t query_token_stride,
@@ -127,7 +137,7 @@ int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen, co
   SHMT_REQUIRE((reinterpret_cast<int64_t>(out) & 15) == 0, "out has to begin on 16 bytes");
   SHMT_REQUIRE(seen != SHMT_SEEN_TREE || (nodes && (reinterpret_cast<int64_t>(nodes) & 15) == 0),
                "nodes is null or does not begin on 16 bytes");
-  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, bits, cache->dim, elem_type, requests, max_query_len);
+  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, bits, seen, cache->dim, elem_type, requests, max_query_len);
   if (scratch_bytes < shape.bytes() || !scratch) {
     set_error("scratch too small: %lld bytes, needed %lld", static_cast<long long>(scratch_bytes),
               static_cast<long long>(shape.bytes()));

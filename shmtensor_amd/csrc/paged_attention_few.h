@@ -23,7 +23,7 @@ struct JoinShared {
 };
 
 template <typename T, int BITS, bool TREE, int DIM, int NT>
-__global__ __launch_bounds__(256, attn_waves(BITS, DIM, NT)) void page_attention_kernel(
+__global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float16>::value, DIM, NT))) void page_attention_kernel(
     AttnArgs a, float *parts, float *part_stats, JoinRecord *records) {
   constexpr int kRows = 16 * NT;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
@@ -164,11 +164,33 @@ __global__ __launch_bounds__(256, attn_waves(BITS, DIM, NT)) void page_attention
       }
       return k;
     };
+    // In 4 bits the next tile waits in registers of its own. In 8 those would be too many: the next keys are loaded into the place of
+    // the present ones when these have been multiplied, the next values likewise, and three waves a SIMD have enough in flight.
+    constexpr bool kInPlace = BITS == 8;
     KvTile<BITS, DIM> ahead;
-    auto fetch = [&](int k) {
+    auto fetch_keys = [&](int k) {
       const int at = 2 * (k - page_base);
-      load_half<BITS, DIM>(places.of_lane(at), 1 << a.v.log2_page, offsets, 0, ahead);
-      load_half<BITS, DIM>(places.of_lane(at + 1), 1 << a.v.log2_page, offsets, 1, ahead);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) load_keys<BITS, DIM>(places.of_lane(at + half), 1 << a.v.log2_page, offsets, half, ahead);
+    };
+    auto fetch_values = [&](int k) {
+      const int at = 2 * (k - page_base);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) load_values<BITS, DIM>(places.of_lane(at + half), offsets, half, ahead);
+    };
+    auto fetch = [&](int k) {
+      if constexpr (kInPlace) {
+        fetch_keys(k);
+        fetch_values(k);
+      } else {
+        const int at = 2 * (k - page_base);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const Place16 x = places.of_lane(at + half);
+          load_keys<BITS, DIM>(x, 1 << a.v.log2_page, offsets, half, ahead);
+          load_values<BITS, DIM>(x, offsets, half, ahead);
+        }
+      }
       return Step{token_of(k), present_of(k)};
     };
     bool wild = false, waiting = true, far = false;
@@ -194,13 +216,25 @@ __global__ __launch_bounds__(256, attn_waves(BITS, DIM, NT)) void page_attention
       bool more, again = false;
       do {
         const Step now = next;
-        KvTile<BITS, DIM> t = ahead;
-        k = find(k + 1);
-        more = k < last;
-        if (more) next = fetch(k);
         const bool whole = tile_whole(now.token0, now.there);
-        attend_tile<kIsFirst, BITS, TREE, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
-                                                           now.there & 2, sight, wild, waiting, again, far);
+        auto attend = [&](KvTile<BITS, DIM> &t, auto keys_done, auto values_done) {
+          attend_tile<kIsFirst, BITS, TREE, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
+                                                             now.there & 2, sight, wild, waiting, again, far, keys_done,
+                                                             values_done);
+        };
+        if constexpr (kInPlace) {
+          k = find(k + 1);
+          more = k < last;
+          const int then = more ? k : page_base;  // behind the last tile some tile is loaded once more
+          next = Step{token_of(then), present_of(then)};
+          attend(ahead, [&] { fetch_keys(then); }, [&] { fetch_values(then); });
+        } else {
+          KvTile<BITS, DIM> t = ahead;
+          k = find(k + 1);
+          more = k < last;
+          if (more) next = fetch(k);
+          attend(t, [] {}, [] {});
+        }
       } while (more && !again);
       return again;
     };

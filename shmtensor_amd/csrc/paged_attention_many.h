@@ -240,6 +240,8 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       for (int i = 0; i < kSteps; ++i) query_fragment<T>(src + 8 * i, r < rows, flip, q[0][n][i], q[kParts - 1][n][i]);
     }
     const int sinks = a.window > 0 ? a.sinks : 0;
+    // Waves without a row only decode. Of up to 128 rows the first four multiply, one on each SIMD.
+    const bool has_rows = 16 * wave * NT < rows;
     // the first and the last place of the wave's rows, and of the item's
     const int r_first = min(16 * wave * NT, rows - 1), r_last = min(16 * (wave + 1) * NT - 1, rows - 1);
     auto place = [&](int r) { return place_of(a, req, row_token(a, row0 + r)); };
@@ -472,7 +474,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
         decode(next, stage[~k & 1]);
         const int t_then = more ? find(t + 1) : last;
         const Step then = fetch(t_then < last ? t_then : page_base);
-        multiply(now, stage[k & 1], pass, unit, again_at[k & 1]);
+        if (has_rows) multiply(now, stage[k & 1], pass, unit, again_at[k & 1]);
         __syncthreads();
         // This word is written again two tiles on only, behind the next barrier: all waves read the same.
         again = pass < kMaximum && again_at[k & 1] != 0;

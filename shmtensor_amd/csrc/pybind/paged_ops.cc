@@ -227,14 +227,15 @@ py::object page_attention(torch::Tensor query, const torch::Tensor &cache, const
   if (return_lse) lse = new_tensor({tokens, heads}, torch::kFloat32, query);
   if (tokens > 0) {
     query = rows_on_16(query);
+    const int seen = tree ? SHMT_SEEN_TREE : causal ? SHMT_SEEN_CAUSAL : SHMT_SEEN_ALL;
     const int64_t scratch_bytes = shmt_page_attention_as_scratch_bytes(tokens, static_cast<int>(heads), c.kv_heads, c.bits,
-                                                                       c.dim, elem_type(query.scalar_type(), "query"), n,
-                                                                       max_query_len);
+                                                                       seen, c.dim, elem_type(query.scalar_type(), "query"),
+                                                                       n, max_query_len);
     TORCH_CHECK(scratch_bytes >= 0, shmt_last_error());
     torch::Tensor scratch = new_tensor({scratch_bytes}, torch::kUInt8, cache);
     const float scale = softmax_scale ? static_cast<float>(*softmax_scale)
                                       : 1.0f / std::sqrt(static_cast<float>(c.dim));
-    check(shmt_page_attention_as(&c, c.bits, tree ? SHMT_SEEN_TREE : causal ? SHMT_SEEN_CAUSAL : SHMT_SEEN_ALL,
+    check(shmt_page_attention_as(&c, c.bits, seen,
                                  tree ? tree->data_ptr<int32_t>() : nullptr, query.data_ptr(), stride_of(query, 0),
                                  stride_of(query, 1), elem_type(query.scalar_type(), "query"), tokens,
                                  static_cast<int>(heads), block_table.data_ptr<int32_t>(), block_table.size(1), stride,
