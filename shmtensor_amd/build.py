@@ -22,7 +22,8 @@ ORACLE_LIB = os.path.join(ORACLE_DIR, "liboracle.so")
 
 HIP_SOURCES = ["hashmap.hip", "fetch.hip", "scan.hip", "relabel.hip", "sample.hip", "misc.hip",
                "paged.hip", "paged_tree.hip", "paged_attention.hip", "paged_attention_few.hip", "paged_attention_many.hip",
-               "paged_attention_tree.hip", "paged_attention_8.hip", "paged_attention_8_tree.hip", "host_mem.hip", "errors.cc"]
+               "paged_attention_tree.hip", "paged_attention_all.hip", "paged_attention_8.hip", "paged_attention_8_tree.hip",
+               "paged_attention_8_all.hip", "host_mem.hip", "errors.cc"]
 
 MODULE_SOURCES = ["module.cc", "batch_driver.cc", "batch_sampler.cc", "host_tensors.cc", "paged_ops.cc"]
 

@@ -1,5 +1,5 @@
 // What the two attention kernels over the paged cache share: how the work is cut and numbered, how tokens are read and
-// decoded (BITS: 4 or 8 a value), what a row sees (TREE: its request's new tokens are trees), the join of parts.
+// decoded (BITS: 4 or 8 a value), what a row sees (SEEN: SHMT_SEEN_CAUSAL, _TREE or _ALL), the join of parts.
 #pragma once
 #include "common.h"
 #include "paged_dev.h"
@@ -26,7 +26,6 @@ struct AttnArgs {
   int32_t limit;  // tokens that a row of the table has room for
   void *out;
   float *lse;
-  int32_t step;       // -1: a row's place moves on with its token; 0: all rows are at the last one (they see all)
   const int4 *nodes;  // trees: number, size, depth and least depth of each row's node
 };
 
@@ -80,30 +79,34 @@ __device__ __forceinline__ Span same(Span s) {
   return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.sink_end), same(s.begin), same(s.end)};
 }
 
+template <int SEEN>
 __device__ __forceinline__ Request attn_request(const AttnArgs &a, int64_t b) {
   Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b);
-  r.before += (r.queries - 1) & ~a.step;  // all rows at the last token
+  if constexpr (SEEN == SHMT_SEEN_ALL) r.before += r.queries - 1;  // all rows look from the last token
   return r;
 }
 
 // The place that a row of the request's query `token` looks from. Of trees, the furthest that it may be.
-__device__ __forceinline__ int place_of(const AttnArgs &a, const Request &r, int token) { return r.before + (token & a.step); }
-
-// The last token that every row from `token` on sees, but for windows: trees, the last that was there before.
-template <bool TREE>
-__device__ __forceinline__ int seen_by_all(const AttnArgs &a, const Request &r, int token) {
-  return min(TREE ? r.before - 1 : place_of(a, r, token), a.limit - 1);
+template <int SEEN>
+__device__ __forceinline__ int place_of(const Request &r, int token) {
+  return SEEN == SHMT_SEEN_ALL ? r.before : r.before + token;
 }
 
-template <bool TREE, int ROWS>
+// The last token that every row from `token` on sees, but for windows: trees, the last that was there before.
+template <int SEEN>
+__device__ __forceinline__ int seen_by_all(const AttnArgs &a, const Request &r, int token) {
+  return min(SEEN == SHMT_SEEN_TREE ? r.before - 1 : place_of<SEEN>(r, token), a.limit - 1);
+}
+
+template <int SEEN, int ROWS>
 __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, int row0) {
   const int all = r.queries * a.group;
   const int t_first = static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group));
   const int t_last =
       static_cast<int>(static_cast<uint32_t>(min(row0 + ROWS, all) - 1) / static_cast<uint32_t>(a.group));
   Span s;
-  s.end = max(min(place_of(a, r, t_last) + 1, a.limit), 0);
-  if constexpr (TREE) {
+  s.end = max(min(place_of<SEEN>(r, t_last) + 1, a.limit), 0);
+  if constexpr (SEEN == SHMT_SEEN_TREE) {
     // A node's place is its depth's, which is at most its token's: what is behind the least place's window in tokens holds all
     // that a window shows. First tokens may be nodes, too.
     s.begin = 0;
@@ -112,7 +115,7 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
       if (a.sinks > r.before) s.begin = min(s.begin, max(r.before, 0));
     }
   } else {
-    s.begin = a.window > 0 ? max(min(max(place_of(a, r, t_first), -1) - a.window + 1, s.end), 0) : 0;
+    s.begin = a.window > 0 ? max(min(max(place_of<SEEN>(r, t_first), -1) - a.window + 1, s.end), 0) : 0;
   }
   s.tile0 = s.begin / kUnit;
   s.sink_end = min(a.sinks, s.begin);
@@ -122,11 +125,11 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
 }
 
 // Units of a request for one head.
-template <bool TREE, int ROWS>
+template <int SEEN, int ROWS>
 __device__ __forceinline__ int64_t attn_units(const AttnArgs &a, const Request &r) {
   int64_t n = 0;
   const int all = r.queries * a.group;
-  for (int row0 = 0; row0 < all; row0 += ROWS) n += attn_span<TREE, ROWS>(a, r, row0).units;
+  for (int row0 = 0; row0 < all; row0 += ROWS) n += attn_span<SEEN, ROWS>(a, r, row0).units;
   return n;
 }
 
@@ -192,15 +195,15 @@ struct Sees {
   int last, after;
   int number;
 };
-template <bool TREE>
+template <int SEEN>
 __device__ __forceinline__ Sees row_sees(const AttnArgs &a, const Request &r, int token, bool there) {
-  if constexpr (TREE) {
+  if constexpr (SEEN == SHMT_SEEN_TREE) {
     if (!there) return {-1, 0x7fffffff, -1};
     const int4 node = a.nodes[r.first_row + token];
     const int64_t after = int64_t{r.before} + node.z - a.window;
     return {min(r.before - 1, a.limit - 1), a.window > 0 ? static_cast<int>(max(after, int64_t{-0x7fffffff})) : -0x7fffffff, node.x};
   } else {
-    const int pos = there ? place_of(a, r, token) : -1;
+    const int pos = there ? place_of<SEEN>(r, token) : -1;
     return {min(max(pos, -1), a.limit - 1), a.window > 0 && pos >= 0 ? pos - a.window : -1, 0};
   }
 }
@@ -208,10 +211,10 @@ __device__ __forceinline__ Sees row_sees(const AttnArgs &a, const Request &r, in
 __device__ __forceinline__ bool is_above(const int4 &node, int number) {
   return static_cast<uint32_t>(number - node.x) < static_cast<uint32_t>(node.y);
 }
-template <bool TREE>
+template <int SEEN>
 __device__ __forceinline__ bool sees_token(const AttnArgs &a, const Request &r, const Sees &s, int j, int sinks) {
   if (j <= s.last) return j > s.after || j < sinks;
-  if (!TREE || j < r.before || j >= r.before + r.queries) return false;
+  if (SEEN != SHMT_SEEN_TREE || j < r.before || j >= r.before + r.queries) return false;
   const int4 node = a.nodes[r.first_row + (j - r.before)];
   const int place = r.before + node.z;
   return is_above(node, s.number) && (place > s.after || place < sinks);
@@ -517,7 +520,7 @@ constexpr uint32_t kWild = BITS == 8 ? 247 : 253;
 // FIRST: `pass` is kFirst or kRaised; rows may be `waiting` for a reference. `again` is set if the wave has to begin its tokens
 // again, `far` if with rounded scores.
 // `keys_done` and `values_done` are called when the tile's keys and values are not needed any more.
-template <bool FIRST, int BITS, bool TREE, int DIM, int NT, int PARTS, typename KeysDone, typename ValuesDone>
+template <bool FIRST, int BITS, int SEEN, int DIM, int NT, int PARTS, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<DIM, NT, PARTS> &q, RowState<DIM, NT> &st,
                                             float scale2, int pass, int lane, bool whole, int token0, bool there0,
                                             bool there1, const Sight<NT> &sight, bool &wild, bool &waiting, bool &again,
@@ -547,7 +550,7 @@ __device__ __forceinline__ void attend_tile(KvTile<BITS, DIM> &t, const Queries<
   if constexpr (NT * DIM >= 512) __builtin_amdgcn_sched_barrier(0);
   keys_done();
   if (!whole) {
-    if (TREE && token0 + kWaveTokens > sight.fresh) {
+    if (SEEN == SHMT_SEEN_TREE && token0 + kWaveTokens > sight.fresh) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int token = token0 + 16 * (j / 4) + 4 * g + j % 4;
@@ -679,7 +682,7 @@ __device__ float score_of(const T *q, const uint8_t *codes, const uint8_t *scale
 
 // Adds, for one row and DIM / 16 of its dimensions from d0 on, the values of the 16 tokens from j0 on (page `at`) that the
 // products left out: those that are not finite in bfloat16 and that the row sees.
-template <typename T, int BITS, bool TREE, int DIM>
+template <typename T, int BITS, int SEEN, int DIM>
 __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at, int j0, const T *q_row, const Request &req,
                                              const Sees &sees, float scale2, float base, int d0, f32x4 (&o)[DIM / 64]) {
 #pragma clang fp contract(off)
@@ -694,7 +697,7 @@ __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at
   for (int i = 0; i < 16; ++i) {
     const int j = j0 + i;
     const uint32_t byte = sc[(DIM / 32 + d0 / 32) * page + i];
-    if (byte < kWild<BITS> || !sees_token<TREE>(a, req, sees, j, sinks)) continue;
+    if (byte < kWild<BITS> || !sees_token<SEEN>(a, req, sees, j, sinks)) continue;
     const float x = score_of<T, BITS, DIM>(q_row, codes + i * kRow, sc + i, page);
     const float e = __builtin_amdgcn_exp2f((a.scale < 0 ? -x : x) * scale2 - base);  // scores rounded, as in kRounded
     const uint8_t *v = codes + (page + i) * kRow;
@@ -825,20 +828,20 @@ struct AttnShape {
 constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
 // Waves per SIMD that the registers of the kernel for few rows are meant for. Trees and 8 bits take more registers, and fewer waves
-// that spill none are quicker. us with one wave more a SIMD and as it is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in
+// that spill none are quicker (and leave fewer parts); so are they for an encoder's states. us with one wave more a SIMD and as it is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in
 // 4 bits, 64 dimensions bfloat16 36 and 30, 128 dimensions 40 and 35, float16 46 and 36; in 8 bits, 64 dimensions float16 43 and
 // 34, 128 dimensions 66 and 54, 256 dimensions 141 and 114 (bfloat16 115 with one wave, 119 with two, but 59 and 57 where
 // requests are short); 32 rows of 256 dimensions 144 and 116.
-constexpr int attn_waves(int bits, bool tree, bool f16, int dim, int tiles) {
-  if (bits == 8 || tree) return dim == 256 ? (tiles == 1 && !f16 ? 2 : 1) : tiles * dim <= 64 ? 3 : 2;
+constexpr int attn_waves(int bits, int seen, bool f16, int dim, int tiles) {
+  if (bits == 8 || seen != SHMT_SEEN_CAUSAL) return dim == 256 ? (tiles == 1 && !f16 ? 2 : 1) : tiles * dim <= 64 ? 3 : 2;
   return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2;
 }
 
 // paged_attention_few.h, paged_attention_many.h
-template <int BITS, bool TREE>
+template <int BITS, int SEEN>
 void launch_attention_few(const AttnArgs &a, int dim, int elem_type, int rows, unsigned groups, const AttnScratch &s,
                           hipStream_t stream);
-template <int BITS, bool TREE>
+template <int BITS, int SEEN>
 void launch_attention_many(const AttnArgs &a, int dim, int elem_type, unsigned groups, const AttnScratch &s, hipStream_t stream);
 constexpr int attn_many_groups() { return 256; }
 

@@ -1,6 +1,6 @@
 // Attention over the paged key/value cache: which kernel a call takes, and the entry points (shmt_page_attention,
 // shmt_page_attention_as). The kernels are in paged_attention_few.h and paged_attention_many.h, compiled in a file each for 4
-// and 8 bits, chains and trees.
+// and 8 bits and each rule of what a row sees.
 #include "paged_attention.h"
 #include "paged_host.h"
 
@@ -21,8 +21,7 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   //   256 dimensions: 64 rows 179 and 185, 96 rows 293 and 191; float16 64 rows 193 and 277, 96 rows 312 and 282.
   // So an item costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the card idles
   // behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
-  // Chains in 4 bits keep that rule, and with it their results. Otherwise a last item of half the rows or fewer is told apart: the
-  // waves that have none of them only decode. Trees, as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and
+  // Trees and 8 bits: a last item of half the rows or fewer is told apart, as the waves that have none of them only decode. Trees, as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and
   // 119, 128 rows 129 and 121, 160 rows 169 and 146; 8 bits, 64 rows 87 and 122, 96 rows 137 and 124; float16: 4 bits, 128 rows 141
   // and 164, 192 rows 216 and 224, 224 rows 251 and 228, 320 rows 344 and 409; 64 dimensions, bfloat16: 96 rows 91 and 90, 128 rows
   // 104 and 90; 256 dimensions, bfloat16: 64 rows 155 and 157, in 8 bits 175 and 167, 96 rows 240 and 203; float16: 64 rows 187 and
@@ -35,7 +34,7 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
     last = dim == 256 ? 1 + f16 : f16 ? 4 : bits == 8 && dim == 128 ? 2 : 3;
   s.many = rows > 2 * many_rows(dim) || (few_items > worth * whole + last && tokens * group * kv_heads >= 16384);
   s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;
-  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(bits, seen == SHMT_SEEN_TREE, f16, dim, s.rows / 16);
+  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(bits, seen, f16, dim, s.rows / 16);
   s.items = s.many ? tokens * group / s.rows + requests : 0;
   const int64_t lines = 2 * s.groups * s.rows;
   s.parts_bytes = lines * dim * 4;
@@ -46,7 +45,7 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   return s;
 }
 
-void launch_attention(const AttnArgs &a, int bits, int dim, int elem_type, const AttnShape &shape, void *scratch,
+void launch_attention(const AttnArgs &a, int bits, int seen, int dim, int elem_type, const AttnShape &shape, void *scratch,
                       hipStream_t stream) {
   char *at = static_cast<char *>(scratch);
   AttnScratch s{};
@@ -61,16 +60,18 @@ void launch_attention(const AttnArgs &a, int bits, int dim, int elem_type, const
   const int64_t units = (a.tokens * a.group / shape.rows + a.requests) * a.v.kv_heads *
                         (a.limit / kUnit + 1 + item_cost(shape.rows));
   const unsigned groups = static_cast<unsigned>(std::min(shape.groups, std::max<int64_t>(units, 1)));
-  auto launch = [&](auto bits, auto tree) {
-    constexpr int kBits = decltype(bits)::value;
-    constexpr bool kTree = decltype(tree)::value;
-    if (shape.many) launch_attention_many<kBits, kTree>(a, dim, elem_type, groups, s, stream);
-    else launch_attention_few<kBits, kTree>(a, dim, elem_type, shape.rows, groups, s, stream);
+  auto launch = [&](auto bits, auto seen) {
+    constexpr int kBits = decltype(bits)::value, kSeen = decltype(seen)::value;
+    if (shape.many) launch_attention_many<kBits, kSeen>(a, dim, elem_type, groups, s, stream);
+    else launch_attention_few<kBits, kSeen>(a, dim, elem_type, shape.rows, groups, s, stream);
   };
-  using Four = std::integral_constant<int, 4>;
-  using Eight = std::integral_constant<int, 8>;
-  if (bits == 8) a.nodes ? launch(Eight{}, std::true_type{}) : launch(Eight{}, std::false_type{});
-  else a.nodes ? launch(Four{}, std::true_type{}) : launch(Four{}, std::false_type{});
+  auto with_seen = [&](auto bits) {
+    if (seen == SHMT_SEEN_TREE) launch(bits, std::integral_constant<int, SHMT_SEEN_TREE>{});
+    else if (seen == SHMT_SEEN_ALL) launch(bits, std::integral_constant<int, SHMT_SEEN_ALL>{});
+    else launch(bits, std::integral_constant<int, SHMT_SEEN_CAUSAL>{});
+  };
+  if (bits == 8) with_seen(std::integral_constant<int, 8>{});
+  else with_seen(std::integral_constant<int, 4>{});
 }
 
 }  // namespace shmt
@@ -149,8 +150,8 @@ int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen, co
                    table_stride, query_starts, kv_lens, len_bytes, requests, softmax_scale,
                    static_cast<int32_t>(std::min(window, kMost)), static_cast<int32_t>(std::min(sinks, kMost)),
                    v.pages > 0 ? static_cast<int32_t>(width * cache->page) : 0, out, lse,
-                   seen == SHMT_SEEN_ALL ? 0 : -1, seen == SHMT_SEEN_TREE ? reinterpret_cast<const int4 *>(nodes) : nullptr};
-  launch_attention(a, bits, cache->dim, elem_type, shape, scratch, as_stream(stream));
+                   seen == SHMT_SEEN_TREE ? reinterpret_cast<const int4 *>(nodes) : nullptr};
+  launch_attention(a, bits, seen, cache->dim, elem_type, shape, scratch, as_stream(stream));
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;
 }

@@ -4,7 +4,8 @@
 
 namespace shmt {
 
-template void launch_attention_few<8, false>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &, hipStream_t);
-template void launch_attention_many<8, false>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
+template void launch_attention_few<8, SHMT_SEEN_CAUSAL>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &,
+                                                    hipStream_t);
+template void launch_attention_many<8, SHMT_SEEN_CAUSAL>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
 
 }  // namespace shmt

@@ -1,0 +1,11 @@
+// Attention over all of an encoder's states in the paged cache, in 4 bits.
+#include "paged_attention_few.h"
+#include "paged_attention_many.h"
+
+namespace shmt {
+
+template void launch_attention_few<4, SHMT_SEEN_ALL>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &,
+                                                    hipStream_t);
+template void launch_attention_many<4, SHMT_SEEN_ALL>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
+
+}  // namespace shmt

@@ -22,8 +22,8 @@ struct JoinShared {
   float top[4][16], sum[4][16];
 };
 
-template <typename T, int BITS, bool TREE, int DIM, int NT>
-__global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float16>::value, DIM, NT))) void page_attention_kernel(
+template <typename T, int BITS, int SEEN, int DIM, int NT>
+__global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float16>::value, DIM, NT))) void page_attention_kernel(
     AttnArgs a, float *parts, float *part_stats, JoinRecord *records) {
   constexpr int kRows = 16 * NT;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
   if (threadIdx.x == 0) row_range[0] = row_range[1] = a.requests > 0 ? 0 : a.tokens;
   __syncthreads();
   for (int64_t i = b_lo; i < b_hi; ++i) {
-    const Request r = attn_request(a, i);
-    mine += attn_units<TREE, kRows>(a, r) * kv_heads;
+    const Request r = attn_request<SEEN>(a, i);
+    mine += attn_units<SEEN, kRows>(a, r) * kv_heads;
     if (i == 0) row_range[0] = r.first_row;
     if (i == a.requests - 1) row_range[1] = r.first_row + r.queries;
   }
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
   if (at <= u_begin && u_begin < at + mine) {
     int64_t before = at;
     for (int64_t i = b_lo;; ++i) {
-      const Request r = attn_request(a, i);
-      const int64_t n = attn_units<TREE, kRows>(a, r);
+      const Request r = attn_request<SEEN>(a, i);
+      const int64_t n = attn_units<SEEN, kRows>(a, r);
       if (u_begin < before + n * kv_heads) {
         found = Found{r, i, before, n};
         break;
@@ -83,11 +83,11 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
   const int64_t per_head = same(found.units);
   int head = same(static_cast<int>(divide(u_begin - u_item, per_head)));
   u_item += head * per_head;
-  Span span = same(attn_span<TREE, kRows>(a, req, 0));
+  Span span = same(attn_span<SEEN, kRows>(a, req, 0));
   while (u_item + span.units <= u_begin) {
     u_item += span.units;
     row0 += kRows;
-    span = same(attn_span<TREE, kRows>(a, req, row0));
+    span = same(attn_span<SEEN, kRows>(a, req, row0));
   }
 
   const float scale2 = powers_of_two(a);
@@ -101,14 +101,14 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
     sight.sinks = a.window > 0 ? a.sinks : 0;
     sight.begin = span.begin, sight.end = span.end, sight.sink_end = span.sink_end;
     sight.fresh = req.before;
-    if constexpr (TREE) sight.node = a.nodes + (req.first_row - req.before);
+    if constexpr (SEEN == SHMT_SEEN_TREE) sight.node = a.nodes + (req.first_row - req.before);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = 16 * n + n_lane;
       const uint32_t row = row0 + min(r, rows - 1);
       const uint32_t token = row / static_cast<uint32_t>(a.group);
       const int h = head * a.group + static_cast<int>(row - token * a.group);
-      const Sees sees = row_sees<TREE>(a, req, static_cast<int>(token), r < rows);
+      const Sees sees = row_sees<SEEN>(a, req, static_cast<int>(token), r < rows);
       sight.last[n] = sees.last, sight.after[n] = sees.after, sight.number[n] = sees.number;
       const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
                      g * (DIM / 4);
@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
     }
     if constexpr (Q::kShared) __syncthreads();
     // All rows see a whole tile that ends at or before the first row's place and begins in the last row's window.
-    const int pos_first = same(seen_by_all<TREE>(a, req, row_token(a, row0)));
-    const int after_last = same(a.window > 0 ? max(place_of(a, req, row_token(a, row0 + rows - 1)), -1) - a.window : -1);
+    const int pos_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0)));
+    const int after_last = same(a.window > 0 ? max(place_of<SEEN>(req, row_token(a, row0 + rows - 1)), -1) - a.window : -1);
     const int32_t *table = a.table + b * a.table_stride;
     const int first = same(static_cast<int>(u - u_item));
     const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item));
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
         const Step now = next;
         const bool whole = tile_whole(now.token0, now.there);
         auto attend = [&](KvTile<BITS, DIM> &t, auto keys_done, auto values_done) {
-          attend_tile<kIsFirst, BITS, TREE, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
+          attend_tile<kIsFirst, BITS, SEEN, DIM, NT, kParts>(t, q, st, scale2, pass, lane, whole, now.token0, now.there & 1,
                                                              now.there & 2, sight, wild, waiting, again, far, keys_done,
                                                              values_done);
         };
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
               o[i] += f[v] * *reinterpret_cast<const f32x4 *>(&shared.join.acc[v][r * JoinShared<DIM>::kStride + d0 + 4 * i]);
           }
           if (any_wild) {
-            const Sees sees = row_sees<TREE>(a, req, static_cast<int>(token), true);
+            const Sees sees = row_sees<SEEN>(a, req, static_cast<int>(token), true);
             const T *q_row = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head;
             for (int k = first; k < last; ++k)
 #pragma unroll 1
@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
                 const int t0 = unit_token(span, k) + w * kWaveTokens;
                 const int p0 = page_at(a, table, span, t0), p1 = page_at(a, table, span, t0 + 16);
                 if (tile_whole(t0, (p0 >= 0 ? 1u : 0u) | (p1 >= 0 ? 2u : 0u))) continue;
-                add_left_out<T, BITS, TREE, DIM>(a, head, p0, t0, q_row, req, sees, scale2, base, d0, o);
-                add_left_out<T, BITS, TREE, DIM>(a, head, p1, t0 + 16, q_row, req, sees, scale2, base, d0, o);
+                add_left_out<T, BITS, SEEN, DIM>(a, head, p0, t0, q_row, req, sees, scale2, base, d0, o);
+                add_left_out<T, BITS, SEEN, DIM>(a, head, p1, t0 + 16, q_row, req, sees, scale2, base, d0, o);
               }
           }
           const float inv = total == 0 ? 0 : 1 / total;
@@ -336,39 +336,39 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, TREE, std::is_same<T, _Float
       row0 = 0;
       if (++head == kv_heads) {
         head = 0;
-        do req = same(attn_request(a, ++b)); while (req.queries == 0);
+        do req = same(attn_request<SEEN>(a, ++b)); while (req.queries == 0);
       }
     }
-    span = same(attn_span<TREE, kRows>(a, req, row0));
+    span = same(attn_span<SEEN, kRows>(a, req, row0));
   }
 }
 
-template <typename T, int BITS, bool TREE, int DIM, int NT>
+template <typename T, int BITS, int SEEN, int DIM, int NT>
 void launch_few(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  hipLaunchKernelGGL((page_attention_kernel<T, BITS, TREE, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, s.parts, s.stats,
+  hipLaunchKernelGGL((page_attention_kernel<T, BITS, SEEN, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, s.parts, s.stats,
                      s.records);
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(std::min(groups, 512u)), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }
 
-template <typename T, int BITS, bool TREE, int DIM>
+template <typename T, int BITS, int SEEN, int DIM>
 void launch_few(const AttnArgs &a, int rows, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  if (rows == 16) launch_few<T, BITS, TREE, DIM, 1>(a, groups, s, stream);
-  else launch_few<T, BITS, TREE, DIM, 2>(a, groups, s, stream);
+  if (rows == 16) launch_few<T, BITS, SEEN, DIM, 1>(a, groups, s, stream);
+  else launch_few<T, BITS, SEEN, DIM, 2>(a, groups, s, stream);
 }
 
-template <typename T, int BITS, bool TREE>
+template <typename T, int BITS, int SEEN>
 void launch_few(const AttnArgs &a, int dim, int rows, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  if (dim == 64) launch_few<T, BITS, TREE, 64>(a, rows, groups, s, stream);
-  else if (dim == 128) launch_few<T, BITS, TREE, 128>(a, rows, groups, s, stream);
-  else launch_few<T, BITS, TREE, 256>(a, rows, groups, s, stream);
+  if (dim == 64) launch_few<T, BITS, SEEN, 64>(a, rows, groups, s, stream);
+  else if (dim == 128) launch_few<T, BITS, SEEN, 128>(a, rows, groups, s, stream);
+  else launch_few<T, BITS, SEEN, 256>(a, rows, groups, s, stream);
 }
 
-template <int BITS, bool TREE>
+template <int BITS, int SEEN>
 void launch_attention_few(const AttnArgs &a, int dim, int elem_type, int rows, unsigned groups, const AttnScratch &s,
                           hipStream_t stream) {
-  if (elem_type == SHMT_F16) launch_few<_Float16, BITS, TREE>(a, dim, rows, groups, s, stream);
-  else launch_few<__bf16, BITS, TREE>(a, dim, rows, groups, s, stream);
+  if (elem_type == SHMT_F16) launch_few<_Float16, BITS, SEEN>(a, dim, rows, groups, s, stream);
+  else launch_few<__bf16, BITS, SEEN>(a, dim, rows, groups, s, stream);
 }
 
 }  // namespace shmt

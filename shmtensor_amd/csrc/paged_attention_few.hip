@@ -3,6 +3,7 @@
 
 namespace shmt {
 
-template void launch_attention_few<4, false>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &, hipStream_t);
+template void launch_attention_few<4, SHMT_SEEN_CAUSAL>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &,
+                                                    hipStream_t);
 
 }  // namespace shmt

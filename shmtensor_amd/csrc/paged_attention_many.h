@@ -8,7 +8,7 @@ namespace shmt {
 // Items of all requests with the units in front of each, for calls in which a request has many row tiles: one workgroup.
 // items[0 .. n) and, behind the last, the number of units; *count = n. (Only starts that descend could make more items than
 // there is room for.)
-template <bool TREE, int ROWS>
+template <int SEEN, int ROWS>
 __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, int32_t *first_item, AttnItem *items,
                                                                     int64_t room, int32_t *count) {
   __shared__ uint64_t lds[16];
@@ -16,7 +16,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
   for (int64_t base = 0; base < a.requests; base += 1024) {
     const int64_t b = base + threadIdx.x;
     int64_t mine = 0;
-    if (b < a.requests) mine = (attn_request(a, b).queries * a.group + ROWS - 1) / ROWS;
+    if (b < a.requests) mine = (attn_request<SEEN>(a, b).queries * a.group + ROWS - 1) / ROWS;
     uint64_t sum;
     const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
     if (b < a.requests) first_item[b] = static_cast<int32_t>(n + at);
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
         if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
       }
       row0 = static_cast<int>(i - first_item[lo]) * ROWS;
-      mine = attn_span<TREE, ROWS>(a, attn_request(a, lo), row0).units;
+      mine = attn_span<SEEN, ROWS>(a, attn_request<SEEN>(a, lo), row0).units;
     }
     uint64_t sum;
     const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
@@ -98,7 +98,7 @@ struct ManyStage {
   u32x4 value[ManyShape<BITS, DIM>::kGroups][ManyShape<BITS, DIM>::kValueFrags][kWave];
 };
 
-template <typename T, int BITS, bool TREE, int DIM>
+template <typename T, int BITS, int SEEN, int DIM>
 __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_attention_many_kernel(
     AttnArgs a, const AttnItem *items, const int32_t *item_count, float *parts, float *part_stats, JoinRecord *records) {
   using Shape = ManyShape<BITS, DIM>;
@@ -119,14 +119,14 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
   int64_t per_head, count;
   if (items) {
     count = same(*item_count), per_head = same(items[count].unit);
-    const Request r0 = attn_request(a, 0), r1 = attn_request(a, a.requests - 1);
+    const Request r0 = attn_request<SEEN>(a, 0), r1 = attn_request<SEEN>(a, a.requests - 1);
     attn_clear_rows<T, DIM>(a, r0.first_row, r1.first_row + r1.queries);
   } else {
     if (threadIdx.x == 0) row_range[0] = row_range[1] = a.tokens;
     __syncthreads();
     Request r{};
     if (threadIdx.x < a.requests) {
-      r = attn_request(a, threadIdx.x);
+      r = attn_request<SEEN>(a, threadIdx.x);
       if (threadIdx.x == 0) row_range[0] = r.first_row;
       if (threadIdx.x == a.requests - 1) row_range[1] = r.first_row + r.queries;
     }
@@ -146,7 +146,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       const int mid = (lo + hi + 1) >> 1;
       if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
     }
-    *r = attn_request(a, lo);
+    *r = attn_request<SEEN>(a, lo);
     *row0 = static_cast<int>(i - first_item[lo]) * kRows;
     return lo;
   };
@@ -157,7 +157,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
         Request r;
         int row0;
         item_of(base + threadIdx.x, &r, &row0);
-        mine = attn_span<TREE, kRows>(a, r, row0).units;
+        mine = attn_span<SEEN, kRows>(a, r, row0).units;
       }
       block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all);
       per_head += same(static_cast<int64_t>(all));
@@ -187,7 +187,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     }
     const AttnItem it = items[item];
     b = same(it.request), row0 = same(it.row0), u_item = head * per_head + same(it.unit);
-    req = same(attn_request(a, b));
+    req = same(attn_request<SEEN>(a, b));
   } else {
     int64_t before = 0;
     for (int64_t base = 0; base < count; base += kThreads) {
@@ -196,7 +196,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       int r0 = 0, lo = 0;
       if (base + threadIdx.x < count) {
         lo = item_of(base + threadIdx.x, &r, &r0);
-        mine = attn_span<TREE, kRows>(a, r, r0).units;
+        mine = attn_span<SEEN, kRows>(a, r, r0).units;
       }
       const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all));
       if (at <= x && x < at + static_cast<int64_t>(mine)) found = Found{r, lo, at, r0};
@@ -223,7 +223,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
   const uint32_t value_scale_at = (DIM / 32 + n_lane * (DIM / 16) / 32) * page + 4 * g;
 
   for (int64_t u = u_begin; u < u_end;) {
-    const Span span = same(attn_span<TREE, kRows>(a, req, row0));
+    const Span span = same(attn_span<SEEN, kRows>(a, req, row0));
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
     int see_last[NT], see_after[NT], see_number[NT];
@@ -232,7 +232,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       const int r = 16 * (wave * NT + n) + n_lane;
       const int row = row0 + min(r, rows - 1), token = row_token(a, row);
       const int h = head * a.group + row - token * a.group;
-      const Sees sees = row_sees<TREE>(a, req, token, r < rows);
+      const Sees sees = row_sees<SEEN>(a, req, token, r < rows);
       see_last[n] = sees.last, see_after[n] = sees.after, see_number[n] = sees.number;
       const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
                      g * (DIM / 4);
@@ -240,14 +240,16 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       for (int i = 0; i < kSteps; ++i) query_fragment<T>(src + 8 * i, r < rows, flip, q[0][n][i], q[kParts - 1][n][i]);
     }
     const int sinks = a.window > 0 ? a.sinks : 0;
-    // Waves without a row only decode. Of up to 128 rows the first four multiply, one on each SIMD.
-    const bool has_rows = 16 * wave * NT < rows;
+    // Waves without a row only decode: of up to 128 rows the first four multiply, one on each SIMD. (16 rows to a wave in turn, so
+    // that the SIMDs share what there is, brought 8 % for 160 and 192 rows of bfloat16 and lost 5 to 9 % for 128 and 256; chains
+    // in 4 bits lose 2 % by the question itself, two prompts 1,071 us instead of 1,050.)
+    const bool has_rows = (BITS == 4 && SEEN == SHMT_SEEN_CAUSAL) || 16 * wave * NT < rows;
     // the first and the last place of the wave's rows, and of the item's
     const int r_first = min(16 * wave * NT, rows - 1), r_last = min(16 * (wave + 1) * NT - 1, rows - 1);
-    auto place = [&](int r) { return place_of(a, req, row_token(a, row0 + r)); };
+    auto place = [&](int r) { return place_of<SEEN>(req, row_token(a, row0 + r)); };
     auto after = [&](int r) { return a.window > 0 ? max(place(r), -1) - a.window : -1; };
-    const int wave_first = same(seen_by_all<TREE>(a, req, row_token(a, row0 + r_first))), wave_after = same(after(r_last));
-    const int item_first = same(seen_by_all<TREE>(a, req, row_token(a, row0))), item_after = same(after(rows - 1));
+    const int wave_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0 + r_first))), wave_after = same(after(r_last));
+    const int item_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0))), item_after = same(after(rows - 1));
     const int32_t *table = a.table + b * a.table_stride;
     const int first = same(static_cast<int>(u - u_item)) * kSub;
     const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item)) * kSub;
@@ -402,7 +404,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
         fence();
         if (!whole) {
           const int token_0 = s.token0 + 32 * group;
-          if (TREE && token_0 + 32 > req.before) {
+          if (SEEN == SHMT_SEEN_TREE && token_0 + 32 > req.before) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int half = 2 * group + j / 4, token = token_0 + 16 * (j / 4) + 4 * g + j % 4;
@@ -508,7 +510,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
 #pragma unroll
         for (int i = 0; i < DIM / 16; ++i) o[i / 4][i % 4] = st.acc[n][i][r4];
         if (add_wild) {
-          const Sees sees = row_sees<TREE>(a, req, token, true);
+          const Sees sees = row_sees<SEEN>(a, req, token, true);
           const T *q_row = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head;
 #pragma unroll 1
           for (int t = first; t < last; ++t) {
@@ -519,7 +521,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
 #pragma unroll 1
             for (int half = 0; half < kHalves; ++half) {
               const int j0 = token_of(t) + 16 * half;
-              add_left_out<T, BITS, TREE, DIM>(a, head, page_at(a, table, span, j0), j0, q_row, req, sees, powers_of_two(a), base,
+              add_left_out<T, BITS, SEEN, DIM>(a, head, page_at(a, table, span, j0), j0, q_row, req, sees, powers_of_two(a), base,
                                                d0, o);
             }
           }
@@ -557,39 +559,39 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       row0 = 0;
       do {
         if (++b == a.requests) b = 0, ++head;
-        req = same(attn_request(a, b));
+        req = same(attn_request<SEEN>(a, b));
       } while (req.queries == 0);
     }
   }
 }
 
-template <typename T, int BITS, bool TREE, int DIM>
+template <typename T, int BITS, int SEEN, int DIM>
 void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
   // A list of items costs a launch; every workgroup counts for itself where that takes no longer, or there is nothing to count.
   const AttnItem *items = nullptr;
   if (a.requests > 256 || (a.requests > 0 && s.room > 1024)) {
-    hipLaunchKernelGGL((page_attention_items_kernel<TREE, many_rows(DIM)>), dim3(1), dim3(1024), 0, stream, a, s.first_item,
+    hipLaunchKernelGGL((page_attention_items_kernel<SEEN, many_rows(DIM)>), dim3(1), dim3(1024), 0, stream, a, s.first_item,
                        s.items, s.room, s.count);
     items = s.items;
   }
-  hipLaunchKernelGGL((page_attention_many_kernel<T, BITS, TREE, DIM>), dim3(groups), dim3(ManyShape<BITS, DIM>::kThreads), 0,
+  hipLaunchKernelGGL((page_attention_many_kernel<T, BITS, SEEN, DIM>), dim3(groups), dim3(ManyShape<BITS, DIM>::kThreads), 0,
                      stream, a, items, s.count, s.parts, s.stats, s.records);
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, many_rows(DIM)>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }
 
-template <typename T, int BITS, bool TREE>
+template <typename T, int BITS, int SEEN>
 void launch_many(const AttnArgs &a, int dim, unsigned groups, const AttnScratch &s, hipStream_t stream) {
-  if (dim == 64) launch_many<T, BITS, TREE, 64>(a, groups, s, stream);
-  else if (dim == 128) launch_many<T, BITS, TREE, 128>(a, groups, s, stream);
-  else launch_many<T, BITS, TREE, 256>(a, groups, s, stream);
+  if (dim == 64) launch_many<T, BITS, SEEN, 64>(a, groups, s, stream);
+  else if (dim == 128) launch_many<T, BITS, SEEN, 128>(a, groups, s, stream);
+  else launch_many<T, BITS, SEEN, 256>(a, groups, s, stream);
 }
 
-template <int BITS, bool TREE>
+template <int BITS, int SEEN>
 void launch_attention_many(const AttnArgs &a, int dim, int elem_type, unsigned groups, const AttnScratch &s,
                            hipStream_t stream) {
-  if (elem_type == SHMT_F16) launch_many<_Float16, BITS, TREE>(a, dim, groups, s, stream);
-  else launch_many<__bf16, BITS, TREE>(a, dim, groups, s, stream);
+  if (elem_type == SHMT_F16) launch_many<_Float16, BITS, SEEN>(a, dim, groups, s, stream);
+  else launch_many<__bf16, BITS, SEEN>(a, dim, groups, s, stream);
 }
 
 }  // namespace shmt

@@ -3,6 +3,6 @@
 
 namespace shmt {
 
-template void launch_attention_many<4, false>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
+template void launch_attention_many<4, SHMT_SEEN_CAUSAL>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
 
 }  // namespace shmt

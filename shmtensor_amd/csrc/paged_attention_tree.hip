@@ -4,7 +4,8 @@
 
 namespace shmt {
 
-template void launch_attention_few<4, true>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &, hipStream_t);
-template void launch_attention_many<4, true>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
+template void launch_attention_few<4, SHMT_SEEN_TREE>(const AttnArgs &, int, int, int, unsigned, const AttnScratch &,
+                                                    hipStream_t);
+template void launch_attention_many<4, SHMT_SEEN_TREE>(const AttnArgs &, int, int, unsigned, const AttnScratch &, hipStream_t);
 
 }  // namespace shmt

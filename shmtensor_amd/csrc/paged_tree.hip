@@ -96,19 +96,22 @@ __device__ __forceinline__ int least_from(int x) {
 
 constexpr int kNoDepth = 0x7fffffff;
 
-// A tree of up to 64 nodes, a lane each.
+// A tree of up to 64 nodes, a lane each. From the last node to the first, each gives its size to its parent and to the siblings in
+// front of it (their `later`); a node's number is what lies in front of it: in its parent, the parent itself, in the parent's, ...
 __device__ __forceinline__ void small_tree(const TreeArgs &a, const Request &r, int p) {
   const int lane = lane_id(), n = r.queries;
-  const uint64_t above = lanes_above(p, lane < n);
-  int size = 0;
-  for (int j = 0; j < n; ++j) {
-    const int below = __popcll(__ballot(above >> j & 1));
-    size = lane == j ? below : size;
+  int size = lane < n ? 1 : 0, later = 0;
+  for (int s = n - 1; s > 0; --s) {
+    const int p_s = __builtin_amdgcn_readlane(p, s), size_s = __builtin_amdgcn_readlane(size, s);
+    size += lane == p_s ? size_s : 0;
+    later += p == p_s && lane < s ? size_s : 0;
   }
-  const int depth = __popcll(above) - 1;
-  const int number = sum_above(p, earlier_siblings(p, size, n)) + depth;
+  const int of_parent = __shfl(size, max(p, 0), kWave);
+  const int before = (p >= 0 ? of_parent - 1 : n) - size - later;  // earlier children of the same parent
+  const int both = sum_above(p, (before + (p >= 0 ? 1 : 0)) | 1 << 16);  // number and depth, which are below 64
+  const int depth = (both >> 16) - 1;
   const int least = least_from(lane < n ? depth : kNoDepth);
-  if (lane < n) put_node(a, r, lane, number, size, depth, least);
+  if (lane < n) put_node(a, r, lane, both & 0xffff, size, depth, least);
 }
 
 // Four words a node that the lanes of one wave hand to each other: in LDS, or in the result itself, past the first-level cache.
@@ -187,38 +190,48 @@ __device__ void large_tree(const TreeArgs &a, const Request &r, Memory m) {
 
 constexpr int kTreeLds = 1024;  // nodes
 
-// A wave takes a request of up to 64 nodes; the larger ones of a workgroup's four are done by all of it (a chain, as a prompt
-// is one), or by its first wave.
-__global__ __launch_bounds__(256) void page_tree_kernel(TreeArgs a) {
+// Whether a request's nodes are one chain, as a prompt's are: node i's parent is i - 1.
+__device__ __forceinline__ bool is_chain(const TreeArgs &a, const Request &r) {
+  constexpr int kEach = 8;  // loads on their way
+  const int n = r.queries;
+  for (int base = 0; base < n; base += kEach * kWave) {
+    int p[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) p[k] = a.parents[r.first_row + min(base + k * kWave + lane_id(), n - 1)];
+    bool other = false;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = min(base + k * kWave + lane_id(), n - 1);
+      other |= (p[k] >= 0 && p[k] < i ? p[k] : -1) != i - 1;
+    }
+    if (__ballot(other)) return false;
+  }
+  return true;
+}
+
+// A wave a request, a workgroup a wave: what there is to do is two dependent reads and some 400 instructions, so a launch is
+// quickest when no wave waits for another. Four requests to a workgroup, the larger ones one after the other by all of it, took
+// 8.8 us instead of 6.5 for 481 trees of up to 64 nodes and 20 prompts of 400; 6 requests of up to 16 nodes 4.3 and 3.8.
+__global__ __launch_bounds__(kWave) void page_tree_kernel(TreeArgs a) {
   __shared__ int words[kTreeLds][4];
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = lane_id();
   const NoRequest none = rows_of_no_request(a.starts, a.len_bytes, a.requests, a.tokens);
-  for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none.lo + a.tokens - none.hi; i += int64_t{gridDim.x} * 256) {
+  for (int64_t i = int64_t{blockIdx.x} * kWave + lane; i < none.lo + a.tokens - none.hi; i += int64_t{gridDim.x} * kWave) {
     const int64_t row = i < none.lo ? i : i - none.lo + none.hi;
     a.nodes[row] = make_int4(-1, -1, -1, -1);
     a.positions[row] = -1;
   }
-  for (int64_t b0 = int64_t{blockIdx.x} * 4; b0 < a.requests; b0 += int64_t{gridDim.x} * 4) {
-    bool large = false;
-    if (b0 + wave < a.requests) {
-      const Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b0 + wave);
-      large = r.queries > kWave;
-      if (!large && r.queries > 0) small_tree(a, r, parent_of(a, r.first_row, lane, r.queries));
-    }
-    if (!__syncthreads_or(large)) continue;
-    for (int w = 0; w < 4 && b0 + w < a.requests; ++w) {
-      const Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b0 + w);
-      const int n = r.queries;
-      if (n <= kWave) continue;
-      bool other = false;
-      for (int i = threadIdx.x; i < n; i += 256) other |= parent_of(a, r.first_row, i, n) != i - 1;
-      if (!__syncthreads_or(other)) {
-        for (int i = threadIdx.x; i < n; i += 256) put_node(a, r, i, i, n - i, i, i);
-      } else if (wave == 0) {
-        if (n <= kTreeLds) large_tree(a, r, TreeInLds{words});
-        else large_tree(a, r, TreeInMemory{reinterpret_cast<int *>(a.nodes + r.first_row)});
-      }
-      __syncthreads();
+  for (int64_t b = blockIdx.x; b < a.requests; b += gridDim.x) {
+    const Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.tokens, b);
+    const int n = r.queries;
+    if (n <= kWave) {
+      if (n > 0) small_tree(a, r, parent_of(a, r.first_row, lane, n));
+    } else if (is_chain(a, r)) {
+      for (int i = lane; i < n; i += kWave) put_node(a, r, i, i, n - i, i, i);
+    } else if (n <= kTreeLds) {
+      large_tree(a, r, TreeInLds{words});
+    } else {
+      large_tree(a, r, TreeInMemory{reinterpret_cast<int *>(a.nodes + r.first_row)});
     }
   }
 }
@@ -251,32 +264,60 @@ __device__ __forceinline__ int64_t slot_of(const KeepArgs &a, int64_t b, int64_t
   return page >= 0 && page < a.v.pages ? (page << a.v.log2_page) + (token & ((1 << a.v.log2_page) - 1)) : -1;
 }
 
+// Where tile t begins, a layer's keys or values of one head: the codes and the scales of page 0.
+struct KeepTile {
+  uint8_t *codes, *scales;
+};
+__device__ __forceinline__ KeepTile keep_tile(const KeepArgs &a, uint32_t t) {
+  const uint32_t parts = 2 * a.v.kv_heads, layer = t / parts, part = t - layer * parts;
+  return {a.v.cache + layer * a.cache_layer + (int64_t{part} << a.v.log2_page << a.log2_pieces << 4),
+          a.v.scales + layer * a.scales_layer + (int64_t{part} * a.blocks << a.v.log2_page)};
+}
+
+// x[i] and y[i], on their way together.
+__device__ __forceinline__ void load_both(const void *x, const void *y, int64_t i, int bytes, int64_t *a, int64_t *b) {
+  if (bytes == 8) {
+    const int64_t u = static_cast<const int64_t *>(x)[i], v = static_cast<const int64_t *>(y)[i];
+    *a = u, *b = v;
+  } else {
+    const int32_t u = static_cast<const int32_t *>(x)[i], v = static_cast<const int32_t *>(y)[i];
+    *a = u, *b = v;
+  }
+}
+
 constexpr int kMoves = 256;  // of a round
 
 // A request's path and moves are found by the first wave of each of its workgroups, 64 nodes at a time in one sweep: children lie
 // behind their parents, and the first that fits is taken. All rows of a layer's keys (or values) of one head are moved by one
 // wave, places ascending: place k is written after the rows for places up to k have been read, which lie at k or behind it.
+// Bound by five dependent reads (lengths, nodes, table, rows, and their writes), so nothing is moved one after the other that
+// can be on its way together: 120 requests of 24 to 64 nodes, 16 layers of 8 heads of 128 in 8 bits, 10 us on the GPU; a tile at
+// a time 14.4, with a wave's lane 0 looking up the slots 12, with twice as many workgroups, that do not all fit, 11.3.
 __global__ __launch_bounds__(256) void page_keep_kernel(KeepArgs a) {
   __shared__ int64_t src[kMoves], dst[kMoves];
   __shared__ int moves, done;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const NoRequest none = rows_of_no_request(a.starts, a.len_bytes, a.requests, a.rows);
-  for (int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x; i < none.lo + a.rows - none.hi; i += int64_t{gridDim.x} * 256)
-    a.path[i < none.lo ? i : i - none.lo + none.hi] = -1;
   const int64_t b = blockIdx.x / a.splits;
   const int split = blockIdx.x % a.splits;
-  if (b >= a.requests) return;
+  auto clear_rows_of_no_request = [&] {
+    if (split != 0) return;
+    const NoRequest none = rows_of_no_request(a.starts, a.len_bytes, a.requests, a.rows);
+    const int64_t groups = gridDim.x / a.splits;
+    for (int64_t i = b * 256 + threadIdx.x; i < none.lo + a.rows - none.hi; i += groups * 256)
+      a.path[i < none.lo ? i : i - none.lo + none.hi] = -1;
+  };
+  if (b >= a.requests) return clear_rows_of_no_request();
   const Request r = load_request(a.starts, a.kv_lens, a.len_bytes, a.rows, b);
   const int n = r.queries;
   if (n == 0) {
     if (split == 0 && threadIdx.x == 0) a.counts[b] = 0, store_int(a.next, b, a.token_bytes, -1);
-    return;
+    return clear_rows_of_no_request();
   }
   const int given = a.given ? min(max(a.given[b], 1), n) : 1;
   if (split == 0)
     for (int i = threadIdx.x; i < given; i += 256) a.path[r.first_row + i] = i;
-  int at = given - 1, count = given, base = given;
-  int64_t want = load_int(a.picked, r.first_row + at, a.token_bytes);
+  int at = given - 1, count = given, base = at;  // the path's end; its nodes; the 64 that are looked at
+  int64_t want = 0;
   for (;;) {
     if (wave == 0) {
       int listed = 0;
@@ -286,9 +327,9 @@ __global__ __launch_bounds__(256) void page_keep_kernel(KeepArgs a) {
         int64_t token = 0, pick = 0;
         if (i < n) {
           p = a.parents[r.first_row + i];
-          token = load_int(a.tokens, r.first_row + i, a.token_bytes);
-          pick = load_int(a.picked, r.first_row + i, a.token_bytes);
+          load_both(a.tokens, a.picked, r.first_row + i, a.token_bytes, &token, &pick);
         }
+        if (base == given - 1) want = lane64(pick, 0);  // the first 64 begin with the path's end, and fill no list
         while (listed < kMoves) {
           const uint64_t fits = __ballot(i < n && i > at && p == at && token == want);
           if (!fits) {
@@ -300,47 +341,67 @@ __global__ __launch_bounds__(256) void page_keep_kernel(KeepArgs a) {
           want = lane64(pick, l);
           if (lane == 0) {
             if (split == 0) a.path[r.first_row + count] = at;
-            if (at != count) {
-              src[listed] = slot_of(a, b, int64_t{r.before} + at);
-              dst[listed] = slot_of(a, b, int64_t{r.before} + count);
-            }
+            if (at != count) src[listed] = at, dst[listed] = count;
           }
           listed += at != count;
           ++count;
         }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int k = lane; k < listed; k += kWave) {  // tokens to slots
+        const int64_t from = slot_of(a, b, r.before + src[k]), to = slot_of(a, b, r.before + dst[k]);
+        src[k] = from, dst[k] = to;
       }
       if (lane == 0) moves = listed, done = base >= n;
     }
     __syncthreads();
     const int m = moves;
     const bool last = done;
-    const int64_t tiles = a.layers * a.v.kv_heads * 2;
-    const int page = 1 << a.v.log2_page;
-    for (int64_t t = split * 4 + wave; m > 0 && t < tiles; t += a.splits * 4) {
-      const int64_t layer = t / (2 * a.v.kv_heads), part = t % (2 * a.v.kv_heads);  // head and keys or values
-      uint8_t *codes = a.v.cache + layer * a.cache_layer + ((part << a.v.log2_page << a.log2_pieces) << 4);
-      uint8_t *scales = a.v.scales + layer * a.scales_layer + (part * a.blocks << a.v.log2_page);
-      const int rows = kWave >> a.log2_pieces, piece = lane & ((1 << a.log2_pieces) - 1);
+    const uint32_t tiles = static_cast<uint32_t>(a.layers * a.v.kv_heads * 2);
+    // As many rows at a time as a wave has lanes for their codes and for their scales; four tiles' are on their way together.
+    const int rows = min(kWave >> a.log2_pieces, kWave / a.blocks), l = a.v.log2_page, in_page = (1 << l) - 1;
+    const int piece = lane & ((1 << a.log2_pieces) - 1), block = lane % a.blocks;
+    const uint32_t stride = a.splits * 4;
+    for (uint32_t t0 = split * 4 + wave; m > 0 && t0 < tiles; t0 += 4 * stride) {
+      KeepTile tile[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tile[j] = keep_tile(a, t0 + j * stride < tiles ? t0 + j * stride : t0);  // or the first again
       for (int k0 = 0; k0 < m; k0 += rows) {
-        const int k = k0 + (lane >> a.log2_pieces);
-        const int64_t s = k < m ? src[k] : -1, d = k < m ? dst[k] : -1;
-        if (s < 0 || d < 0) continue;
-        const int64_t from = (s >> a.v.log2_page) * a.v.cache_stride + ((s & (page - 1)) << a.log2_pieces << 4) + 16 * piece;
-        const int64_t to = (d >> a.v.log2_page) * a.v.cache_stride + ((d & (page - 1)) << a.log2_pieces << 4) + 16 * piece;
-        *reinterpret_cast<uint4 *>(codes + to) = *reinterpret_cast<const uint4 *>(codes + from);
-      }
-      const int each = kWave / a.blocks, block = lane % a.blocks;
-      for (int k0 = 0; k0 < m; k0 += each) {
-        const int k = k0 + lane / a.blocks;
-        const int64_t s = k < m ? src[k] : -1, d = k < m ? dst[k] : -1;
-        if (s < 0 || d < 0) continue;
-        scales[(d >> a.v.log2_page) * a.v.scales_stride + block * page + (d & (page - 1))] =
-            scales[(s >> a.v.log2_page) * a.v.scales_stride + block * page + (s & (page - 1))];
+        const int k = k0 + (lane >> a.log2_pieces), k_scale = k0 + lane / a.blocks;
+        const int64_t s = src[min(k, m - 1)], d = dst[min(k, m - 1)];
+        const int64_t s_scale = src[min(k_scale, m - 1)], d_scale = dst[min(k_scale, m - 1)];
+        const bool move = lane >> a.log2_pieces < rows && k < m && s >= 0 && d >= 0;
+        const bool move_scale = lane / a.blocks < rows && k_scale < m && s_scale >= 0 && d_scale >= 0;
+        const int64_t from = (s >> l) * a.v.cache_stride + ((s & in_page) << a.log2_pieces << 4) + 16 * piece;
+        const int64_t to = (d >> l) * a.v.cache_stride + ((d & in_page) << a.log2_pieces << 4) + 16 * piece;
+        const int64_t from_scale = (s_scale >> l) * a.v.scales_stride + (block << l) + (s_scale & in_page);
+        const int64_t to_scale = (d_scale >> l) * a.v.scales_stride + (block << l) + (d_scale & in_page);
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 codes[4];
+        uint8_t scale[4];
+        if (move) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) codes[j] = *reinterpret_cast<const u32x4 *>(tile[j].codes + from);
+        }
+        if (move_scale) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) scale[j] = tile[j].scales[from_scale];
+        }
+        if (move) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4 *>(tile[j].codes + to) = codes[j];
+        }
+        if (move_scale) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tile[j].scales[to_scale] = scale[j];
+        }
       }
     }
     __syncthreads();
     if (last) break;
   }
+  clear_rows_of_no_request();
   if (split != 0 || wave != 0) return;
   if (lane == 0) a.counts[b] = count, store_int(a.next, b, a.token_bytes, want);
   for (int i = count + lane; i < n; i += kWave) a.path[r.first_row + i] = -1;
@@ -362,7 +423,7 @@ int shmt_page_tree(const int32_t *parents, const void *query_starts, const void 
   SHMT_REQUIRE(requests == 0 || (query_starts && kv_lens), "query_starts or kv_lens is null");
   SHMT_REQUIRE((reinterpret_cast<int64_t>(nodes) & 15) == 0, "nodes has to begin on 16 bytes");
   const TreeArgs a{parents, query_starts, kv_lens, len_bytes, requests, tokens, reinterpret_cast<int4 *>(nodes), positions};
-  hipLaunchKernelGGL(page_tree_kernel, dim3(grid_for(std::max<int64_t>(requests, 1), 4, 65536)), dim3(256), 0, as_stream(stream), a);
+  hipLaunchKernelGGL(page_tree_kernel, dim3(grid_for(std::max<int64_t>(requests, 1), 1, 65536)), dim3(kWave), 0, as_stream(stream), a);
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;
 }
@@ -375,7 +436,7 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers, int6
   PagedView v;
   const int rc = paged_view(cache, bits, &v);
   if (rc != SHMT_OK) return rc;
-  SHMT_REQUIRE(layers >= 0 && layers <= 65535, "the number of layers must be in [0, 65535]");
+  SHMT_REQUIRE(layers >= 0 && layers < (int64_t{1} << 28) / cache->kv_heads, "too many layers and heads: 2^28 or more");
   SHMT_REQUIRE(((cache_layer_stride | scales_layer_stride) & 15) == 0, "every layer has to begin on 16 bytes");
   const int64_t values = int64_t{cache->kv_heads} * 2 * cache->page * cache->dim;  // of a page
   SHMT_REQUIRE(layers <= 1 || cache->pages == 0 || (cache_layer_stride >= values * bits / 8 && scales_layer_stride >= values / 32),
@@ -394,9 +455,9 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers, int6
              query_starts, kv_lens, len_bytes, requests, rows, parents, tokens, picked, token_bytes, given, counts, path, next, 1};
   while (16 << a.log2_pieces < cache->dim * bits / 8) ++a.log2_pieces;
   if (v.pages == 0) a.width = 0;
-  // workgroups of a request: each has to find the path first, so no more than fill the card, and four tiles for each wave
+  // workgroups of a request: each has to find the path first, so no more than the card holds, and four tiles for each wave
   const int64_t tiles = layers * cache->kv_heads * 2;
-  a.splits = static_cast<int>(std::max<int64_t>(1, std::min((tiles + 15) / 16, 2048 / std::max<int64_t>(requests, 1))));
+  a.splits = static_cast<int>(std::max<int64_t>(1, std::min((tiles + 15) / 16, 1024 / std::max<int64_t>(requests, 1))));
   const int64_t groups = std::max<int64_t>(requests, 1) * a.splits;
   SHMT_REQUIRE(groups < (int64_t{1} << 24), "too many requests in one call");
   hipLaunchKernelGGL(page_keep_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, as_stream(stream), a);
