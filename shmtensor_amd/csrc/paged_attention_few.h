@@ -347,8 +347,10 @@ template <typename T, int BITS, int SEEN, int DIM, int NT>
 void launch_few(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
   hipLaunchKernelGGL((page_attention_kernel<T, BITS, SEEN, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, s.parts, s.stats,
                      s.records);
-  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(std::min(groups, 512u)), dim3(256), 0, stream, a,
-                     s.parts, s.stats, s.records, static_cast<int>(groups));
+  // a workgroup of the join for each row, as far as 512 go
+  const unsigned rows = static_cast<unsigned>(std::min<int64_t>(a.tokens * a.heads, 512));
+  hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(rows), dim3(256), 0, stream, a, s.parts, s.stats,
+                     s.records, static_cast<int>(groups));
 }
 
 template <typename T, int BITS, int SEEN, int DIM>

@@ -45,43 +45,27 @@ __device__ __forceinline__ void put_node(const TreeArgs &a, const Request &r, in
   a.positions[r.first_row + i] = r.before + depth;
 }
 
-// Of 64 nodes, one a lane: which of them are the lane's own or above it, `p` being the parent's lane or -1.
-__device__ __forceinline__ uint64_t lanes_above(int p, bool there) {
+// Of 64 nodes, one a lane, `p` being the parent's lane or -1: x (and y) become their sums over the lane's own and those above it.
+__device__ __forceinline__ void sum_above(int p, int &x, int *y = nullptr) {
   const int lane = lane_id();
-  uint64_t above = there ? uint64_t{1} << lane : 0;
   int jump = p;
   while (__ballot(jump >= 0)) {  // twice as many generations a turn
     const int at = jump >= 0 ? jump : lane;
-    const uint64_t more = static_cast<uint64_t>(shfl64(static_cast<int64_t>(above), at));
-    const int next = __shfl(jump, at, kWave);
-    above |= jump >= 0 ? more : 0;
-    jump = jump >= 0 ? next : -1;
-  }
-  return above;
-}
-
-// The sum of x over the lane's own and those above it.
-__device__ __forceinline__ int sum_above(int p, int x) {
-  const int lane = lane_id();
-  int jump = p;
-  while (__ballot(jump >= 0)) {
-    const int at = jump >= 0 ? jump : lane;
-    const int more = __shfl(x, at, kWave), next = __shfl(jump, at, kWave);
+    const int more = __shfl(x, at, kWave), more_y = y ? __shfl(*y, at, kWave) : 0, next = __shfl(jump, at, kWave);
     x += jump >= 0 ? more : 0;
+    if (y) *y += jump >= 0 ? more_y : 0;
     jump = jump >= 0 ? next : -1;
   }
-  return x;
 }
 
-// The sum of `size` over the lanes in front that have the same parent.
-__device__ __forceinline__ int earlier_siblings(int p, int size, int lanes) {
+// From the last of 64 nodes to the first: each gives its size to its parent, the lane p - base, and to the siblings in front of it.
+__device__ __forceinline__ void give_sizes(int p, int base, int lanes, int &size, int &later) {
   const int lane = lane_id();
-  int sum = 0;
-  for (int s = 0; s < lanes; ++s) {
+  for (int s = lanes - 1; s >= 0; --s) {
     const int p_s = __builtin_amdgcn_readlane(p, s), size_s = __builtin_amdgcn_readlane(size, s);
-    sum += p_s == p && s < lane ? size_s : 0;
+    size += lane == p_s - base ? size_s : 0;
+    later += p == p_s && lane < s ? size_s : 0;
   }
-  return sum;
 }
 
 // The least x from the lane on.
@@ -96,19 +80,15 @@ __device__ __forceinline__ int least_from(int x) {
 
 constexpr int kNoDepth = 0x7fffffff;
 
-// A tree of up to 64 nodes, a lane each. From the last node to the first, each gives its size to its parent and to the siblings in
-// front of it (their `later`); a node's number is what lies in front of it: in its parent, the parent itself, in the parent's, ...
+// A tree of up to 64 nodes, a lane each. A node's number is what lies in front of it: below its parent, in front of that, ...
 __device__ __forceinline__ void small_tree(const TreeArgs &a, const Request &r, int p) {
   const int lane = lane_id(), n = r.queries;
   int size = lane < n ? 1 : 0, later = 0;
-  for (int s = n - 1; s > 0; --s) {
-    const int p_s = __builtin_amdgcn_readlane(p, s), size_s = __builtin_amdgcn_readlane(size, s);
-    size += lane == p_s ? size_s : 0;
-    later += p == p_s && lane < s ? size_s : 0;
-  }
+  give_sizes(p, 0, n, size, later);
   const int of_parent = __shfl(size, max(p, 0), kWave);
   const int before = (p >= 0 ? of_parent - 1 : n) - size - later;  // earlier children of the same parent
-  const int both = sum_above(p, (before + (p >= 0 ? 1 : 0)) | 1 << 16);  // number and depth, which are below 64
+  int both = (before + (p >= 0 ? 1 : 0)) | 1 << 16;  // number and depth, which are below 64
+  sum_above(p, both);
   const int depth = (both >> 16) - 1;
   const int least = least_from(lane < n ? depth : kNoDepth);
   if (lane < n) put_node(a, r, lane, both & 0xffff, size, depth, least);
@@ -135,46 +115,38 @@ struct TreeInMemory {
   }
   __device__ void fence() const { __threadfence(); }
 };
-enum : int { kNumber, kSize, kDepth, kTaken };  // kTaken: nodes below the earlier children
+enum : int { kNumber, kSize, kDepth, kLater };  // kLater: what is below the later children of the same parent
 
 // A larger tree, by one wave, 64 nodes at a time: parents lie in front, so sizes come from the last nodes to the first, numbers
-// and depths from the first to the last. What crosses the 64 goes through `m`.
+// and depths from the first to the last. What crosses the 64 goes through `m`; until a node's turn comes, its size there is what
+// its children have brought so far, and its number its parent.
 template <typename Memory>
 __device__ void large_tree(const TreeArgs &a, const Request &r, Memory m) {
   const int lane = lane_id(), n = r.queries;
   const int last = (n - 1) / kWave * kWave;
-  for (int i = lane; i < n; i += kWave) m.put(i, kSize, 0), m.put(i, kTaken, 0);
+  for (int i = lane; i < n; i += kWave) m.put(i, kSize, 0), m.put(i, kNumber, parent_of(a, r.first_row, i, n));
   m.fence();
+  int roots = 0;  // nodes below later roots
   for (int base = last; base >= 0; base -= kWave) {
-    const int i = base + lane, p = parent_of(a, r.first_row, i, n);
-    const uint64_t above = lanes_above(p >= base ? p - base : -1, i < n);
-    const int weight = i < n ? 1 + m.get(i, kSize) : 0;  // itself and what later nodes brought
-    int size = 0;
-    for (int j = 0; j < kWave; ++j) {
-      const uint64_t above_j = static_cast<uint64_t>(lane64(static_cast<int64_t>(above), j));
-      const int weight_j = __builtin_amdgcn_readlane(weight, j);
-      size += above_j >> lane & 1 ? weight_j : 0;
-    }
-    if (i < n) m.put(i, kSize, size);
+    const int i = base + lane, p = i < n ? m.get(i, kNumber) : -1;
+    int size = i < n ? 1 + m.get(i, kSize) : 0, later = p >= 0 ? m.get(p, kSize) : roots;
+    give_sizes(p, base, kWave, size, later);
+    roots += static_cast<int>(wave_last(wave_inclusive_scan(static_cast<uint32_t>(p < 0 ? size : 0))));
+    m.fence();  // sizes have been read
+    if (i < n) m.put(i, kSize, size), m.put(i, kLater, later);
     if (p >= 0 && p < base) m.add(p, kSize, size);
     m.fence();
   }
-  int roots = 0;  // nodes below earlier roots
   for (int base = 0; base < n; base += kWave) {
-    const int i = base + lane, p = parent_of(a, r.first_row, i, n), near = p >= base ? p - base : -1;
-    const int size = i < n ? m.get(i, kSize) : 0;
-    const int before = (p >= 0 ? m.get(p, kTaken) : roots) + earlier_siblings(p, size, kWave);
-    int number = before + (p >= 0 ? 1 : 0), depth = p >= 0 ? 1 : 0;
-    if (p >= 0 && p < base) number += m.get(p, kNumber), depth += m.get(p, kDepth);
-    number = sum_above(near, number);
-    depth = sum_above(near, depth);
-    int all = p < 0 ? size : 0;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) all += __shfl_xor(all, d, kWave);
-    roots += all;
-    m.fence();  // kTaken has been read
+    const int i = base + lane, p = i < n ? m.get(i, kNumber) : -1, near = p >= base ? p - base : -1;
+    int number = 0, depth = 0;
+    if (i < n) {
+      const int before = (p >= 0 ? m.get(p, kSize) - 1 : n) - m.get(i, kSize) - m.get(i, kLater);
+      number = before + (p >= 0 ? 1 : 0), depth = p >= 0 ? 1 : 0;
+      if (p >= 0 && p < base) number += m.get(p, kNumber), depth += m.get(p, kDepth);
+    }
+    sum_above(near, number, &depth);
     if (i < n) m.put(i, kNumber, number), m.put(i, kDepth, depth);
-    if (p >= 0) m.add(p, kTaken, size);
     m.fence();
   }
   int least = kNoDepth;
