@@ -26,6 +26,7 @@ struct AttnArgs {
   int32_t limit;  // tokens that a row of the table has room for
   void *out;
   float *lse;
+  int32_t alone;      // few rows: an item is one unit, and a workgroup's own: nothing is joined
   const int4 *nodes;  // trees: number, size, depth and least depth of each row's node
 };
 
@@ -63,7 +64,8 @@ struct JoinRecord {
 struct Span {
   int32_t sink_tiles;  // tiles 0 .. sink_tiles
   int32_t tile0;       // then tiles from here
-  int32_t units;
+  int32_t units;       // in the numbering
+  int32_t tiles;       // that there are, at least 1
   int32_t sink_end;    // tokens [0, sink_end) and [begin, end) are all that any row of the item sees
   int32_t begin, end;
 };
@@ -76,7 +78,7 @@ __device__ __forceinline__ int64_t same(int64_t v) {
 }
 __device__ __forceinline__ Request same(Request r) { return {same(r.first_row), same(r.queries), same(r.before)}; }
 __device__ __forceinline__ Span same(Span s) {
-  return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.sink_end), same(s.begin), same(s.end)};
+  return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.tiles), same(s.sink_end), same(s.begin), same(s.end)};
 }
 
 template <int SEEN>
@@ -120,7 +122,8 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
   s.tile0 = s.begin / kUnit;
   s.sink_end = min(a.sinks, s.begin);
   s.sink_tiles = min((s.sink_end + kUnit - 1) / kUnit, s.tile0);
-  s.units = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1) + item_cost(ROWS);
+  s.tiles = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1);
+  s.units = a.alone ? 1 : s.tiles + item_cost(ROWS);
   return s;
 }
 

@@ -45,7 +45,15 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   return s;
 }
 
-void launch_attention(const AttnArgs &a, int bits, int seen, int dim, int elem_type, const AttnShape &shape, void *scratch,
+// Up to how many tokens, as far as the table has room for them, an item is one workgroup's own. Nothing is joined then, which
+// spares a launch and the parts, but an item's tiles come one after the other. us, dealt out and alone, 8 heads of 4 query heads:
+// few rows, 128 dimensions, one request of 256 / 512 / 1,024 tokens, 4 rows: 13.5 and 10.0 / 13.5 and 11.7 / 13.7 and 15.0; 64
+// requests, 32 rows: 19.7 and 16.9 / 24.3 and 21.7; 256 dimensions in 8 bits, one request, 32 rows: 22.6 and 20.9 / 22.7 and 25.8.
+// Many rows, one request, 256 rows of 256 / 512 tokens: 24.2 and 20.7 / 26.4 and 27.5; 8 requests: 36.5 and 22.7 / 40.5 and 29.4.
+// Chains in 4 bits are always dealt out, and keep their results.
+constexpr int alone_tokens(bool many, int dim) { return many || dim == 256 ? 256 : 512; }
+
+void launch_attention(AttnArgs a, int bits, int seen, int dim, int elem_type, const AttnShape &shape, void *scratch,
                       hipStream_t stream) {
   char *at = static_cast<char *>(scratch);
   AttnScratch s{};
@@ -56,9 +64,10 @@ void launch_attention(const AttnArgs &a, int bits, int seen, int dim, int elem_t
   s.count = reinterpret_cast<int32_t *>(s.items + shape.items + 1);
   s.first_item = reinterpret_cast<int32_t *>(at += shape.item_bytes);
   s.room = shape.items;
+  a.alone = (bits == 8 || seen != SHMT_SEEN_CAUSAL) && a.limit <= alone_tokens(shape.many, dim);
   // no more workgroups than there can be units
   const int64_t units = (a.tokens * a.group / shape.rows + a.requests) * a.v.kv_heads *
-                        (a.limit / kUnit + 1 + item_cost(shape.rows));
+                        (a.alone ? 1 : a.limit / kUnit + 1 + item_cost(shape.rows));
   const unsigned groups = static_cast<unsigned>(std::min(shape.groups, std::max<int64_t>(units, 1)));
   auto launch = [&](auto bits, auto seen) {
     constexpr int kBits = decltype(bits)::value, kSeen = decltype(seen)::value;
@@ -149,7 +158,7 @@ int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen, co
   const AttnArgs a{v, query, query_token_stride, query_head_stride, tokens, heads, heads / cache->kv_heads, block_table,
                    table_stride, query_starts, kv_lens, len_bytes, requests, softmax_scale,
                    static_cast<int32_t>(std::min(window, kMost)), static_cast<int32_t>(std::min(sinks, kMost)),
-                   v.pages > 0 ? static_cast<int32_t>(width * cache->page) : 0, out, lse,
+                   v.pages > 0 ? static_cast<int32_t>(width * cache->page) : 0, out, lse, 0,
                    seen == SHMT_SEEN_TREE ? reinterpret_cast<const int4 *>(nodes) : nullptr};
   launch_attention(a, bits, seen, cache->dim, elem_type, shape, scratch, as_stream(stream));
   SHMT_LAUNCH_CHECK();

@@ -27,6 +27,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
     AttnArgs a, float *parts, float *part_stats, JoinRecord *records) {
   constexpr int kRows = 16 * NT;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
+  constexpr bool kOther = BITS == 8 || SEEN != SHMT_SEEN_CAUSAL;  // than chains in 4 bits
   using Q = Queries<DIM, NT, kParts>;
   union Shared {
     JoinShared<DIM> join;
@@ -95,45 +96,18 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
   const LaneOffsets offsets = lane_offsets<BITS, DIM>(lane, 1 << a.v.log2_page);
   for (int64_t u = u_begin; u < u_end;) {
     const int rows = min(kRows, req.queries * a.group - row0);
-    Q q;
-    q.shared = shared.queries;
     Sight<NT> sight;
     sight.sinks = a.window > 0 ? a.sinks : 0;
     sight.begin = span.begin, sight.end = span.end, sight.sink_end = span.sink_end;
     sight.fresh = req.before;
     if constexpr (SEEN == SHMT_SEEN_TREE) sight.node = a.nodes + (req.first_row - req.before);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = 16 * n + n_lane;
-      const uint32_t row = row0 + min(r, rows - 1);
-      const uint32_t token = row / static_cast<uint32_t>(a.group);
-      const int h = head * a.group + static_cast<int>(row - token * a.group);
-      const Sees sees = row_sees<SEEN>(a, req, static_cast<int>(token), r < rows);
-      sight.last[n] = sees.last, sight.after[n] = sees.after, sight.number[n] = sees.number;
-      const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
-                     g * (DIM / 4);
-      constexpr int kSteps = DIM / 32;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        if (Q::kShared && ((n * kSteps + i) & 3) != wave) continue;  // the waves fill LDS together
-        u32x4 y, z;
-        query_fragment<T>(src + 8 * i, r < rows, flip, y, z);
-        if constexpr (Q::kShared) {
-          shared.queries[(n * kSteps + i) * kWave + lane] = y;
-          if constexpr (kParts == 2) shared.queries[((NT + n) * kSteps + i) * kWave + lane] = z;
-        } else {
-          q.own[n * kSteps + i] = y;
-          if constexpr (kParts == 2) q.own[(NT + n) * kSteps + i] = z;
-        }
-      }
-    }
-    if constexpr (Q::kShared) __syncthreads();
     // All rows see a whole tile that ends at or before the first row's place and begins in the last row's window.
     const int pos_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0)));
     const int after_last = same(a.window > 0 ? max(place_of<SEEN>(req, row_token(a, row0 + rows - 1)), -1) - a.window : -1);
     const int32_t *table = a.table + b * a.table_stride;
-    const int first = same(static_cast<int>(u - u_item));
-    const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item));
+    const bool alone = kOther && a.alone;
+    const int first = alone ? 0 : same(static_cast<int>(u - u_item));
+    const int last = alone ? span.tiles : same(static_cast<int>(min(u_item + span.units, u_end) - u_item));
     auto token_of = [&](int k) { return unit_token(span, k) + wave * kWaveTokens; };  // unit k's first token of this wave
     // Whether all rows see all of a wave's 32 tokens from token0 on, of which `there` are present.
     auto tile_whole = [&](int token0, uint32_t there) {
@@ -193,6 +167,44 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
       }
       return Step{token_of(k), present_of(k)};
     };
+    // The first tile, which is on its way before the queries are. (Chains in 4 bits ask for their queries first: that is how they
+    // were measured, and turned round they gain nothing.)
+    int k_first = 0;
+    Step step_first{};
+    auto begin_tokens = [&] {
+      look_up(first);
+      k_first = find(first);
+      if (k_first < last) step_first = fetch(k_first);
+    };
+    if constexpr (kOther) begin_tokens();
+    Q q;
+    q.shared = shared.queries;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 16 * n + n_lane;
+      const uint32_t row = row0 + min(r, rows - 1);
+      const uint32_t token = row / static_cast<uint32_t>(a.group);
+      const int h = head * a.group + static_cast<int>(row - token * a.group);
+      const Sees sees = row_sees<SEEN>(a, req, static_cast<int>(token), r < rows);
+      sight.last[n] = sees.last, sight.after[n] = sees.after, sight.number[n] = sees.number;
+      const T *src = static_cast<const T *>(a.query) + (req.first_row + token) * a.query_token + h * a.query_head +
+                     g * (DIM / 4);
+      constexpr int kSteps = DIM / 32;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (Q::kShared && ((n * kSteps + i) & 3) != wave) continue;  // the waves fill LDS together
+        u32x4 y, z;
+        query_fragment<T>(src + 8 * i, r < rows, flip, y, z);
+        if constexpr (Q::kShared) {
+          shared.queries[(n * kSteps + i) * kWave + lane] = y;
+          if constexpr (kParts == 2) shared.queries[((NT + n) * kSteps + i) * kWave + lane] = z;
+        } else {
+          q.own[n * kSteps + i] = y;
+          if constexpr (kParts == 2) q.own[(NT + n) * kSteps + i] = z;
+        }
+      }
+    }
+    if constexpr (Q::kShared) __syncthreads();
     bool wild = false, waiting = true, far = false;
     RowState<DIM, NT> st;
 #pragma unroll
@@ -209,10 +221,10 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
 #pragma unroll
         for (int i = 0; i < DIM / 16; ++i) st.acc[n][i] = f32x4{0, 0, 0, 0};
       }
-      look_up(first);
-      int k = find(first);
+      if (!kOther || pass != kFirst) begin_tokens();
+      int k = k_first;
       if (k >= last) return false;
-      Step next = fetch(k);
+      Step next = step_first;
       bool more, again = false;
       do {
         const Step now = next;
@@ -242,10 +254,10 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
     for (int pass = kFirst; pass <= kRaised && again && !far; ++pass) again = go(std::true_type{}, pass);
     if (again)
       for (int pass = kMaximum; pass <= kRounded; ++pass) go(std::false_type{}, pass);
-    u = u_item + last;
+    u = u_item + (alone ? 1 : last);
 
     // The four waves' states, 16 rows at a time, into the result or into a part.
-    const bool begins = u_item >= u_begin, ends = last == span.units;
+    const bool begins = u_item >= u_begin, ends = alone || last == span.units;
     const int64_t slot = 2 * wg + (begins ? 1 : 0);
     const bool any_wild = __syncthreads_or(wild);
 #pragma unroll
@@ -347,6 +359,7 @@ template <typename T, int BITS, int SEEN, int DIM, int NT>
 void launch_few(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipStream_t stream) {
   hipLaunchKernelGGL((page_attention_kernel<T, BITS, SEEN, DIM, NT>), dim3(groups), dim3(256), 0, stream, a, s.parts, s.stats,
                      s.records);
+  if (a.alone) return;
   // a workgroup of the join for each row, as far as 512 go
   const unsigned rows = static_cast<unsigned>(std::min<int64_t>(a.tokens * a.heads, 512));
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, 16 * NT>), dim3(rows), dim3(256), 0, stream, a, s.parts, s.stats,

@@ -251,8 +251,9 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     const int wave_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0 + r_first))), wave_after = same(after(r_last));
     const int item_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0))), item_after = same(after(rows - 1));
     const int32_t *table = a.table + b * a.table_stride;
-    const int first = same(static_cast<int>(u - u_item)) * kSub;
-    const int last = same(static_cast<int>(min(u_item + span.units, u_end) - u_item)) * kSub;
+    const bool alone = (BITS == 8 || SEEN != SHMT_SEEN_CAUSAL) && a.alone;
+    const int first = alone ? 0 : same(static_cast<int>(u - u_item)) * kSub;
+    const int last = (alone ? span.tiles : same(static_cast<int>(min(u_item + span.units, u_end) - u_item))) * kSub;
 
     auto token_of = [&](int t) { return unit_token(span, t / kSub) + t % kSub * kTile; };  // of the item's tile t
     // Where the next tiles' tokens lie, 16 tokens a lane, and of which of them any row sees any.
@@ -489,10 +490,10 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       if (threadIdx.x == 0) again_at[0] = again_at[1] = 0;
       pass = pass == kFirst && same(far_any) == 0 ? kRaised : std::max<int>(pass + 1, kMaximum);
     }
-    u = u_item + last / kSub;
+    u = u_item + (alone ? 1 : last / kSub);
 
     // Each wave's rows into the result or into a part.
-    const bool begins = u_item >= u_begin, ends = last == span.units * kSub;
+    const bool begins = u_item >= u_begin, ends = alone || last == span.units * kSub;
     const int64_t slot = 2 * wg + (begins ? 1 : 0);
     const bool add_wild = same(wild_any) != 0;
 #pragma unroll
@@ -576,6 +577,7 @@ void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipSt
   }
   hipLaunchKernelGGL((page_attention_many_kernel<T, BITS, SEEN, DIM>), dim3(groups), dim3(ManyShape<BITS, DIM>::kThreads), 0,
                      stream, a, items, s.count, s.parts, s.stats, s.records);
+  if (a.alone) return;
   hipLaunchKernelGGL((page_attention_join_kernel<T, DIM, many_rows(DIM)>), dim3(2048), dim3(256), 0, stream, a,
                      s.parts, s.stats, s.records, static_cast<int>(groups));
 }

@@ -126,14 +126,14 @@ def test_windows_whose_first_tokens_are_nodes(capi, bits):
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_a_chain_is_the_causal_rule(capi, dim):
-    """The same bits as without a tree, in both kernels and with windows."""
+    """With a tree that is a chain and without one, in both kernels and with windows: the same sums, though in other parts."""
     for q in (1, 7, 150):
         b = Batch(q + dim, [500, 260, 150], [q, q, q], 8, 2, dim, 16, torch.bfloat16, 4, "tree", kinds=("chain",))
         for kw in ({}, dict(window=90, sinks=3)):
-            got = capi.page_attention(*b.args(), b.scale, max_query_len=q, **b.rule(capi), **kw)
-            want = capi.page_attention(*b.args(), b.scale, max_query_len=q, **kw)
-            # units that a tree has to mask are whole in a chain; sums are the same
-            assert torch.equal(got, want)
+            want = b.want(**kw)
+            for rule in (b.rule(capi), {}):
+                got, lse = capi.page_attention(*b.args(), b.scale, max_query_len=q, return_lse=True, **rule, **kw)
+                _close(got, lse, want, torch.bfloat16, dim)
 
 
 @pytest.mark.parametrize("bits, seen", RULES)
