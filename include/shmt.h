@@ -1,7 +1,7 @@
 /*
  * shmt.h — C ABI of libshmt.so: the GPU-cache hot path of ShmTensor
  * (static hashmap, cached feature fetch/set, cached neighbour sampling,
- * relabel, scan) and a paged key/value cache held in 4 bits (plan, set, fetch,
+ * relabel, scan) and a paged key/value cache held in 4 or 8 bits (plan, set, fetch,
  * attention) as hand-written HIP for gfx950 (MI355X).
  *
  * Conventions
@@ -720,8 +720,9 @@ int shmt_page_fetch(const shmt_paged_cache *cache, const void *slots,
  * bits a value is a float of 8 bits (sign, 4 exponent bits, 3 mantissa bits,
  * no infinities, 2^-9 .. 448 in size):
  *   cache   uint8 [pages][kv_heads][2][page][dim]
- * and the power of two of 32 values the smallest with max |x| < 464 * 2^e. All
- * else is as in 4 bits. A cache is written and read with one number of bits.  */
+ * and the power of two of 32 values the smallest with max |x| < 464 * 2^e. The
+ * codes 127 and 255 are not numbers and are never written. All else is as in 4
+ * bits. A cache is written and read with one number of bits.                 */
 int shmt_page_set_as(const shmt_paged_cache *cache, int bits,
                      const void *slots, int slot_bytes, int64_t n,
                      const void *keys, int64_t key_token_stride,
@@ -744,8 +745,8 @@ int shmt_page_fetch_as(const shmt_paged_cache *cache, int bits,
  *   the nodes of its subtree, itself among them; its depth;
  *   the least depth from this node to the request's last one.
  * Rows of no request get -1. nodes: int32 [tokens][4], on 16 bytes. A tree is
- * as large as it likes to be; those of up to 64 nodes, and chains, are the
- * quick ones. query_starts must not descend; starts and kv_lens are len_bytes in
+ * as large as it likes to be (tokens < 2^30 in all); those of up to 64 nodes,
+ * and chains, are the quick ones. query_starts must not descend; starts and kv_lens are len_bytes in
  * {4,8} wide.                                                               */
 int shmt_page_tree(const int32_t *parents, const void *query_starts,
                    const void *kv_lens, int len_bytes, int64_t requests,
@@ -831,6 +832,8 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query,
  *   SHMT_SEEN_ALL     every row sees all kv_lens[b] tokens (an encoder's states,
  *     which are as many as they are, however many rows look at them); no window.
  * nodes: int32 [tokens][4] on 16 bytes, not read unless trees are asked for.
+ * In 8 bits a value that is seen must be a number by its code (those that
+ * shmt_page_set_as writes are); what no row sees may be anything there too.
  * scratch: shmt_page_attention_as_scratch_bytes(...) bytes.                  */
 #define SHMT_SEEN_CAUSAL 0
 #define SHMT_SEEN_TREE 1

@@ -387,7 +387,7 @@ extern "C" {
 
 int shmt_page_tree(const int32_t *parents, const void *query_starts, const void *kv_lens, int len_bytes, int64_t requests,
                    int64_t tokens, int32_t *nodes, int32_t *positions, void *stream) {
-  SHMT_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31), "the number of nodes must be in [0, 2^31)");
+  SHMT_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 30), "the number of nodes must be in [0, 2^30)");
   SHMT_REQUIRE(requests >= 0 && requests < (int64_t{1} << 31), "the number of requests must be in [0, 2^31)");
   SHMT_REQUIRE(width_ok(len_bytes), "query_starts and kv_lens can only be int32 or int64");
   if (tokens == 0) return SHMT_OK;
@@ -413,7 +413,7 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers, int6
   const int64_t values = int64_t{cache->kv_heads} * 2 * cache->page * cache->dim;  // of a page
   SHMT_REQUIRE(layers <= 1 || cache->pages == 0 || (cache_layer_stride >= values * bits / 8 && scales_layer_stride >= values / 32),
                "layers overlap");
-  SHMT_REQUIRE(rows >= 0 && rows < (int64_t{1} << 31), "the number of nodes must be in [0, 2^31)");
+  SHMT_REQUIRE(rows >= 0 && rows < (int64_t{1} << 30), "the number of nodes must be in [0, 2^30)");
   SHMT_REQUIRE(requests >= 0 && requests < (int64_t{1} << 31), "the number of requests must be in [0, 2^31)");
   SHMT_REQUIRE(width >= 0 && width <= (int64_t{1} << 30) / cache->page,
                "the block table holds too many tokens: more than 2^30 a request");

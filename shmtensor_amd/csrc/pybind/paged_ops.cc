@@ -272,7 +272,7 @@ std::vector<torch::Tensor> page_tree(torch::Tensor parents, torch::Tensor query_
   kv_lens = cuda_ids(kv_lens, "kv_lens");
   const int64_t n = check_lengths(query_starts, kv_lens), tokens = parents.numel();
   TORCH_CHECK(query_starts.device() == parents.device(), "all tensors must be on one device");
-  TORCH_CHECK(tokens < (int64_t{1} << 31), "there must be less than 2^31 nodes");
+  TORCH_CHECK(tokens < (int64_t{1} << 30), "there must be less than 2^30 nodes");
   torch::Tensor nodes = new_tensor({tokens, 4}, torch::kInt32, parents), positions = new_tensor({tokens}, torch::kInt32, parents);
   check(shmt_page_tree(parents.data_ptr<int32_t>(), query_starts.data_ptr(), kv_lens.data_ptr(),
                        static_cast<int>(kv_lens.element_size()), n, tokens, nodes.data_ptr<int32_t>(),

@@ -1,7 +1,7 @@
 """Mirror of the reference's `shmtensor` Python package
 (python/shmtensor/__init__.py:1-4): host tensor providers and the GPU
 sampling dataloader on top of the `ShmTensorLib` operators. PagedCache (a key/value
-cache in pages, 4 bits a value) has no counterpart there."""
+cache in pages, 4 or 8 bits a value) has no counterpart there."""
 from .. import install_aliases as _install_aliases
 
 capi = _install_aliases()

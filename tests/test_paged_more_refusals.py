@@ -23,8 +23,8 @@ def test_page_tree(cabi):
         a.update(kw)
         rc = cabi.load().shmt_page_tree(*a.values(), None)
         _refused(cabi, rc, text)
-    call("in [0, 2^31)", tokens=-1)
-    call("in [0, 2^31)", tokens=1 << 31)
+    call("in [0, 2^30)", tokens=-1)
+    call("in [0, 2^30)", tokens=1 << 30)
     call("in [0, 2^31)", requests=-1)
     call("int32 or int64", len_bytes=2)
     call("null", parents=None)
@@ -51,7 +51,7 @@ def test_page_keep(cabi):
     call("layer has to begin", cl=(16 << 20) + 8)
     call("layers overlap", cl=16)
     call("layers overlap", sl=0)
-    call("in [0, 2^31)", rows=-2)
+    call("in [0, 2^30)", rows=-2)
     call("in [0, 2^31)", requests=1 << 31)
     call("too many requests", requests=1 << 26)
     call("too many tokens", width=1 << 30)
