@@ -821,8 +821,10 @@ struct AttnScratch {
 // How many rows an item has, and how many workgroups share the units: as many as the card holds at once.
 struct AttnShape {
   bool many;       // rows: 32 a wave instead of 16 or 32 a workgroup
+  bool alone;      // an item is one workgroup's own
   int rows;        // of an item
   int64_t groups;  // workgroups
+  int64_t room_rows, room_groups;  // room for parts and records, whichever items are chosen
   int64_t items;   // many: room in the list
   int64_t parts_bytes, stats_bytes, record_bytes, item_bytes, first_bytes;
   int64_t bytes() const { return parts_bytes + stats_bytes + record_bytes + item_bytes + first_bytes; }

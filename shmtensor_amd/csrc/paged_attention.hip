@@ -8,8 +8,17 @@ namespace shmt {
 
 // ---- launch ------------------------------------------------------------------------
 
+// Up to how many tokens, as far as the table has room for them, an item is one workgroup's own. Nothing is joined then, which
+// spares a launch and the parts, but an item's tiles come one after the other. us, dealt out and alone, 8 heads of 4 query heads:
+// few rows, 128 dimensions, one request of 256 / 512 / 1,024 tokens, 4 rows: 13.5 and 10.0 / 13.5 and 11.7 / 13.7 and 15.0; 64
+// requests, 32 rows: 19.7 and 16.9 / 24.3 and 21.7; 256 dimensions in 8 bits, one request, 32 rows: 22.6 and 20.9 / 22.7 and 25.8.
+// Many rows, one request, 256 rows of 256 / 512 tokens: 24.2 and 20.7 / 26.4 and 27.5; 8 requests: 36.5 and 22.7 / 40.5 and 29.4.
+// Chains in 4 bits are always dealt out, and keep their results.
+constexpr int alone_tokens(bool many, int dim) { return many || dim == 256 ? 256 : 512; }
+
+// `limit`: the tokens that a row of the table has room for; -1: not known, room for all that may be chosen.
 inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, int seen, int dim, int elem_type, int64_t requests,
-                            int64_t max_query_len) {
+                            int64_t max_query_len, int64_t limit) {
   const int64_t longest = max_query_len > 0 ? std::min(max_query_len, tokens) : std::max<int64_t>(tokens - requests + 1, 1);
   const int64_t group = heads / kv_heads, rows = longest * group;
   AttnShape s;
@@ -33,25 +42,29 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   if (rest > 0 && rest <= many_rows(dim) / 2 && (bits == 8 || seen != SHMT_SEEN_CAUSAL))
     last = dim == 256 ? 1 + f16 : f16 ? 4 : bits == 8 && dim == 128 ? 2 : 3;
   s.many = rows > 2 * many_rows(dim) || (few_items > worth * whole + last && tokens * group * kv_heads >= 16384);
+  const bool other = bits == 8 || seen != SHMT_SEEN_CAUSAL;  // than chains in 4 bits
+  auto few_groups = [&](int rows_of_item) { return int64_t{256} * attn_waves(bits, seen, f16, dim, rows_of_item / 16); };
+  s.alone = other && limit >= 0 && limit <= alone_tokens(s.many, dim);
   s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;
-  s.groups = s.many ? attn_many_groups() : 256 * attn_waves(bits, seen, f16, dim, s.rows / 16);
+  s.groups = s.many ? attn_many_groups() : few_groups(s.rows);
+  s.room_rows = s.groups * s.rows;
+  s.room_groups = s.groups;
+  // 16 rows at a time where that leaves no workgroup more than one unit: one request of 912 tokens, 36 rows, 15.0 us instead of
+  // 17.4; alone, 256 tokens, 32 rows: 10.9 us instead of 13.7.
+  if (other && !s.many && s.rows == 32) {
+    const int64_t groups = few_groups(16), items = requests * kv_heads * ((rows + 15) / 16);
+    s.room_rows = std::max(s.room_rows, groups * 16), s.room_groups = std::max(s.room_groups, groups);
+    if (limit >= 0 && items <= groups / (s.alone ? 1 : limit / kUnit + 1 + item_cost(16))) s.rows = 16, s.groups = groups;
+  }
   s.items = s.many ? tokens * group / s.rows + requests : 0;
-  const int64_t lines = 2 * s.groups * s.rows;
+  const int64_t lines = 2 * s.room_rows;
   s.parts_bytes = lines * dim * 4;
   s.stats_bytes = lines * 8;
-  s.record_bytes = s.groups * static_cast<int64_t>(sizeof(JoinRecord));
+  s.record_bytes = s.room_groups * static_cast<int64_t>(sizeof(JoinRecord));
   s.item_bytes = s.items ? (s.items + 2) * static_cast<int64_t>(sizeof(AttnItem)) : 0;  // the count behind the last one
   s.first_bytes = s.items ? (requests + 4) / 4 * 16 : 0;
   return s;
 }
-
-// Up to how many tokens, as far as the table has room for them, an item is one workgroup's own. Nothing is joined then, which
-// spares a launch and the parts, but an item's tiles come one after the other. us, dealt out and alone, 8 heads of 4 query heads:
-// few rows, 128 dimensions, one request of 256 / 512 / 1,024 tokens, 4 rows: 13.5 and 10.0 / 13.5 and 11.7 / 13.7 and 15.0; 64
-// requests, 32 rows: 19.7 and 16.9 / 24.3 and 21.7; 256 dimensions in 8 bits, one request, 32 rows: 22.6 and 20.9 / 22.7 and 25.8.
-// Many rows, one request, 256 rows of 256 / 512 tokens: 24.2 and 20.7 / 26.4 and 27.5; 8 requests: 36.5 and 22.7 / 40.5 and 29.4.
-// Chains in 4 bits are always dealt out, and keep their results.
-constexpr int alone_tokens(bool many, int dim) { return many || dim == 256 ? 256 : 512; }
 
 void launch_attention(AttnArgs a, int bits, int seen, int dim, int elem_type, const AttnShape &shape, void *scratch,
                       hipStream_t stream) {
@@ -64,7 +77,7 @@ void launch_attention(AttnArgs a, int bits, int seen, int dim, int elem_type, co
   s.count = reinterpret_cast<int32_t *>(s.items + shape.items + 1);
   s.first_item = reinterpret_cast<int32_t *>(at += shape.item_bytes);
   s.room = shape.items;
-  a.alone = (bits == 8 || seen != SHMT_SEEN_CAUSAL) && a.limit <= alone_tokens(shape.many, dim);
+  a.alone = shape.alone;
   // no more workgroups than there can be units
   const int64_t units = (a.tokens * a.group / shape.rows + a.requests) * a.v.kv_heads *
                         (a.alone ? 1 : a.limit / kUnit + 1 + item_cost(shape.rows));
@@ -96,7 +109,7 @@ int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads, int kv_h
     set_error("bad arguments for the attention's scratch size");
     return -1;
   }
-  return attn_shape(tokens, heads, kv_heads, bits, seen, dim, elem_type, requests, max_query_len).bytes();
+  return attn_shape(tokens, heads, kv_heads, bits, seen, dim, elem_type, requests, max_query_len, -1).bytes();
 }
 
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads, int kv_heads, int dim, int elem_type,
@@ -147,7 +160,8 @@ int shmt_page_attention_as(const shmt_paged_cache *cache, int bits, int seen, co
   SHMT_REQUIRE((reinterpret_cast<int64_t>(out) & 15) == 0, "out has to begin on 16 bytes");
   SHMT_REQUIRE(seen != SHMT_SEEN_TREE || (nodes && (reinterpret_cast<int64_t>(nodes) & 15) == 0),
                "nodes is null or does not begin on 16 bytes");
-  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, bits, seen, cache->dim, elem_type, requests, max_query_len);
+  const AttnShape shape = attn_shape(tokens, heads, cache->kv_heads, bits, seen, cache->dim, elem_type, requests, max_query_len,
+                                     v.pages > 0 ? width * cache->page : 0);
   if (scratch_bytes < shape.bytes() || !scratch) {
     set_error("scratch too small: %lld bytes, needed %lld", static_cast<long long>(scratch_bytes),
               static_cast<long long>(shape.bytes()));
