@@ -713,6 +713,17 @@ __device__ __forceinline__ void add_left_out(const AttnArgs &a, int head, int at
   }
 }
 
+// Where a part holds dimensions 4 p .. 4 p + 3 of a row. Many rows: as the lanes of a wave have them, so that 64 of them write a
+// kilobyte at a time; a row's are then pieces of 64 bytes.
+template <int DIM, int ROWS>
+__device__ __forceinline__ int64_t part_at(int64_t row, int p) {
+  if constexpr (ROWS > 32) {
+    const int64_t r = row & 15;
+    return (row & ~int64_t{15}) * DIM + (p % (DIM / 16) * 64 + r * 4 + p / (DIM / 16)) * 4;
+  }
+  return row * DIM + p * 4;
+}
+
 // Puts the parts of the items together that more than one workgroup had a share in. Every workgroup makes itself a list of the
 // rows to join (a grid that has a workgroup for each row that there could be takes longer to start than to run). Where they
 // are few, a workgroup takes one at a time, its teams of DIM / 4 threads a part each; else every team takes a row.
@@ -768,7 +779,7 @@ __global__ __launch_bounds__(256) void page_attention_join_kernel(AttnArgs a, co
           const int64_t w = min(w0 + i * stride, w_end);
           const int64_t line = (2 * w + (w == rec.first ? 1 : 0)) * ROWS + r;
           stats[i] = *reinterpret_cast<const f32x2 *>(part_stats + line * 2);
-          o[i] = *reinterpret_cast<const f32x4 *>(parts + line * DIM + lane * 4);
+          o[i] = *reinterpret_cast<const f32x4 *>(parts + part_at<DIM, ROWS>(line, lane));
         }
         float next = top;
 #pragma unroll
@@ -833,10 +844,10 @@ struct AttnShape {
 constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
 // Waves per SIMD that the registers of the kernel for few rows are meant for. Trees and 8 bits take more registers, and fewer waves
-// that spill none are quicker (and leave fewer parts); so are they for an encoder's states. us with one wave more a SIMD and as it is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in
-// 4 bits, 64 dimensions bfloat16 36 and 30, 128 dimensions 40 and 35, float16 46 and 36; in 8 bits, 64 dimensions float16 43 and
-// 34, 128 dimensions 66 and 54, 256 dimensions 141 and 114 (bfloat16 115 with one wave, 119 with two, but 59 and 57 where
-// requests are short); 32 rows of 256 dimensions 144 and 116.
+// that spill none are quicker (and leave fewer parts); so are they for an encoder's states. us with one wave more a SIMD and as it
+// is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in 4 bits, 64 dimensions bfloat16 36 and 30, 128 dimensions 40 and 35,
+// float16 46 and 36; in 8 bits, 64 dimensions float16 43 and 34, 128 dimensions 66 and 54, 256 dimensions 141 and 114 (bfloat16
+// 115 with one wave, 119 with two, but 59 and 57 where requests are short); 32 rows of 256 dimensions 144 and 116.
 constexpr int attn_waves(int bits, int seen, bool f16, int dim, int tiles) {
   if (bits == 8 || seen != SHMT_SEEN_CAUSAL) return dim == 256 ? (tiles == 1 && !f16 ? 2 : 1) : tiles * dim <= 64 ? 3 : 2;
   return tiles * dim <= 64 ? 4 : tiles * dim <= 128 ? 3 : 2;

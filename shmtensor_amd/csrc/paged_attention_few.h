@@ -94,7 +94,25 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
   const float scale2 = powers_of_two(a);
   const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
   const LaneOffsets offsets = lane_offsets<BITS, DIM>(lane, 1 << a.v.log2_page);
-  for (int64_t u = u_begin; u < u_end;) {
+  auto next_item = [&] {
+    row0 += kRows;
+    if (row0 >= req.queries * a.group) {
+      row0 = 0;
+      if (++head == kv_heads) {
+        head = 0;
+        do req = same(attn_request<SEEN>(a, ++b)); while (req.queries == 0);
+      }
+    }
+    span = same(attn_span<SEEN, kRows>(a, req, row0));
+  };
+  int64_t u = u_begin;
+  // Of what others have begun, units without tokens may be left, and are nobody's part. (Chains in 4 bits make it one.)
+  if (kOther && u - u_item >= span.tiles) {
+    u = u_item += span.units;
+    if (u >= u_end) return;
+    next_item();
+  }
+  while (u < u_end) {
     const int rows = min(kRows, req.queries * a.group - row0);
     Sight<NT> sight;
     sight.sinks = a.window > 0 ? a.sinks : 0;
@@ -139,7 +157,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
       return k;
     };
     // In 4 bits the next tile waits in registers of its own. In 8 those would be too many: the next keys are loaded into the place of
-    // the present ones when these have been multiplied, the next values likewise, and three waves a SIMD have enough in flight.
+    // the present ones when these have been multiplied, the next values likewise, and two or three waves a SIMD have enough in flight.
     constexpr bool kInPlace = BITS == 8;
     KvTile<BITS, DIM> ahead;
     auto fetch_keys = [&](int k) {
@@ -257,7 +275,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
     u = u_item + (alone ? 1 : last);
 
     // The four waves' states, 16 rows at a time, into the result or into a part.
-    const bool begins = u_item >= u_begin, ends = alone || last == span.units;
+    const bool begins = u_item >= u_begin, ends = alone || last >= (kOther ? span.tiles : span.units);
     const int64_t slot = 2 * wg + (begins ? 1 : 0);
     const bool any_wild = __syncthreads_or(wild);
 #pragma unroll
@@ -343,15 +361,7 @@ __global__ __launch_bounds__(256, (attn_waves(BITS, SEEN, std::is_same<T, _Float
     if (u >= u_end) break;
     // the next item
     u_item = u;
-    row0 += kRows;
-    if (row0 >= req.queries * a.group) {
-      row0 = 0;
-      if (++head == kv_heads) {
-        head = 0;
-        do req = same(attn_request<SEEN>(a, ++b)); while (req.queries == 0);
-      }
-    }
-    span = same(attn_span<SEEN, kRows>(a, req, row0));
+    next_item();
   }
 }
 

@@ -106,6 +106,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
   constexpr int kRows = Shape::kRows, NT = Shape::NT, kSteps = DIM / 32, kTile = Shape::kTile, kHalves = Shape::kHalves;
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
   constexpr int kSub = kUnit / kTile;  // tiles of a unit
+  constexpr bool kOther = BITS == 8 || SEEN != SHMT_SEEN_CAUSAL;  // than chains in 4 bits
   __shared__ ManyStage<BITS, DIM> stage[2];
   __shared__ Found found;
   __shared__ uint64_t scan[Shape::kWaves];
@@ -222,7 +223,26 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       (page + 4 * g) * (DIM * BITS / 8) + n_lane * (DIM * BITS / 128) + (BITS == 8 ? value_dim0 : value_word * 4);
   const uint32_t value_scale_at = (DIM / 32 + n_lane * (DIM / 16) / 32) * page + 4 * g;
 
-  for (int64_t u = u_begin; u < u_end;) {
+  auto next_item = [&] {
+    row0 += kRows;
+    if (row0 >= req.queries * a.group) {
+      row0 = 0;
+      do {
+        if (++b == a.requests) b = 0, ++head;
+        req = same(attn_request<SEEN>(a, b));
+      } while (req.queries == 0);
+    }
+  };
+  int64_t u = u_begin;
+  if constexpr (kOther) {  // of what others have begun, units without tokens may be left, and are nobody's part
+    const Span span = same(attn_span<SEEN, kRows>(a, req, row0));
+    if (u - u_item >= span.tiles) {
+      u = u_item += span.units;
+      if (u >= u_end) return;
+      next_item();
+    }
+  }
+  while (u < u_end) {
     const Span span = same(attn_span<SEEN, kRows>(a, req, row0));
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
@@ -243,7 +263,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     // Waves without a row only decode: of up to 128 rows the first four multiply, one on each SIMD. (16 rows to a wave in turn, so
     // that the SIMDs share what there is, brought 8 % for 160 and 192 rows of bfloat16 and lost 5 to 9 % for 128 and 256; chains
     // in 4 bits lose 2 % by the question itself, two prompts 1,071 us instead of 1,050.)
-    const bool has_rows = (BITS == 4 && SEEN == SHMT_SEEN_CAUSAL) || 16 * wave * NT < rows;
+    const bool has_rows = !kOther || 16 * wave * NT < rows;
     // the first and the last place of the wave's rows, and of the item's
     const int r_first = min(16 * wave * NT, rows - 1), r_last = min(16 * (wave + 1) * NT - 1, rows - 1);
     auto place = [&](int r) { return place_of<SEEN>(req, row_token(a, row0 + r)); };
@@ -251,7 +271,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     const int wave_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0 + r_first))), wave_after = same(after(r_last));
     const int item_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0))), item_after = same(after(rows - 1));
     const int32_t *table = a.table + b * a.table_stride;
-    const bool alone = (BITS == 8 || SEEN != SHMT_SEEN_CAUSAL) && a.alone;
+    const bool alone = kOther && a.alone;
     const int first = alone ? 0 : same(static_cast<int>(u - u_item)) * kSub;
     const int last = (alone ? span.tiles : same(static_cast<int>(min(u_item + span.units, u_end) - u_item))) * kSub;
 
@@ -493,7 +513,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     u = u_item + (alone ? 1 : last / kSub);
 
     // Each wave's rows into the result or into a part.
-    const bool begins = u_item >= u_begin, ends = alone || last == span.units * kSub;
+    const bool begins = u_item >= u_begin, ends = alone || last >= (kOther ? span.tiles : span.units) * kSub;
     const int64_t slot = 2 * wg + (begins ? 1 : 0);
     const bool add_wild = same(wild_any) != 0;
 #pragma unroll
@@ -535,7 +555,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
                 out_vec{static_cast<T>(o[i][0] * inv), static_cast<T>(o[i][1] * inv), static_cast<T>(o[i][2] * inv),
                         static_cast<T>(o[i][3] * inv)};
           } else {
-            *reinterpret_cast<f32x4 *>(parts + (slot * kRows + r) * DIM + d0 + 4 * i) = o[i];
+            *reinterpret_cast<f32x4 *>(parts + part_at<DIM, kRows>(slot * kRows + r, (4 * g + r4) * (DIM / 64) + i)) = o[i];
           }
         }
       }
@@ -555,14 +575,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     if (u >= u_end) break;
     // the next item
     u_item = u;
-    row0 += kRows;
-    if (row0 >= req.queries * a.group) {
-      row0 = 0;
-      do {
-        if (++b == a.requests) b = 0, ++head;
-        req = same(attn_request<SEEN>(a, b));
-      } while (req.queries == 0);
-    }
+    next_item();
   }
 }
 
