@@ -47,6 +47,11 @@ constexpr float kLowest = -3.40282347e38f;  // the lowest float, subtracted inst
 // the sake of even shares.
 constexpr int item_cost(int rows) { return rows > 32 ? 2 : 1; }
 
+// Many rows, but for chains in 4 bits (FINE): units of a quarter of kUnit, of which items of up to half the rows, which half the
+// waves multiply, have three for kUnit tokens (128 dimensions in bfloat16: 3.0 us instead of 3.9), so that shares are even in time.
+// 40 trees of 24 to 64 tokens, four heads to one of the cache's: 234 us instead of 238.
+constexpr int kFineUnits = 4;
+
 struct AttnItem {
   int64_t unit;  // units of one head in front of it
   int32_t request, row0;
@@ -66,6 +71,7 @@ struct Span {
   int32_t tile0;       // then tiles from here
   int32_t units;       // in the numbering
   int32_t tiles;       // that there are, at least 1
+  int32_t weight;      // units of a tile
   int32_t sink_end;    // tokens [0, sink_end) and [begin, end) are all that any row of the item sees
   int32_t begin, end;
 };
@@ -78,7 +84,7 @@ __device__ __forceinline__ int64_t same(int64_t v) {
 }
 __device__ __forceinline__ Request same(Request r) { return {same(r.first_row), same(r.queries), same(r.before)}; }
 __device__ __forceinline__ Span same(Span s) {
-  return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.tiles), same(s.sink_end), same(s.begin), same(s.end)};
+  return {same(s.sink_tiles), same(s.tile0), same(s.units), same(s.tiles), same(s.weight), same(s.sink_end), same(s.begin), same(s.end)};
 }
 
 template <int SEEN>
@@ -100,7 +106,7 @@ __device__ __forceinline__ int seen_by_all(const AttnArgs &a, const Request &r, 
   return min(SEEN == SHMT_SEEN_TREE ? r.before - 1 : place_of<SEEN>(r, token), a.limit - 1);
 }
 
-template <int SEEN, int ROWS>
+template <int SEEN, int ROWS, bool FINE = false>
 __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, int row0) {
   const int all = r.queries * a.group;
   const int t_first = static_cast<int>(static_cast<uint32_t>(row0) / static_cast<uint32_t>(a.group));
@@ -123,7 +129,8 @@ __device__ __forceinline__ Span attn_span(const AttnArgs &a, const Request &r, i
   s.sink_end = min(a.sinks, s.begin);
   s.sink_tiles = min((s.sink_end + kUnit - 1) / kUnit, s.tile0);
   s.tiles = max(s.sink_tiles + (s.end + kUnit - 1) / kUnit - s.tile0, 1);
-  s.units = a.alone ? 1 : s.tiles + item_cost(ROWS);
+  s.weight = FINE ? kFineUnits - (all - row0 <= ROWS / 2) : 1;
+  s.units = a.alone ? 1 : s.tiles * s.weight + item_cost(ROWS) * (FINE ? kFineUnits : 1);
   return s;
 }
 

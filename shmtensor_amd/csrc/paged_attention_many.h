@@ -8,7 +8,7 @@ namespace shmt {
 // Items of all requests with the units in front of each, for calls in which a request has many row tiles: one workgroup.
 // items[0 .. n) and, behind the last, the number of units; *count = n. (Only starts that descend could make more items than
 // there is room for.)
-template <int SEEN, int ROWS>
+template <int SEEN, int ROWS, bool FINE>
 __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, int32_t *first_item, AttnItem *items,
                                                                     int64_t room, int32_t *count) {
   __shared__ uint64_t lds[16];
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
         if (first_item[mid] <= i) lo = mid; else hi = mid - 1;
       }
       row0 = static_cast<int>(i - first_item[lo]) * ROWS;
-      mine = attn_span<SEEN, ROWS>(a, attn_request<SEEN>(a, lo), row0).units;
+      mine = attn_span<SEEN, ROWS, FINE>(a, attn_request<SEEN>(a, lo), row0).units;
     }
     uint64_t sum;
     const int64_t at = block_exclusive_scan<uint64_t, 1024>(mine, lds, &sum);
@@ -158,14 +158,14 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
         Request r;
         int row0;
         item_of(base + threadIdx.x, &r, &row0);
-        mine = attn_span<SEEN, kRows>(a, r, row0).units;
+        mine = attn_span<SEEN, kRows, kOther>(a, r, row0).units;
       }
       block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all);
       per_head += same(static_cast<int64_t>(all));
     }
   const int64_t U = per_head * a.v.kv_heads;
   // With a unit for everyone, neighbours in the numbering of units are on one XCD: they read the same pages.
-  const int64_t G = min(int64_t{gridDim.x}, U);
+  const int64_t G = min(int64_t{gridDim.x}, kOther && !a.alone ? U / kFineUnits : U);
   const int64_t wg = G == gridDim.x && G % 8 == 0 ? (blockIdx.x & 7) * (G / 8) + (blockIdx.x >> 3) : blockIdx.x;
   if (threadIdx.x == 0) records[wg].first = -1;
   if (wg >= G) return;
@@ -197,7 +197,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       int r0 = 0, lo = 0;
       if (base + threadIdx.x < count) {
         lo = item_of(base + threadIdx.x, &r, &r0);
-        mine = attn_span<SEEN, kRows>(a, r, r0).units;
+        mine = attn_span<SEEN, kRows, kOther>(a, r, r0).units;
       }
       const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all));
       if (at <= x && x < at + static_cast<int64_t>(mine)) found = Found{r, lo, at, r0};
@@ -235,15 +235,15 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
   };
   int64_t u = u_begin;
   if constexpr (kOther) {  // of what others have begun, units without tokens may be left, and are nobody's part
-    const Span span = same(attn_span<SEEN, kRows>(a, req, row0));
-    if (u - u_item >= span.tiles) {
+    const Span span = same(attn_span<SEEN, kRows, kOther>(a, req, row0));
+    if (u - u_item > (span.tiles - 1) * int64_t{span.weight}) {
       u = u_item += span.units;
       if (u >= u_end) return;
       next_item();
     }
   }
   while (u < u_end) {
-    const Span span = same(attn_span<SEEN, kRows>(a, req, row0));
+    const Span span = same(attn_span<SEEN, kRows, kOther>(a, req, row0));
     const int rows = min(kRows, req.queries * a.group - row0);
     u32x4 q[kParts][NT][kSteps];
     int see_last[NT], see_after[NT], see_number[NT];
@@ -272,8 +272,13 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     const int item_first = same(seen_by_all<SEEN>(a, req, row_token(a, row0))), item_after = same(after(rows - 1));
     const int32_t *table = a.table + b * a.table_stride;
     const bool alone = kOther && a.alone;
-    const int first = alone ? 0 : same(static_cast<int>(u - u_item)) * kSub;
-    const int last = (alone ? span.tiles : same(static_cast<int>(min(u_item + span.units, u_end) - u_item))) * kSub;
+    // A tile is the workgroup's that its first unit belongs to.
+    auto tiles_before = [&](int64_t units) {
+      const int n = same(static_cast<int>(units));
+      return kOther ? min((n + span.weight - 1) / span.weight, span.tiles) : n;
+    };
+    const int first = alone ? 0 : tiles_before(u - u_item) * kSub;
+    const int last = (alone ? span.tiles : tiles_before(min(u_item + span.units, u_end) - u_item)) * kSub;
 
     auto token_of = [&](int t) { return unit_token(span, t / kSub) + t % kSub * kTile; };  // of the item's tile t
     // Where the next tiles' tokens lie, 16 tokens a lane, and of which of them any row sees any.
@@ -510,7 +515,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
       if (threadIdx.x == 0) again_at[0] = again_at[1] = 0;
       pass = pass == kFirst && same(far_any) == 0 ? kRaised : std::max<int>(pass + 1, kMaximum);
     }
-    u = u_item + (alone ? 1 : last / kSub);
+    u = kOther ? min(u_item + span.units, u_end) : u_item + last / kSub;
 
     // Each wave's rows into the result or into a part.
     const bool begins = u_item >= u_begin, ends = alone || last >= (kOther ? span.tiles : span.units) * kSub;
@@ -584,7 +589,7 @@ void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipSt
   // A list of items costs a launch; every workgroup counts for itself where that takes no longer, or there is nothing to count.
   const AttnItem *items = nullptr;
   if (a.requests > 256 || (a.requests > 0 && s.room > 1024)) {
-    hipLaunchKernelGGL((page_attention_items_kernel<SEEN, many_rows(DIM)>), dim3(1), dim3(1024), 0, stream, a, s.first_item,
+    hipLaunchKernelGGL((page_attention_items_kernel<SEEN, many_rows(DIM), BITS == 8 || SEEN != SHMT_SEEN_CAUSAL>), dim3(1), dim3(1024), 0, stream, a, s.first_item,
                        s.items, s.room, s.count);
     items = s.items;
   }
