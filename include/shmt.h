@@ -746,7 +746,8 @@ int shmt_page_fetch_as(const shmt_paged_cache *cache, int bits,
  *   the least depth from this node to the request's last one.
  * Rows of no request get -1. nodes: int32 [tokens][4], on 16 bytes. A tree is
  * as large as it likes to be (tokens < 2^30 in all); those of up to 64 nodes,
- * and chains, are the quick ones. query_starts must not descend; starts and kv_lens are len_bytes in
+ * and chains, are the quick ones. query_starts must not descend (requests that
+ * overlap get words without a meaning); starts and kv_lens are len_bytes in
  * {4,8} wide.                                                               */
 int shmt_page_tree(const int32_t *parents, const void *query_starts,
                    const void *kv_lens, int len_bytes, int64_t requests,
@@ -768,9 +769,9 @@ int shmt_page_tree(const int32_t *parents, const void *query_starts,
  * and in each of `layers` caches of one layout (strides between them in bytes;
  * addresses, pages and layers on 16 bytes) the keys and values of the k-th node
  * are copied to the place of node k, codes and scales as they are. Other rows
- * are not touched; where a place or a row has no page, nothing is copied. The request
- * holds kv_lens[b] - n + counts[b] tokens then, at positions without a gap.
- * Requests must not share pages that are written. cache->cache and
+ * are not touched; where a place or a row has no page, nothing is copied. The
+ * request holds kv_lens[b] - n + counts[b] tokens then, at positions without a
+ * gap. Requests must not share pages that are written. cache->cache and
  * cache->scales are the first layer's.                                      */
 int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers,
                    int64_t cache_layer_stride, int64_t scales_layer_stride,

@@ -30,11 +30,12 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   //   256 dimensions: 64 rows 179 and 185, 96 rows 293 and 191; float16 64 rows 193 and 277, 96 rows 312 and 282.
   // So an item costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the card idles
   // behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
-  // Trees and 8 bits: a last item of half the rows or fewer is told apart, as the waves that have none of them only decode. Trees, as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and
-  // 119, 128 rows 129 and 121, 160 rows 169 and 146; 8 bits, 64 rows 87 and 122, 96 rows 137 and 124; float16: 4 bits, 128 rows 141
-  // and 164, 192 rows 216 and 224, 224 rows 251 and 228, 320 rows 344 and 409; 64 dimensions, bfloat16: 96 rows 91 and 90, 128 rows
-  // 104 and 90; 256 dimensions, bfloat16: 64 rows 155 and 157, in 8 bits 175 and 167, 96 rows 240 and 203; float16: 64 rows 187 and
-  // 232, 96 rows 289 and 280, in 8 bits 96 rows 357 and 363, 128 rows 402 and 374.
+  // Trees and 8 bits: a last item of half the rows or fewer is told apart, as the waves that have none of them only decode. Trees,
+  // as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and 119, 128 rows 129 and 121, 160 rows 169 and 146;
+  // 8 bits, 64 rows 87 and 122, 96 rows 137 and 124; float16: 4 bits, 128 rows 141 and 164, 192 rows 216 and 224, 224 rows 251 and
+  // 228, 320 rows 344 and 409; 64 dimensions, bfloat16: 96 rows 91 and 90, 128 rows 104 and 90; 256 dimensions, bfloat16: 64 rows
+  // 155 and 157, in 8 bits 175 and 167, 96 rows 240 and 203; float16: 64 rows 187 and 232, 96 rows 289 and 280, in 8 bits 96 rows
+  // 357 and 363, 128 rows 402 and 374.
   const bool f16 = elem_type == SHMT_F16;
   const int64_t few_items = (rows + 31) / 32, whole = rows / many_rows(dim), rest = rows % many_rows(dim);
   const int64_t worth = dim == 256 ? 2 + (f16 && bits == 8) : f16 ? 6 : 4;
@@ -104,7 +105,8 @@ extern "C" {
 
 int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads, int kv_heads, int bits, int seen, int dim, int elem_type,
                                              int64_t requests, int64_t max_query_len) {
-  if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (bits != 4 && bits != 8) || seen < SHMT_SEEN_CAUSAL || seen > SHMT_SEEN_ALL || (dim != 64 && dim != 128 && dim != 256) ||
+  if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (bits != 4 && bits != 8) ||
+      seen < SHMT_SEEN_CAUSAL || seen > SHMT_SEEN_ALL || (dim != 64 && dim != 128 && dim != 256) ||
       (elem_type != SHMT_F16 && elem_type != SHMT_BF16) || requests < 0 || max_query_len < 0) {
     set_error("bad arguments for the attention's scratch size");
     return -1;
@@ -114,7 +116,8 @@ int64_t shmt_page_attention_as_scratch_bytes(int64_t tokens, int heads, int kv_h
 
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads, int kv_heads, int dim, int elem_type,
                                           int64_t requests, int64_t max_query_len) {
-  return shmt_page_attention_as_scratch_bytes(tokens, heads, kv_heads, 4, SHMT_SEEN_CAUSAL, dim, elem_type, requests, max_query_len);
+  return shmt_page_attention_as_scratch_bytes(tokens, heads, kv_heads, 4, SHMT_SEEN_CAUSAL, dim, elem_type, requests,
+                                              max_query_len);
 }
 
 int shmt_page_attention(const shmt_paged_cache *cache, const void *query, int64_t query_token_stride,

@@ -120,6 +120,11 @@ enum : int { kNumber, kSize, kDepth, kLater };  // kLater: what is below the lat
 // A larger tree, by one wave, 64 nodes at a time: parents lie in front, so sizes come from the last nodes to the first, numbers
 // and depths from the first to the last. What crosses the 64 goes through `m`; until a node's turn comes, its size there is what
 // its children have brought so far, and its number its parent.
+//
+// Requests whose rows overlap, where starts descend, write into each other's words: what is read as a parent is made one again
+// before it is used, so that they reach nobody else's and every loop ends.
+__device__ __forceinline__ int parent_again(int p, int i, int n) { return i < n && p >= 0 && p < i ? p : -1; }
+
 template <typename Memory>
 __device__ void large_tree(const TreeArgs &a, const Request &r, Memory m) {
   const int lane = lane_id(), n = r.queries;
@@ -128,7 +133,7 @@ __device__ void large_tree(const TreeArgs &a, const Request &r, Memory m) {
   m.fence();
   int roots = 0;  // nodes below later roots
   for (int base = last; base >= 0; base -= kWave) {
-    const int i = base + lane, p = i < n ? m.get(i, kNumber) : -1;
+    const int i = base + lane, p = parent_again(i < n ? m.get(i, kNumber) : -1, i, n);
     int size = i < n ? 1 + m.get(i, kSize) : 0, later = p >= 0 ? m.get(p, kSize) : roots;
     give_sizes(p, base, kWave, size, later);
     roots += static_cast<int>(wave_last(wave_inclusive_scan(static_cast<uint32_t>(p < 0 ? size : 0))));
@@ -138,7 +143,7 @@ __device__ void large_tree(const TreeArgs &a, const Request &r, Memory m) {
     m.fence();
   }
   for (int base = 0; base < n; base += kWave) {
-    const int i = base + lane, p = i < n ? m.get(i, kNumber) : -1, near = p >= base ? p - base : -1;
+    const int i = base + lane, p = parent_again(i < n ? m.get(i, kNumber) : -1, i, n), near = p >= base ? p - base : -1;
     int number = 0, depth = 0;
     if (i < n) {
       const int before = (p >= 0 ? m.get(p, kSize) - 1 : n) - m.get(i, kSize) - m.get(i, kLater);

@@ -99,3 +99,16 @@ def test_refusals(capi):
                       (lambda: capi.page_tree(ints(0, 0), ints(0, 2).float(), ints(2).float()), "int")):
         with pytest.raises(RuntimeError, match=text):
             bad()
+
+
+def test_starts_that_descend(capi):
+    """Requests whose rows overlap get words without a meaning, at their own rows only, and the call ends."""
+    rng = np.random.default_rng(11)
+    last = grown(rng, 100, "late")
+    parents = np.concatenate([grown(rng, 2000, "tree"), grown(rng, 500, "star"), last])
+    put = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+    for _ in range(3):
+        nodes, positions = capi.page_tree(put(parents), put([0, 2000, 500, 2500, 2600]), put([2000, 7, 2500, 130]))
+        want = paged_more.tree(last, [0, 100], [130])
+        assert np.array_equal(nodes[2500:].cpu().numpy(), want[0])
+        assert np.array_equal(positions[2500:].cpu().numpy(), want[1])
