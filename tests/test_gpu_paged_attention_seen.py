@@ -167,6 +167,22 @@ def test_work_split_over_long_requests(capi, bits, seen, dtype):
 
 
 @pytest.mark.parametrize("bits, seen", RULES)
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 256)])
+@pytest.mark.parametrize("most, requests", [(7, 70), (260, 25)])
+def test_shares_that_end_anywhere(capi, bits, seen, dtype, dim, most, requests):
+    """Items of all lengths and fillings, so that shares of the work begin and end at every place of an item: within its tokens, at
+    its end, behind it."""
+    rng = np.random.default_rng(dim)
+    lens = rng.integers(0, 900, requests)
+    q = np.minimum(rng.integers(0, most + 1, requests), lens + (1 if seen == "all" else 0))
+    heads, kv_heads = (12, 12) if most == 7 else (8, 4)
+    b = Batch(dim, lens, q, heads, kv_heads, dim, 16, dtype, bits, seen)
+    _check(capi, b)
+    if seen != "all" and most == 7:
+        _check(capi, b, window=300, sinks=20)
+
+
+@pytest.mark.parametrize("bits, seen", RULES)
 @pytest.mark.parametrize("q", [1, 9, 100])
 def test_not_a_number_where_it_is_seen_and_nowhere_else(capi, bits, seen, q):
     for dim in (64, 128, 256):
