@@ -154,16 +154,20 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     *row0 = static_cast<int>(i - first_item[lo]) * kRows;
     return lo;
   };
+  // Of the last kThreads items, which mostly are all: the thread's own, and the units in front of it.
+  Found own{};
+  uint64_t own_units = 0;
   if (!items)
     for (int64_t base = 0; base < count; base += kThreads) {
-      uint64_t mine = 0, all;
+      uint64_t all;
+      own_units = 0;
       if (base + threadIdx.x < count) {
-        Request r;
-        int row0;
-        item_of(base + threadIdx.x, &r, &row0);
-        mine = attn_span<SEEN, kRows, kOther>(a, r, row0).units;
+        int r0;
+        own.request = item_of(base + threadIdx.x, &own.req, &r0);
+        own.units = r0;
+        own_units = attn_span<SEEN, kRows, kOther>(a, own.req, r0).units;
       }
-      block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all);
+      own.before = per_head + static_cast<int64_t>(block_exclusive_scan<uint64_t, kThreads>(own_units, scan, &all));
       per_head += same(static_cast<int64_t>(all));
     }
   const int64_t U = per_head * a.v.kv_heads;
@@ -193,15 +197,14 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     b = same(it.request), row0 = same(it.row0), u_item = head * per_head + same(it.unit);
     req = same(attn_request<SEEN>(a, b));
   } else {
+    if (own.before <= x && x < own.before + static_cast<int64_t>(own_units)) found = own;
     int64_t before = 0;
-    for (int64_t base = 0; base < count; base += kThreads) {
+    for (int64_t base = 0; base + kThreads < count; base += kThreads) {
       uint64_t mine = 0, all;
       Request r{};
       int r0 = 0, lo = 0;
-      if (base + threadIdx.x < count) {
-        lo = item_of(base + threadIdx.x, &r, &r0);
-        mine = attn_span<SEEN, kRows, kOther>(a, r, r0).units;
-      }
+      lo = item_of(base + threadIdx.x, &r, &r0);
+      mine = attn_span<SEEN, kRows, kOther>(a, r, r0).units;
       const int64_t at = before + static_cast<int64_t>(block_exclusive_scan<uint64_t, kThreads>(mine, scan, &all));
       if (at <= x && x < at + static_cast<int64_t>(mine)) found = Found{r, lo, at, r0};
       before += same(static_cast<int64_t>(all));
