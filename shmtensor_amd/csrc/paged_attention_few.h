@@ -10,7 +10,7 @@
 // At 64 dimensions half the bytes come with the same softmax, and the vector units are what it waits for: 96 requests with a
 // window of 4,000 tokens, float16, 66 us, 3.1 TB/s (some 230 vector instructions for 32 tokens of a wave).
 // In 8 bits twice the bytes come with the same softmax: 64 ragged requests as above 143 us, 5.2 TB/s. With more than 16 rows it is
-// issue again: a tree of 65 rows behind 100,000 tokens in 8 bits, float16, 115 us, 363 vector instructions for 32 tokens and 32
+// issue again: a tree of 65 rows behind 100,000 tokens in 8 bits, float16, 120 us, 363 vector instructions for 32 tokens and 32
 // rows of a wave. Over an encoder's states, 80 requests of 300 to 1,500, 5 rows each, 16 heads of 64, 37 us, of which the join 5.
 #pragma once
 #include "paged_attention.h"

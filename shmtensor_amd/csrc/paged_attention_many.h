@@ -71,9 +71,9 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // has room for. They read it twice as often but wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (0.76
 // now, 710 TFLOP/s) against 1.02 with four waves of 32 rows and tiles of 32 tokens and 0.95 with eight and 32; chunks of 17 to
 // 2,000 tokens behind a window 87 us against 95 and 92.
-// Trees of 24 to 64 nodes, four heads to one of the cache's, behind 1,000 to 12,000 tokens, 40 requests: 231 us; what is lost there
+// Trees of 24 to 64 nodes, four heads to one of the cache's, behind 1,000 to 12,000 tokens, 40 requests: 226 us; what is lost there
 // are waves without rows and the ends of items, 8 us each. 6 answers of 100 to 1,200 tokens over an encoder's 700 to 5,000
-// states in 8 bits: 77 us, 43 of them in the tiles.
+// states in 8 bits: 76 us, 43 of them in the tiles.
 template <int BITS, int DIM>
 struct ManyShape {
   static constexpr int kTile = DIM == 256 ? 64 : 128;  // tokens
