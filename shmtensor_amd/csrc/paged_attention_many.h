@@ -154,7 +154,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     *row0 = static_cast<int>(i - first_item[lo]) * kRows;
     return lo;
   };
-  // Of the last kThreads items, which mostly are all: the thread's own, and the units in front of it.
+  // Of the last kThreads items, or fewer, which mostly are all: the thread's own, and the units in front of it.
   Found own{};
   uint64_t own_units = 0;
   if (!items)
@@ -595,8 +595,8 @@ void launch_many(const AttnArgs &a, unsigned groups, const AttnScratch &s, hipSt
   // A list of items costs a launch; every workgroup counts for itself where that takes no longer, or there is nothing to count.
   const AttnItem *items = nullptr;
   if (a.requests > 256 || (a.requests > 0 && s.room > 1024)) {
-    hipLaunchKernelGGL((page_attention_items_kernel<SEEN, many_rows(DIM), BITS == 8 || SEEN != SHMT_SEEN_CAUSAL>), dim3(1), dim3(1024), 0, stream, a, s.first_item,
-                       s.items, s.room, s.count);
+    hipLaunchKernelGGL((page_attention_items_kernel<SEEN, many_rows(DIM), BITS == 8 || SEEN != SHMT_SEEN_CAUSAL>), dim3(1),
+                       dim3(1024), 0, stream, a, s.first_item, s.items, s.room, s.count);
     items = s.items;
   }
   hipLaunchKernelGGL((page_attention_many_kernel<T, BITS, SEEN, DIM>), dim3(groups), dim3(ManyShape<BITS, DIM>::kThreads), 0,

@@ -182,6 +182,13 @@ def test_shares_that_end_anywhere(capi, bits, seen, dtype, dim, most, requests):
         _check(capi, b, window=300, sinks=20)
 
 
+@pytest.mark.parametrize("bits, seen", [(4, "all"), (8, "causal"), (8, "all")])
+@pytest.mark.parametrize("lens, queries", [([300, 40, 270], [4000, 5000, 1500]), ([300, 20], [9000, 9000]), ([30], [11000])])
+def test_more_items_than_threads(capi, bits, seen, lens, queries):
+    """600 and 1,100 items of 256 rows, which a workgroup's threads do not count at once."""
+    _check(capi, Batch(sum(lens), lens, queries, 16, 1, 64, 16, torch.bfloat16, bits, seen))
+
+
 @pytest.mark.parametrize("bits, seen", RULES)
 @pytest.mark.parametrize("q", [1, 9, 100])
 def test_not_a_number_where_it_is_seen_and_nowhere_else(capi, bits, seen, q):
