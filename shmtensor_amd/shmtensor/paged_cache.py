@@ -91,7 +91,7 @@ class PagedCache:
         changes nothing, if there are not enough free pages or a request grows beyond max_len. With parents, one for each new
         token, the requests' new tokens are trees: keep() ends such a step. (An int32 tensor on the GPU; host integers are
         copied there, which waits for what is queued.)"""
-        new = np.array(new_lens, dtype=np.int64)     # a copy: the step and trim() go by it until keep()
+        new = np.asarray(new_lens, dtype=np.int64).copy()    # the step and trim() go by it until keep()
         if new.shape != self.lens.shape or (new < 0).any():
             raise ValueError("new_lens must hold a length >= 0 for each of %d requests" % len(self.lens))
         total = self.lens + new
