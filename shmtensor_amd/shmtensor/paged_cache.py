@@ -104,7 +104,7 @@ class PagedCache:
             parents = torch.as_tensor(parents, dtype=torch.int32)
             if parents.shape != (int(new.sum()),):
                 raise ValueError("parents must hold an entry for each of %d new tokens" % new.sum())
-            parents = parents.to(self._free.device)
+            parents = parents.to(self._free.device, copy=True)    # keep() follows them
         device_new = self._to_device(new)
         starts, kv_lens, positions, slots, _ = capi.page_plan(self._kv_lens, device_new, self.block_table, self._free,
                                                               self.page, int(new.sum()))

@@ -77,3 +77,15 @@ def test_lengths_are_the_callers_own(host_cache):
         counts, _, _ = cache.keep(step, tokens, picked)
         assert counts.tolist() == [2, 5, 1]
         _in_order(cache, [42, 38, 1])
+
+
+def test_parents_are_the_callers_own(host_cache):
+    """So may the tensor of parents: the step keeps what it was planned with."""
+    cache = host_cache()
+    parents = torch.tensor([-1, 0, 1, 2, -1, 0], dtype=torch.int32)
+    step = cache.plan([4, 2, 0], parents=parents)
+    parents.fill_(-1)
+    ones = torch.ones(6, dtype=torch.int64)
+    counts, path, _ = cache.keep(step, ones, ones)
+    assert counts.tolist() == [4, 2, 0] and path.tolist() == [0, 1, 2, 3, 0, 1]
+    _in_order(cache, [4, 2, 0])
