@@ -60,6 +60,8 @@ class PagedCache:
         self.lens = np.zeros(requests, dtype=np.int64)
         self._dropped = [(0, 0)] * requests          # pages [from, to) of a request that trim() gave back
         self._drafted = np.zeros(requests, dtype=np.int64)   # new tokens that keep() may still take back
+        self._open = None                            # the step over trees that keep() may end
+        self._gone = set()                           # requests that were released since it was planned
         self._free = torch.arange(pages, dtype=torch.int32, device=device)
         self._kv_lens = torch.zeros(requests, dtype=torch.int32, device=device)
         # New lengths on their way to the GPU: from memory that is not pinned a copy waits for all that is queued, and so does
@@ -90,7 +92,8 @@ class PagedCache:
         """Pages and slots for new_lens[r] further tokens of every request r (host integers). Raises RuntimeError, and
         changes nothing, if there are not enough free pages or a request grows beyond max_len. With parents, one for each new
         token, the requests' new tokens are trees: keep() ends such a step. (An int32 tensor on the GPU; host integers are
-        copied there, which waits for what is queued.)"""
+        copied there, which waits for what is queued.) A step over trees that is not ended before the next plan() stays whole:
+        its nodes are text from then on, one behind the other."""
         new = np.asarray(new_lens, dtype=np.int64).copy()    # the step and trim() go by it until keep()
         if new.shape != self.lens.shape or (new < 0).any():
             raise ValueError("new_lens must hold a length >= 0 for each of %d requests" % len(self.lens))
@@ -114,7 +117,9 @@ class PagedCache:
         if parents is not None:
             nodes, positions = capi.page_tree(parents, starts, kv_lens)
             self._drafted = new
-        return Step(starts, kv_lens, positions, slots, int(new.max(initial=0)), new, parents, nodes)
+        step = Step(starts, kv_lens, positions, slots, int(new.max(initial=0)), new, parents, nodes)
+        self._open, self._gone = step if parents is not None else None, set()
+        return step
 
     def set(self, step, layer, keys, values):
         """Rounds the step's keys and values [tokens, kv_heads, dim] into the cache."""
@@ -145,19 +150,27 @@ class PagedCache:
         model's choice behind each node) agrees with `tokens`, both [step.tokens] on the GPU; their rows are moved together
         in all layers, the places and pages behind them are free again. given (int32 on the GPU): how many of a request's
         first nodes are no drafts (default 1). Returns (counts, path, token): counts (host integers) nodes of each request
-        that stay; path [step.tokens] their indices, then -1; token [requests] what was picked behind the last of them.
+        that stay; path [step.tokens] their indices, then -1; token [requests] what was picked behind the last of them. Of a
+        request that was released since plan() nothing stays: its count is 0, its path and token are -1.
         Waits for the GPU: the counts are the requests' new lengths."""
         if step.parents is None:
             raise ValueError("the step has no trees: plan() was called without parents")
-        if step.kv_lens is not self._kv_lens:
-            raise ValueError("the step is not the last one that was planned")
+        if step is not self._open:
+            raise ValueError("the step is not the last one that was planned, or it has been ended")
         counts, path, token = capi.page_keep(self.cache, self.scales, self.block_table, step.query_starts, step.kv_lens,
                                              step.parents, tokens, picked, given)
         kept = counts.cpu().numpy().astype(np.int64)
         before = self.lens - step.new
-        held, need = self._pages(self.lens), self._pages(before + kept)
         self._kv_lens = step.kv_lens - (step.query_starts[1:] - step.query_starts[:-1]) + counts
+        ends = np.cumsum(step.new)
+        for r in self._gone:                         # (it has no pages: nothing of it was moved)
+            before[r] = kept[r] = 0
+            self._kv_lens[r:r + 1].zero_()
+            path[int(ends[r] - step.new[r]):int(ends[r])].fill_(-1)
+            token[r:r + 1].fill_(-1)
+        held, need = self._pages(self.lens), self._pages(before + kept)
         self.lens, self._drafted = before + kept, np.zeros_like(kept)
+        self._open, self._gone = None, set()
         spans = [(r, int(need[r]), int(held[r])) for r in np.nonzero(need < held)[0]]
         if spans:
             at = np.concatenate([r * self.block_table.shape[1] + np.arange(a, b) for r, a, b in spans])
@@ -180,7 +193,7 @@ class PagedCache:
             pages.fill_(-1)
 
     def release(self, request):
-        """The request is done; its place is empty again."""
+        """The request is done; its place is empty again, for the next plan() to fill."""
         a, b = self._dropped[request]
         self._give_back(request, 0, a)
         self._give_back(request, b, self._pages(int(self.lens[request])))
@@ -189,6 +202,7 @@ class PagedCache:
         self.lens[request] = 0
         self._drafted = self._drafted.copy()
         self._drafted[request] = 0
+        self._gone.add(request)
         self._kv_lens = self._kv_lens.clone()        # a step that is still in use keeps its own
         self._kv_lens[request:request + 1].zero_()
 

@@ -89,3 +89,45 @@ def test_parents_are_the_callers_own(host_cache):
     counts, path, _ = cache.keep(step, ones, ones)
     assert counts.tolist() == [4, 2, 0] and path.tolist() == [0, 1, 2, 3, 0, 1]
     _in_order(cache, [4, 2, 0])
+
+
+def test_a_request_is_released_while_its_step_runs(host_cache):
+    """Its pages are free at once; the step ends for the others, and keeps nothing of the one that is gone."""
+    for gone in ([1], [0, 2], [0, 1, 2], [1, 1]):
+        cache = host_cache()
+        cache.plan([40, 16, 30])
+        parents = [-1, 0, 0, 2] + [-1, 0, 1] + [-1, 0, 1, 2, 3]
+        step = cache.plan([4, 3, 5], parents=parents)
+        for r in gone:
+            cache.release(r)
+        assert cache.lens.tolist() == [0 if r in gone else n for r, n in enumerate((44, 19, 35))]
+        tokens = torch.tensor([7, 8, 9, 7] + [7, 7, 7] + [1, 2, 3, 4, 5])
+        picked = torch.tensor([9, 5, 7, 6] + [7, 7, 4] + [2, 3, 6, 6, 6])
+        counts, path, token = cache.keep(step, tokens, picked)
+        want = [(3, [0, 2, 3, -1], 6), (3, [0, 1, 2], 4), (3, [0, 1, 2, -1, -1], 6)]
+        want = [(0, [-1] * len(p), -1) if r in gone else (n, p, t) for r, (n, p, t) in enumerate(want)]
+        assert counts.tolist() == [n for n, _, _ in want]
+        assert path.tolist() == sum((p for _, p, _ in want), []) and token.tolist() == [t for _, _, t in want]
+        lens = [0 if r in gone else n for r, n in enumerate((43, 19, 33))]
+        _in_order(cache, lens)
+        with pytest.raises(ValueError, match="not the last one"):
+            cache.keep(step, tokens, picked)
+        step = cache.plan([1, 20, 1])                                   # the places serve on
+        assert step.kv_lens.tolist() == [lens[0] + 1, lens[1] + 20, lens[2] + 1]
+        _in_order(cache, step.kv_lens.tolist())
+
+
+def test_a_step_that_is_never_ended_stays_whole(host_cache):
+    """The next plan() takes all of its nodes for the requests' text."""
+    cache = host_cache()
+    cache.plan([10, 0, 3])
+    step = cache.plan([3, 2, 0], parents=[-1, 0, 0, -1, 0])
+    with pytest.raises(RuntimeError, match="beyond max_len"):
+        cache.plan([150, 150, 150])                                     # refused: the step is still the last one
+    assert cache.keep(step, torch.ones(5, dtype=torch.int64), torch.zeros(5, dtype=torch.int64))[0].tolist() == [1, 1, 0]
+    step = cache.plan([3, 2, 0], parents=[-1, 0, 0, -1, 0])
+    after = cache.plan([1, 1, 1])
+    assert after.positions.tolist() == [14, 3, 3] and after.kv_lens.tolist() == [15, 4, 4]
+    with pytest.raises(ValueError, match="not the last one"):
+        cache.keep(step, torch.ones(5, dtype=torch.int64), torch.ones(5, dtype=torch.int64))
+    _in_order(cache, [15, 4, 4])
