@@ -194,6 +194,7 @@ class PagedCache:
 
     def release(self, request):
         """The request is done; its place is empty again, for the next plan() to fill."""
+        request = range(len(self.lens))[request]
         a, b = self._dropped[request]
         self._give_back(request, 0, a)
         self._give_back(request, b, self._pages(int(self.lens[request])))
@@ -208,6 +209,7 @@ class PagedCache:
 
     def trim(self, request, window, sinks=0):
         """Gives back the pages that no further query of the request can see with this window and these sinks."""
+        request = range(len(self.lens))[request]
         if window <= 0:
             return
         a, b = self._dropped[request]

@@ -131,3 +131,21 @@ def test_a_step_that_is_never_ended_stays_whole(host_cache):
     with pytest.raises(ValueError, match="not the last one"):
         cache.keep(step, torch.ones(5, dtype=torch.int64), torch.ones(5, dtype=torch.int64))
     _in_order(cache, [15, 4, 4])
+
+
+def test_requests_counted_from_the_end(host_cache):
+    """release(-1) and trim(-1) mean the last request, lengths on the GPU included; a request that there is not is refused."""
+    cache = host_cache()
+    cache.plan([40, 16, 100])
+    cache.trim(-1, window=20)
+    assert (cache.block_table[2] >= 0).sum() == 2 and cache._dropped[2] == (0, 5)
+    cache.release(-1)
+    assert cache._kv_lens.tolist() == [40, 16, 0]
+    cache.plan([1, 1, 30])
+    _in_order(cache, [41, 17, 30])
+    for wrong in (3, -4):
+        with pytest.raises(IndexError):
+            cache.release(wrong)
+        with pytest.raises(IndexError):
+            cache.trim(wrong, window=1)
+    _in_order(cache, [41, 17, 30])
