@@ -798,13 +798,14 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers,
  * log(sum_j exp(softmax_scale q . K[j])), with which results over parts of the
  * tokens can be joined. out: contiguous, of query's type. query_starts must
  * not descend; starts and kv_lens are len_bytes in {4,8} wide. max_query_len:
- * the most queries of a request, if known (0: not known): it only chooses the
- * kernel. A row of the table has room for 2^30 tokens at most, and tokens *
+ * the most queries of a request, if known (0: not known): it chooses the kernel
+ * (for few or for many rows), and with it the bits of the weights. A row of the table has room for 2^30 tokens at most, and tokens *
  * heads are below 2^30. scratch: shmt_page_attention_scratch_bytes(...) bytes
  * of device memory, 16-byte aligned, free again when the work queued has run.
  * Sums and the softmax are held in 32 bits; the weights meet the values in 16
- * bits, for many rows of bfloat16 in 8, which may move a result by 2^-16 (2^-8)
- * sum_j w_j |V[j]| besides its own rounding. The same call gives the same bits. softmax_scale q . K[j] log2(e) has to lie within the range of
+ * bits, in the kernel for many rows of bfloat16 in 8, which may move a result by
+ * 2^-16 (2^-8) sum_j w_j |V[j]| besides its own rounding. The same call gives
+ * the same bits. softmax_scale q . K[j] log2(e) has to lie within the range of
  * 32-bit floats. Values of 2^80 and more may overflow where they would not have
  * to. No gradient goes through a cache.                                      */
 int64_t shmt_page_attention_scratch_bytes(int64_t tokens, int heads,
@@ -833,6 +834,8 @@ int shmt_page_attention(const shmt_paged_cache *cache, const void *query,
  *   SHMT_SEEN_ALL     every row sees all kv_lens[b] tokens (an encoder's states,
  *     which are as many as they are, however many rows look at them); no window.
  * nodes: int32 [tokens][4] on 16 bytes, not read unless trees are asked for.
+ * Weights meet the values in 16 bits in both kernels, but for what
+ * shmt_page_attention computes (4 bits, SHMT_SEEN_CAUSAL), which is as there.
  * In 8 bits a value that is seen must be a number by its code (those that
  * shmt_page_set_as writes are); what no row sees may be anything there too.
  * scratch: shmt_page_attention_as_scratch_bytes(...) bytes.                  */

@@ -12,7 +12,8 @@ namespace shmt {
 // spares a launch and the parts, but an item's tiles come one after the other. us, dealt out and alone, 8 heads of 4 query heads:
 // few rows, 128 dimensions, one request of 256 / 512 / 1,024 tokens, 4 rows: 13.5 and 10.0 / 13.5 and 11.7 / 13.7 and 15.0; 64
 // requests, 32 rows: 19.7 and 16.9 / 24.3 and 21.7; 256 dimensions in 8 bits, one request, 32 rows: 22.6 and 20.9 / 22.7 and 25.8.
-// Many rows, one request, 256 rows of 256 / 512 tokens: 24.2 and 20.7 / 26.4 and 27.5; 8 requests: 36.5 and 22.7 / 40.5 and 29.4.
+// Many rows, trees, one request, 256 rows of 256 / 512 tokens: 22.1 and 15.6 / 22.6 and 17.3; 8 requests: 37.4 and 32.2 / 40.5 and
+// 42.2.
 // Chains in 4 bits are always dealt out, and keep their results.
 constexpr int alone_tokens(bool many, int dim) { return many || dim == 256 ? 256 : 512; }
 
@@ -28,22 +29,26 @@ inline AttnShape attn_shape(int64_t tokens, int heads, int kv_heads, int bits, i
   //   float16: 192 rows 208 and 212, 224 rows 245 and 214, 352 rows 376 and 386, 384 rows 405 and 388;
   //   64 dimensions: bfloat16 128 rows 102 and 105, 160 rows 123 and 106; float16 192 rows 141 and 152, 224 rows 176 and 153;
   //   256 dimensions: 64 rows 179 and 185, 96 rows 293 and 191; float16 64 rows 193 and 277, 96 rows 312 and 282.
-  // So an item costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the card idles
-  // behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
-  // Trees and 8 bits: a last item of half the rows or fewer is told apart, as the waves that have none of them only decode. Trees,
-  // as above, us, few and many: 128 dimensions, bfloat16: 4 bits, 96 rows 115 and 119, 128 rows 129 and 121, 160 rows 169 and 146;
-  // 8 bits, 64 rows 87 and 122, 96 rows 137 and 124; float16: 4 bits, 128 rows 141 and 164, 192 rows 216 and 224, 224 rows 251 and
-  // 228, 320 rows 344 and 409; 64 dimensions, bfloat16: 96 rows 91 and 90, 128 rows 104 and 90; 256 dimensions, bfloat16: 64 rows
-  // 155 and 157, in 8 bits 175 and 167, 96 rows 240 and 203; float16: 64 rows 187 and 232, 96 rows 289 and 280, in 8 bits 96 rows
-  // 357 and 363, 128 rows 402 and 374.
+  // So an item of chains in 4 bits costs as much as 4 (float16 6, 256 dimensions 2) of 32 rows. Where there are few items most of the
+  // card idles behind the first of them: one request of 8,000 tokens, 384 / 512 / 768 rows: 49 / 58 / 75 us and 49 / 58 / 56 us.
+  // Trees, an encoder's states and 8 bits, where the weights of bfloat16 queries have two parts too: a last item of half the rows or
+  // fewer is told apart, as the waves that have none of them only decode. As above, bfloat16, us, few and many:
+  //   128 dimensions: trees in 4 bits 128 rows 128 and 143, 160 rows 167 and 191, 192 rows 191 and 194, 224 rows 227 and 196, 320 rows
+  //   313 and 320, 384 rows 368 and 319; in 8 bits 96 rows 142 and 151, 128 rows 145 and 152, 160 rows 211 and 203, 320 rows 362 and 341;
+  //   states in 4 bits 160 rows 166 and 185, 192 rows 189 and 188; chains in 8 bits 128 rows 133 and 144, 160 rows 206 and 198;
+  //   64 dimensions: trees in 4 bits 128 rows 103 and 106, 160 rows 130 and 144, 192 rows 151 and 147, 320 rows 245 and 240; in 8 bits
+  //   160 rows 137 and 152, 192 rows 155 and 153; states in 4 bits 160 rows 128 and 138, 192 rows 147 and 140;
+  //   256 dimensions: trees in 4 bits 64 rows 162 and 177, 96 rows 243 and 235, 160 rows 389 and 395; in 8 bits 32 rows 124 and 178, 64
+  //   rows 197 and 188, 96 rows 330 and 249.
+  // float16, trees: 128 dimensions in 4 bits, 128 rows 141 and 164, 192 rows 216 and 224, 224 rows 251 and 228, 320 rows 344 and 409;
+  //   256 dimensions: 64 rows 187 and 232, 96 rows 289 and 280, in 8 bits 96 rows 357 and 363, 128 rows 402 and 374.
   const bool f16 = elem_type == SHMT_F16;
-  const int64_t few_items = (rows + 31) / 32, whole = rows / many_rows(dim), rest = rows % many_rows(dim);
-  const int64_t worth = dim == 256 ? 2 + (f16 && bits == 8) : f16 ? 6 : 4;
-  int64_t last = rest > 0 ? worth : 0;  // what the last item is worth
-  if (rest > 0 && rest <= many_rows(dim) / 2 && (bits == 8 || seen != SHMT_SEEN_CAUSAL))
-    last = dim == 256 ? 1 + f16 : f16 ? 4 : bits == 8 && dim == 128 ? 2 : 3;
-  s.many = rows > 2 * many_rows(dim) || (few_items > worth * whole + last && tokens * group * kv_heads >= 16384);
   const bool other = bits == 8 || seen != SHMT_SEEN_CAUSAL;  // than chains in 4 bits
+  const int64_t few_items = (rows + 31) / 32, whole = rows / many_rows(dim), rest = rows % many_rows(dim);
+  const int64_t worth = dim == 256 ? 2 + (f16 && bits == 8) : f16 ? 6 : !other ? 4 : dim == 64 ? 5 : bits == 8 ? 4 : 6;
+  int64_t last = rest > 0 ? worth : 0;  // what the last item is worth
+  if (other && rest > 0 && rest <= many_rows(dim) / 2) last = dim == 256 ? 2 - (!f16 && bits == 8) : 4;
+  s.many = rows > 2 * many_rows(dim) || (few_items > worth * whole + last && tokens * group * kv_heads >= 16384);
   auto few_groups = [&](int rows_of_item) { return int64_t{256} * attn_waves(bits, seen, f16, dim, rows_of_item / 16); };
   s.alone = other && limit >= 0 && limit <= alone_tokens(s.many, dim);
   s.rows = s.many ? many_rows(dim) : rows <= 16 ? 16 : 32;

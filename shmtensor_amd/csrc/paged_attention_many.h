@@ -53,10 +53,11 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // each, into LDS as bfloat16 fragments of the two products (a kilobyte each, lane by lane, so that reading and writing them is
 // free of bank conflicts), and each multiplies its own rows with all of it. While a tile is multiplied the next one is
 // decoded into the other half of the LDS and the one behind it is on its way from memory; a tile costs one barrier.
-// The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them. Only
-// that the weights of bfloat16 queries are rounded to one bfloat16 here, an error of the size of the result's own rounding
-// (2.3e-3 in all instead of 1.66e-3): in two parts the prompts below take 1.36 ms instead of 1.06, with 64 dimensions 1.00
-// instead of 0.79.
+// The products are those of the kernel for few rows: S^T = K Q^T leaves the weights where O^T += V^T P^T wants them. For chains in
+// 4 bits the weights of bfloat16 queries are rounded to one bfloat16, an error of the size of the result's own rounding (2.3e-3 in
+// all instead of 1.66e-3): in two parts the prompts below take 1.36 ms instead of 1.06, with 64 dimensions 1.00 instead of 0.79.
+// For all else they have two parts as in the kernel for few rows, and both kernels are as near to the definition (1.66e-3): the
+// trees below take 275 us so and 226 in one part, the answers 91 and 76, two prompts of 8,192 in 8 bits 1.48 ms and 1.17.
 // Bound by what the vector units and the matrix cores have to issue: for 64 tokens a wave has 64 products, of which each keeps
 // the vector units from about 9 of its 16 cycles (measured with one wave of each kind on a SIMD), and some 200 vector
 // instructions, two thirds of them the softmax. Two prompts of 8,192 tokens, 32 query and 8 key heads of 128, bfloat16: 1.06
@@ -71,9 +72,9 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // has room for. They read it twice as often but wait less: two prompts of 4,096 tokens, other sizes as above, 0.80 ms (0.76
 // now, 710 TFLOP/s) against 1.02 with four waves of 32 rows and tiles of 32 tokens and 0.95 with eight and 32; chunks of 17 to
 // 2,000 tokens behind a window 87 us against 95 and 92.
-// Trees of 24 to 64 nodes, four heads to one of the cache's, behind 1,000 to 12,000 tokens, 40 requests: 226 us; what is lost there
+// Trees of 24 to 64 nodes, four heads to one of the cache's, behind 1,000 to 12,000 tokens, 40 requests: 275 us; what is lost there
 // are waves without rows and the ends of items, 8 us each. 6 answers of 100 to 1,200 tokens over an encoder's 700 to 5,000
-// states in 8 bits: 76 us, 43 of them in the tiles.
+// states in 8 bits: 91 us, 58 of them in the tiles.
 template <int BITS, int DIM>
 struct ManyShape {
   static constexpr int kTile = DIM == 256 ? 64 : 128;  // tokens
@@ -110,6 +111,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
   constexpr int kParts = std::is_same<T, _Float16>::value ? 2 : 1;
   constexpr int kSub = kUnit / kTile;  // tiles of a unit
   constexpr bool kOther = BITS == 8 || SEEN != SHMT_SEEN_CAUSAL;  // than chains in 4 bits
+  constexpr int kWeightParts = kOther ? 2 : kParts;
   __shared__ ManyStage<BITS, DIM> stage[2];
   __shared__ Found found;
   __shared__ uint64_t scan[Shape::kWaves];
@@ -267,8 +269,8 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
     }
     const int sinks = a.window > 0 ? a.sinks : 0;
     // Waves without a row only decode: of up to 128 rows the first four multiply, one on each SIMD. (16 rows to a wave in turn, so
-    // that the SIMDs share what there is, brought 8 % for 160 and 192 rows of bfloat16 and lost 5 to 9 % for 128 and 256; chains
-    // in 4 bits lose 2 % by the question itself, two prompts 1,071 us instead of 1,050.)
+    // that the SIMDs share what there is, brought 8 % for 160 and 192 rows of bfloat16 and lost 5 to 9 % for 128 and 256,
+    // with weights in one part; chains in 4 bits lose 2 % by the question itself, two prompts 1,071 us instead of 1,050.)
     const bool has_rows = !kOther || 16 * wave * NT < rows;
     // the first and the last place of the wave's rows, and of the item's
     const int r_first = min(16 * wave * NT, rows - 1), r_last = min(16 * (wave + 1) * NT - 1, rows - 1);
@@ -465,9 +467,9 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
           if (pass < kMaximum) waiting = first_reference<NT>(x, unit, st, again, far_any);
           else round_scores<NT>(x, powers_of_two(a), st, pass);
         }
-        u32x4 w[kParts][NT];
+        u32x4 w[kWeightParts][NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) weights<kParts>(x[n], unit, st.top[n], st.sum[n], w, n);
+        for (int n = 0; n < NT; ++n) weights<kWeightParts>(x[n], unit, st.top[n], st.sum[n], w, n);
         raise_reference<NT>(st, again, far_any);
         if (group + 1 < Shape::kGroups) read_keys(group + 1);
 #pragma unroll
@@ -475,7 +477,7 @@ __global__ __launch_bounds__((ManyShape<BITS, DIM>::kThreads), 2) void page_atte
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) st.acc[n][i] = mfma(values[i], w[p][n], st.acc[n][i]);
+            for (int p = 0; p < kWeightParts; ++p) st.acc[n][i] = mfma(values[i], w[p][n], st.acc[n][i]);
       }
     };
 
