@@ -772,7 +772,7 @@ int shmt_page_tree(const int32_t *parents, const void *query_starts,
  * are not touched; where a place or a row has no page, nothing is copied. The
  * request holds kv_lens[b] - n + counts[b] tokens then, at positions without a
  * gap. Requests must not share pages that are written. cache->cache and
- * cache->scales are the first layer's.                                      */
+ * cache->scales are the first layer's. requests < 2^24 (page_tree takes more). */
 int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers,
                    int64_t cache_layer_stride, int64_t scales_layer_stride,
                    const int32_t *block_table, int64_t width,

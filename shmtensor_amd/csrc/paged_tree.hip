@@ -420,6 +420,7 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers, int6
                "layers overlap");
   SHMT_REQUIRE(rows >= 0 && rows < (int64_t{1} << 30), "the number of nodes must be in [0, 2^30)");
   SHMT_REQUIRE(requests >= 0 && requests < (int64_t{1} << 31), "the number of requests must be in [0, 2^31)");
+  SHMT_REQUIRE(requests < (int64_t{1} << 24), "too many requests in one call: 2^24 or more");  // a workgroup each
   SHMT_REQUIRE(width >= 0 && width <= (int64_t{1} << 30) / cache->page,
                "the block table holds too many tokens: more than 2^30 a request");
   SHMT_REQUIRE(width_ok(len_bytes), "query_starts and kv_lens can only be int32 or int64");
@@ -436,7 +437,6 @@ int shmt_page_keep(const shmt_paged_cache *cache, int bits, int64_t layers, int6
   const int64_t tiles = layers * cache->kv_heads * 2;
   a.splits = static_cast<int>(std::max<int64_t>(1, std::min((tiles + 15) / 16, 1024 / std::max<int64_t>(requests, 1))));
   const int64_t groups = std::max<int64_t>(requests, 1) * a.splits;
-  SHMT_REQUIRE(groups < (int64_t{1} << 24), "too many requests in one call");
   hipLaunchKernelGGL(page_keep_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, as_stream(stream), a);
   SHMT_LAUNCH_CHECK();
   return SHMT_OK;

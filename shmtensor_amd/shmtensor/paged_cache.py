@@ -104,6 +104,8 @@ class PagedCache:
         if need > self.free_pages:
             raise RuntimeError("%d pages needed, %d free" % (need, self.free_pages))
         if parents is not None:
+            if len(new) >= 1 << 24:
+                raise ValueError("a step over trees has less than 2^24 requests, as keep() does")
             parents = torch.as_tensor(parents, dtype=torch.int32)
             if parents.shape != (int(new.sum()),):
                 raise ValueError("parents must hold an entry for each of %d new tokens" % new.sum())

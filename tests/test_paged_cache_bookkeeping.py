@@ -149,3 +149,12 @@ def test_requests_counted_from_the_end(host_cache):
         with pytest.raises(IndexError):
             cache.trim(wrong, window=1)
     _in_order(cache, [41, 17, 30])
+
+
+def test_more_requests_than_a_step_over_trees_may_have(host_cache):
+    """Refused before the step, not at its end."""
+    cache = host_cache(requests=1 << 24, max_len=16)
+    new = np.zeros(1 << 24, np.int64)
+    with pytest.raises(ValueError, match="2\\^24"):
+        cache.plan(new, parents=[])
+    assert cache.free_pages == 40 and not cache.lens.any()

@@ -112,3 +112,10 @@ def test_operators_refuse_tensors_that_are_not_on_the_gpu(capi):
     cache = torch.zeros((1, 2, 1, 2, 16, 64), dtype=torch.uint8).view(torch.float8_e4m3fn)
     with pytest.raises(RuntimeError, match="CUDA"):
         capi.page_keep(cache, torch.zeros((1, 2, 1, 2, 2, 16), dtype=torch.uint8), ints[None], ints, ints[:2], ints, ints, ints)
+
+
+def test_requests_of_a_step_over_trees(cabi):
+    """page_keep has a workgroup for each request, so 2^24 of them are too many; the header says so."""
+    view = _view(cabi)
+    rc = cabi.load().shmt_page_keep(ctypes.byref(view), 4, 1, 0, 0, A, 3, 3, A, A, 4, 1 << 24, 5, A, A, A, 8, None, A, A, A, None)
+    _refused(cabi, rc, "2^24 or more")
