@@ -853,7 +853,8 @@ struct AttnShape {
 constexpr int many_rows(int dim) { return dim == 256 ? 128 : 256; }
 
 // Waves per SIMD that the registers of the kernel for few rows are meant for. Trees and 8 bits take more registers, and fewer waves
-// that spill none are quicker (and leave fewer parts); so are they for an encoder's states. us with one wave more a SIMD and as it
+// are quicker (and leave fewer parts), as they spill next to none: trees of float16, 128 dimensions, 32 rows 9 vector registers in 8
+// bits and 7 in 4, of bfloat16, 256 dimensions, 16 rows 8 and 4, others at most 3. So are they for an encoder's states. us with one wave more a SIMD and as it
 // is, 16 requests of 8,000 tokens, 8 heads, 16 rows: trees in 4 bits, 64 dimensions bfloat16 36 and 30, 128 dimensions 40 and 35,
 // float16 46 and 36; in 8 bits, 64 dimensions float16 43 and 34, 128 dimensions 66 and 54, 256 dimensions 141 and 114 (bfloat16
 // 115 with one wave, 119 with two, but 59 and 57 where requests are short); 32 rows of 256 dimensions 144 and 116.

@@ -9,9 +9,9 @@
 // 16,000 tokens 85 us, 4.4 TB/s; one request of 130,000 tokens with float16 queries 46 us, 3.1 TB/s, of which the join 7 us.
 // At 64 dimensions half the bytes come with the same softmax, and the vector units are what it waits for: 96 requests with a
 // window of 4,000 tokens, float16, 66 us, 3.1 TB/s (some 230 vector instructions for 32 tokens of a wave).
-// In 8 bits twice the bytes come with the same softmax: 64 ragged requests as above 143 us, 5.2 TB/s. With more than 16 rows it is
-// issue again: a tree of 65 rows behind 100,000 tokens in 8 bits, float16, 120 us, 363 vector instructions for 32 tokens and 32
-// rows of a wave. Over an encoder's states, 80 requests of 300 to 1,500, 5 rows each, 16 heads of 64, 37 us, of which the join 5.
+// In 8 bits twice the bytes come with the same softmax: 64 ragged requests as above 143 us, 5.2 TB/s. More
+// than 32 rows read the cache once for each 32: a tree of 65 rows behind 100,000 tokens in 8 bits, float16, 120 us, in which 651 MB
+// come from HBM (counted; the cache has 211), 6.0 TB/s, with vector units at 46 % and matrix cores at 30 % of the time. Over an encoder's states, 80 requests of 300 to 1,500, 5 rows each, 16 heads of 64, 37 us, of which the join 5.
 #pragma once
 #include "paged_attention.h"
 

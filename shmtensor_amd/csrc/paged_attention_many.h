@@ -74,7 +74,8 @@ __global__ __launch_bounds__(1024) void page_attention_items_kernel(AttnArgs a, 
 // 2,000 tokens behind a window 87 us against 95 and 92.
 // Trees of 24 to 64 nodes, four heads to one of the cache's, behind 1,000 to 12,000 tokens, 40 requests: 275 us; what is lost there
 // are waves without rows and the ends of items, 8 us each. 6 answers of 100 to 1,200 tokens over an encoder's 700 to 5,000
-// states in 8 bits: 91 us, 58 of them in the tiles.
+// states in 8 bits: 91 us, 58 of them in the tiles. At 128 dimensions bfloat16 spills 22 vector registers for trees and 4 to 6 for
+// states and 8 bits (chains in 4 bits none), float16 28 to 67 (24); at 256 dimensions 11 to 27 (12), float16 34 to 70 (36); at 64 none.
 template <int BITS, int DIM>
 struct ManyShape {
   static constexpr int kTile = DIM == 256 ? 64 : 128;  // tokens
